@@ -17,6 +17,7 @@ from dionw_amd._keys import (
     ROUTE_KEY,
     ROW_NORMALIZATION_KEY,
 )
+from dionw_amd._adamw_8bit import AdamWState
 from dionw_amd.ema import EMAConfig, EMADevice, EMASchedule, IntegratedEMAOptimizer
 from dionw_amd.matrix_update import (
     DION3_UPDATE,
@@ -47,6 +48,7 @@ __all__ = [
     "NUM_HEADS_KEY",
     "ROUTE_KEY",
     "ROW_NORMALIZATION_KEY",
+    "AdamWState",
     "Dion",
     "EMAConfig",
     "EMADevice",

@@ -27,7 +27,9 @@ from typing import Any, Final
 import torch
 from torch import Tensor
 
+from dionw_amd._adamw_8bit import AdamWState
 from dionw_amd._keys import (
+    ADAMW_STATE_KEY,
     FRACTION_KEY,
     MOMENTUM_FORM_KEY,
     NEWTON_SCHULZ_KEY,
@@ -115,6 +117,7 @@ class GroupSpec:
         newton_schulz: The orthogonalization.
         row_normalization: NorMuon or none.
         momentum_form: Heavy ball or Nesterov.
+        adamw_state: How the moments are held (ADAMW).
     """
 
     kind: RouteKind
@@ -123,6 +126,7 @@ class GroupSpec:
     newton_schulz: NewtonSchulz
     row_normalization: RowNormalization
     momentum_form: MomentumForm
+    adamw_state: AdamWState = AdamWState.FLOAT32
 
     @classmethod
     def of(cls, group: Mapping[str, Any]) -> GroupSpec:
@@ -147,6 +151,7 @@ class GroupSpec:
             newton_schulz=NewtonSchulz(group[NEWTON_SCHULZ_KEY]),
             row_normalization=RowNormalization(group[ROW_NORMALIZATION_KEY]),
             momentum_form=MomentumForm(group[MOMENTUM_FORM_KEY]),
+            adamw_state=AdamWState(group.get(ADAMW_STATE_KEY, AdamWState.FLOAT32.value)),
         )
         if spec.kind is RouteKind.MATRIX:
             spec._check_matrix(group["params"])
@@ -190,4 +195,10 @@ def refuse_structural_change(saved: Sequence[Mapping[str, Any]],
                 raise ValueError(
                     f"param group {index} {key!r} differs: checkpoint {old[key]!r}, optimizer "
                     f"{new[key]!r}; build the groups as they were built for the checkpoint")
+        # Groups without the key hold float32 moments; matrix groups hold none.
+        states = [g.get(ADAMW_STATE_KEY, AdamWState.FLOAT32.value) for g in (old, new)]
+        if new[ROUTE_KEY] == RouteKind.ADAMW.value and states[0] != states[1]:
+            raise ValueError(
+                f"param group {index} {ADAMW_STATE_KEY!r} differs: checkpoint {states[0]!r}, "
+                f"optimizer {states[1]!r}; build the groups as they were built for the checkpoint")
     return completed

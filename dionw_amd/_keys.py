@@ -25,6 +25,9 @@ MUON_BETA2_KEY: Final = "muon_beta2"             # NorMuon second-moment decay
 ROW_NORMALIZATION_KEY: Final = "row_normalization"  # a RowNormalization value
 MOMENTUM_FORM_KEY: Final = "momentum_form"       # a MomentumForm value
 
+# Not in the reference, and present only in groups that ask for it: an AdamWState value.
+ADAMW_STATE_KEY: Final = "adamw_state"
+
 # Fixed when the groups are built; load_state_dict refuses a change.
 STRUCTURAL_KEYS: Final = (
     ROUTE_KEY,
@@ -40,12 +43,21 @@ MOMENTUM_STATE: Final = "momentum"
 VARIANCE_STATE: Final = "variance"
 EXP_AVG_STATE: Final = "exp_avg"
 EXP_AVG_SQ_STATE: Final = "exp_avg_sq"
+# 8-bit AdamW state (not in the reference): the scales of exp_avg, and the codes and scales
+# of the root of the second moment, which take exp_avg_sq's place.
+EXP_AVG_SCALE_STATE: Final = "exp_avg_scale"
+EXP_AVG_RMS_STATE: Final = "exp_avg_rms"
+EXP_AVG_RMS_SCALE_STATE: Final = "exp_avg_rms_scale"
 # Not "step": torch's loader would move a "step" entry to the CPU, and this
 # counter must stay a device scalar so that a step never synchronizes.
 ADAMW_STEP_STATE: Final = "adamw_step"
 
 __all__ = [
+    "ADAMW_STATE_KEY",
     "ADAMW_STEP_STATE",
+    "EXP_AVG_RMS_SCALE_STATE",
+    "EXP_AVG_RMS_STATE",
+    "EXP_AVG_SCALE_STATE",
     "EXP_AVG_SQ_STATE",
     "EXP_AVG_STATE",
     "FRACTION_KEY",

@@ -115,6 +115,14 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         ctypes.c_int,
         [_pp, _pp, _pp, _pp, _pp, _pp, _pi64, _i32, _f64, _f64, _f64, _f64, _f64, _f32, _p],
     ),
+    "dionw_adamw_8bit": (
+        ctypes.c_int,
+        [_pp, _pp, _pp, _pi64, _pi64, _pi32, _i32, _i64, _i32, _p, _p, _p, _p, _p, _p, _f64, _f64,
+         _f64, _f64, _f64, _f32, _p],
+    ),
+    "dionw_adamw_8bit_values": (
+        ctypes.c_int, [_pi64, _pi64, _i32, _i64, _p, _p, _p, _p, _p, _p, _p],
+    ),
     "dionw_ema_update": (ctypes.c_int, [_pp, _pp, _pi64, _i32, _f32, _i32, _p]),
 }
 

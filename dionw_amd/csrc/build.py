@@ -16,7 +16,8 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 PACKAGE = HERE.parent
 LIBRARY = PACKAGE / "libdionw_hip.so"
-SOURCES = ("errors.cpp", "momentum.hip", "select.hip", "normuon.hip", "adamw_ema.hip", "gemm.hip")
+SOURCES = ("errors.cpp", "momentum.hip", "select.hip", "normuon.hip", "adamw_ema.hip",
+           "adamw_8bit.hip", "gemm.hip")
 ARCH = "gfx950"
 FLAGS = (
     f"--offload-arch={ARCH}",

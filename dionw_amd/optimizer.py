@@ -30,9 +30,11 @@ from torch import Tensor
 
 from dionw_amd import _workspace
 from dionw_amd._adamw import adamw_step, init_adamw_state
+from dionw_amd._adamw_8bit import AdamWPack, AdamWState, adamw_8bit_step, pack_adamw
 from dionw_amd._buckets import Bucket, pack_buckets
 from dionw_amd._groups import GroupSpec, check_decays, check_parameter, refuse_structural_change
 from dionw_amd._keys import (
+    ADAMW_STATE_KEY,
     EXP_AVG_STATE,
     FRACTION_KEY,
     MOMENTUM_FORM_KEY,
@@ -116,8 +118,13 @@ class Dion(IntegratedEMAOptimizer):
         matrix_update: MatrixUpdate = DION3_UPDATE,
         ema: EMAConfig | None = None,
         profile_region: ProfileRegion = no_profile,
+        adamw_state: AdamWState = AdamWState.FLOAT32,
     ) -> None:
         """Create the optimizer.
+
+        ``adamw_state`` (not in the reference) is how AdamW groups hold their moments:
+        ``AdamWState.EIGHT_BIT`` takes a quarter of the memory. A group's own
+        ``"adamw_state"`` entry overrides it.
 
         Raises:
             TypeError: For a group without a route, or parameters that are not float32.
@@ -128,6 +135,10 @@ class Dion(IntegratedEMAOptimizer):
                      decays={MOMENTUM_KEY: momentum, MUON_BETA2_KEY: muon_beta2,
                              "beta1": betas[0], "beta2": betas[1]})
         self._packed: list[Bucket] | None = None
+        self._adamw_packs: dict[int, list[AdamWPack]] = {}  # by group: the 8-bit ones
+        # The key is left out where nothing asks for it, so that checkpoints stay the reference's.
+        more = ({} if adamw_state is AdamWState.FLOAT32
+                else {ADAMW_STATE_KEY: AdamWState(adamw_state).value})
         super().__init__(params, {
             "lr": lr,
             "betas": betas,
@@ -140,6 +151,7 @@ class Dion(IntegratedEMAOptimizer):
             NEWTON_SCHULZ_KEY: matrix_update.newton_schulz.value,
             ROW_NORMALIZATION_KEY: matrix_update.row_normalization.value,
             MOMENTUM_FORM_KEY: matrix_update.momentum_form.value,
+            **more,
         })
         self._profile_region = profile_region
         self._init_integrated_ema(ema, profile_region)
@@ -173,6 +185,9 @@ class Dion(IntegratedEMAOptimizer):
         # With AdamW state present from the start, an integrated EMA tracks
         # every parameter; matrix state appears with the buckets.
         if spec.kind is RouteKind.ADAMW:
+            if spec.adamw_state is AdamWState.EIGHT_BIT:
+                self._adamw_packs[len(self.param_groups) - 1] = pack_adamw(params, self.state)
+                return
             for param in params:
                 init_adamw_state(param, self.state[param])
 
@@ -202,6 +217,43 @@ class Dion(IntegratedEMAOptimizer):
         groups = refuse_structural_change(state_dict["param_groups"], self.param_groups)
         super().load_state_dict({**state_dict, "param_groups": groups})
         self._repack()
+        for packs in self._adamw_packs.values():
+            for pack in packs:
+                pack.adopt(self.state)
+
+    def adamw_moments(self, params: Iterable[Tensor]) -> tuple[Tensor, Tensor]:
+        """The moments that 8-bit AdamW state stands for (not in the reference).
+
+        Returns:
+            Two float32 vectors, the tensors' elements one after another in row-major
+            order: the first moment and the root of the second.
+
+        Raises:
+            ValueError: Without a parameter, for one that no 8-bit AdamW group of this
+                optimizer holds, or for parameters of several devices.
+        """
+        held = {id(p): (pack, place) for packs in self._adamw_packs.values() for pack in packs
+                for place, p in enumerate(pack.params)}
+        params = list(params)
+        if not params or any(id(p) not in held for p in params):
+            raise ValueError("adamw_moments takes parameters of this optimizer's 8-bit AdamW "
+                             f"groups ({ADAMW_STATE_KEY!r}: {AdamWState.EIGHT_BIT.value!r})")
+        device = params[0].device
+        if any(p.device != device for p in params):
+            raise ValueError("adamw_moments takes parameters of one device")
+        total = sum(p.numel() for p in params)
+        exp_avg, rms = torch.empty(total, device=device), torch.empty(total, device=device)
+        at = start = 0
+        while start < len(params):
+            pack, places, size = held[id(params[start])][0], [], 0
+            while start < len(params) and held[id(params[start])][0] is pack:
+                places.append(held[id(params[start])][1])
+                size += params[start].numel()
+                start += 1
+            if size:
+                pack.moments(places, exp_avg[at:at + size], rms[at:at + size])
+            at += size
+        return exp_avg, rms
 
     def _buckets(self) -> list[Bucket]:
         if self._packed is None:
@@ -258,7 +310,11 @@ class Dion(IntegratedEMAOptimizer):
                                 if g[ROUTE_KEY] == RouteKind.ADAMW.value]
                 if adamw_groups:
                     with region(ADAMW_REGION):
-                        for group in adamw_groups:
-                            adamw_step(group, self.state)
+                        for index, group in enumerate(self.param_groups):
+                            if index in self._adamw_packs:
+                                for pack in self._adamw_packs[index]:
+                                    adamw_8bit_step(group, pack)
+                            elif group[ROUTE_KEY] == RouteKind.ADAMW.value:
+                                adamw_step(group, self.state)
         return loss
 

@@ -310,6 +310,33 @@ int dionw_adamw_ema(float* const* params, const float* const* grads, float* cons
                     double weight_decay, double eps, float ema_weight, dionw_stream_t stream);
 
 /*
+ * Multi-tensor AdamW with the moments in 8 bits (not in the reference). The state of
+ * `tensors` tensors lies in shared arrays of `blocks` blocks of 256 elements: exp_avg
+ * (e4m3 bytes) and rms (the root of the second moment: unsigned bytes of 4 exponent bits,
+ * bias 8, and 4 fraction bits), 256 a block, and one float32 power of two a block in
+ * exp_avg_scale and rms_scale. Tensor i of the call has numels[i] contiguous elements, its
+ * blocks from first_blocks[i] on and its step at steps[ids[i]]. No two tensors of a call may
+ * share blocks or an id. Increments the steps, then
+ *   m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * and stores m and sqrt(v) rounded stochastically by a hash of (step, id, element).
+ * shadows (may be NULL): EMA shadows, lerped towards the new parameters by ema_weight.
+ * scalars: float32 scratch, 4 for each of the `tensors`.
+ */
+int dionw_adamw_8bit(float* const* params, const float* const* grads, float* const* shadows,
+                     const int64_t* numels, const int64_t* first_blocks, const int32_t* ids,
+                     int32_t count, int64_t blocks, int32_t tensors, void* exp_avg,
+                     float* exp_avg_scale, void* rms, float* rms_scale, float* steps,
+                     float* scalars, double lr, double beta1, double beta2, double weight_decay,
+                     double eps, float ema_weight, dionw_stream_t stream);
+
+/* The float32 values of that state for `count` tensors, one after another in the outputs. */
+int dionw_adamw_8bit_values(const int64_t* numels, const int64_t* first_blocks, int32_t count,
+                            int64_t blocks, const void* exp_avg, const float* exp_avg_scale,
+                            const void* rms, const float* rms_scale, float* exp_avg_out,
+                            float* rms_out, dionw_stream_t stream);
+
+/*
  * GPU EMA of float32 sources: shadow = lerp(shadow, source, weight), or a
  * copy when copy != 0. Replaces foreach_ema_update_ (ema/_update.py:32-70)
  * and the first-update _foreach_copy_ (ema/tracker.py:142-145).
