@@ -19,6 +19,13 @@ from dionw_amd._keys import (
 )
 from dionw_amd._adamw_8bit import AdamWState
 from dionw_amd.ema import EMAConfig, EMADevice, EMASchedule, IntegratedEMAOptimizer
+from dionw_amd.float8 import (
+    Float8Linear,
+    Float8Matrix,
+    float8_linear,
+    float8_matmul,
+    float8_quantize,
+)
 from dionw_amd.matrix_update import (
     DION3_UPDATE,
     MUON_UPDATE,
@@ -53,6 +60,8 @@ __all__ = [
     "EMAConfig",
     "EMADevice",
     "EMASchedule",
+    "Float8Linear",
+    "Float8Matrix",
     "IntegratedEMAOptimizer",
     "MatrixUpdate",
     "MomentumForm",
@@ -66,5 +75,8 @@ __all__ = [
     "RoutingReport",
     "RowNormalization",
     "__version__",
+    "float8_linear",
+    "float8_matmul",
+    "float8_quantize",
     "param_groups",
 ]

@@ -123,6 +123,15 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "dionw_adamw_8bit_values": (
         ctypes.c_int, [_pi64, _pi64, _i32, _i64, _p, _p, _p, _p, _p, _p, _p],
     ),
+    "dionw_float8_quantize": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p],
+    ),
+    "dionw_sum_parts": (ctypes.c_int, [_p, _i64, _i64, _i32, _p, _p]),
+    "dionw_float8_gemm": (
+        ctypes.c_int,
+        [_i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _p],
+    ),
     "dionw_ema_update": (ctypes.c_int, [_pp, _pp, _pi64, _i32, _f32, _i32, _p]),
 }
 

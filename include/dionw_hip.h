@@ -337,6 +337,37 @@ int dionw_adamw_8bit_values(const int64_t* numels, const int64_t* first_blocks, 
                             float* rms_out, dionw_stream_t stream);
 
 /*
+ * 8-bit matrices (not in the reference). A quantized matrix [rows, cols] is e4m3 codes
+ * [rows][data_ld] (data_ld a multiple of 16, at least cols rounded up to 128; 16-byte aligned;
+ * the columns up to that multiple of 128 hold zeros) and the exponent bytes of float32 powers
+ * of two [blocks of 128 columns][scale_ld], scale_ld >= rows.
+ *
+ * dionw_float8_quantize rounds x [rows, cols] (row pitch ld, element code elem) to nearest:
+ * into data/scale by rows, and into data_t/scale_t as the transpose [cols, rows]; either may
+ * be NULL. One scale for each row (of the transpose: column of x) and block of 128, or for
+ * each 128 x 128 tile when tiles != 0. Values that are not finite become NaN and leave their
+ * block's scale alone. sums (may be NULL): float32 [ceil(rows / 128)][cols], the column sums
+ * of each 128 rows.
+ */
+int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
+                          int32_t tiles, void* data, int64_t data_ld, void* scale,
+                          int64_t scale_ld, void* data_t, int64_t data_t_ld, void* scale_t,
+                          int64_t scale_t_ld, float* sums, dionw_stream_t stream);
+
+/* out[c] = parts[0][c] + parts[1][c] + ... in order, in element code elem. */
+int dionw_sum_parts(const float* parts, int64_t count, int64_t cols, int32_t elem, void* out,
+                    dionw_stream_t stream);
+
+/*
+ * C [m, n] = A B^T + bias for quantized A [m, depth] and B [n, depth] (depth: a multiple of
+ * 128), summed in float32 and rounded once to element code elem; bias: n floats or NULL.
+ */
+int dionw_float8_gemm(int64_t m, int64_t n, int64_t depth, const void* a, int64_t lda,
+                      const void* a_scale, int64_t a_scale_ld, const void* b, int64_t ldb,
+                      const void* b_scale, int64_t b_scale_ld, const float* bias, int32_t elem,
+                      void* c, int64_t ldc, dionw_stream_t stream);
+
+/*
  * GPU EMA of float32 sources: shadow = lerp(shadow, source, weight), or a
  * copy when copy != 0. Replaces foreach_ema_update_ (ema/_update.py:32-70)
  * and the first-update _foreach_copy_ (ema/tracker.py:142-145).
