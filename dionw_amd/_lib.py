@@ -125,12 +125,15 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     ),
     "dionw_float8_quantize": (
         ctypes.c_int,
-        [_i32, _p, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p],
+        [_i32, _p, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p],
     ),
+    "dionw_float8_expand": (ctypes.c_int, [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "dionw_float8_gemm_workspace": (ctypes.c_size_t, [_i32, _i64, _i64, _i64]),
     "dionw_sum_parts": (ctypes.c_int, [_p, _i64, _i64, _i32, _p, _p]),
     "dionw_float8_gemm": (
         ctypes.c_int,
-        [_i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _p],
+        [_i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _p,
+         ctypes.c_size_t, _p],
     ),
     "dionw_ema_update": (ctypes.c_int, [_pp, _pp, _pi64, _i32, _f32, _i32, _p]),
 }

@@ -9,57 +9,12 @@
 // accumulation in float32 from the first block to the last. Bytes are kept by column block,
 // [blocks][rows], so that the rows of a tile lie side by side.
 //
-// Products run on one of two instructions, by their output's type:
-// - float16 and bfloat16: v_mfma_scale_f32_16x16x128_f8f6f4, one block deep, scales
-//   included, at twice the 16-bit rate. It adds groups of 8 products after cutting each to
-//   13 bits below the exponent of the group's largest (measured: beside 2^16, 2^3 counts and
-//   2^2 does not), and adds the groups in float32. On normal random operands the result is
-//   1.3e-5 off (2-norm), on log-normal ones 6e-5: below the output's rounding (2e-4, 2e-3).
-// - float32: v_mfma_f32_16x16x32_bf16 on codes expanded to bfloat16, scale included, which is
-//   exact: 3e-8 off, the accumulation's own rounding. Weight gradients and whatever else asks
-//   for float32 sums get them.
-//
 // A weight's bytes are equal within each 128 x 128 tile, so that its transpose holds the
 // same values; an activation's differ from row to row.
-#include "common.h"
-
-#include <algorithm>
-#include <mutex>
+#include "float8.h"
 
 namespace dionw {
 namespace {
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-constexpr int kTile = 128;  // columns (and rows) that share a scale
-
-// The scale's exponent byte of a block whose largest finite magnitude has the bits `largest`
-// (at least 1: the scale and its reciprocal are normal).
-__device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
-  const uint32_t field = (largest + 0x1FFFFFu) >> 23;  // fractions above 1.75 carry
-  return field > 8u ? field - 8u : 1u;
-}
-__device__ __forceinline__ float power(uint32_t byte) { return __uint_as_float(byte << 23); }
-
-// The bits of |v|, 0 where it is not finite (such values become NaN codes and leave the
-// block's scale alone).
-__device__ __forceinline__ uint32_t magnitude(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? b : 0u;
-}
-
-// Four codes of four values, rounded to nearest even; infinities become NaN.
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float inv) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
-}
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
-__device__ __forceinline__ float to_float(__bf16 v) { return (float)v; }
 
 // ---- quantization ------------------------------------------------------------------
 //
@@ -74,13 +29,14 @@ struct QuantizeArgs {
   int64_t data_ld;
   uint8_t* scale;     // [blocks][scale_ld]
   int64_t scale_ld;
-  uint8_t* data_t;    // the transpose: [cols][data_t_ld] or null
+  uint8_t* data_t;    // the transpose: [cols][data_t_ld bytes] or null
   int64_t data_t_ld;
   uint8_t* scale_t;
   int64_t scale_t_ld;
   float* sums;        // [row tiles][cols]: each tile's column sums, or null
   int32_t tiles_c;
   int32_t vec;        // rows start at multiples of 16 bytes
+  int32_t expand_t;   // the transpose in bfloat16, scales included
 };
 
 template <typename T, bool TILES>
@@ -206,7 +162,18 @@ __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
   __syncthreads();
   if (q.data && tid < kTile && r0 + tid < q.scale_ld)
     q.scale[c0 / kTile * q.scale_ld + r0 + tid] = row_bytes[tid];
-  if (q.data_t) {
+  if (q.data_t && q.expand_t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = j * 32 + tid / 8, at = tid % 8 * 16;
+      if (c0 + c >= q.cols) continue;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(turned + c * kPitch + at);
+      const float scale = half_power(col_bytes[c]);
+      bf16x8* out = reinterpret_cast<bf16x8*>(q.data_t + (c0 + c) * q.data_t_ld + 2 * (r0 + at));
+      out[0] = expand(w[0], w[1], scale);
+      out[1] = expand(w[2], w[3], scale);
+    }
+  } else if (q.data_t) {
     if (tid < kTile && c0 + tid < q.scale_t_ld)
       q.scale_t[r0 / kTile * q.scale_t_ld + c0 + tid] = col_bytes[tid];
 #pragma unroll
@@ -217,6 +184,21 @@ __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
             *reinterpret_cast<const u32x4*>(turned + c * kPitch + at);
     }
   }
+}
+
+// Codes to bfloat16 halves of their values, 16 a thread.
+__global__ __launch_bounds__(256) void float8_expand_kernel(const uint8_t* data, int64_t data_ld,
+                                                            const uint8_t* scale, int64_t scale_ld,
+                                                            int64_t rows, int64_t chunks,
+                                                            __bf16* out, int64_t out_ld) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / chunks, c = (at - row * chunks) * 16;
+  if (row >= rows) return;
+  const u32x4 w = *reinterpret_cast<const u32x4*>(data + row * data_ld + c);
+  const float s = half_power(scale[c / kTile * scale_ld + row]);
+  bf16x8* to = reinterpret_cast<bf16x8*>(out + row * out_ld + c);
+  to[0] = expand(w[0], w[1], s);
+  to[1] = expand(w[2], w[3], s);
 }
 
 // out[c] = the parts' sums in order.
@@ -239,109 +221,6 @@ int launch_quantize(const QuantizeArgs& q, bool tiles, unsigned grid, hipStream_
   return check_launch("float8_quantize");
 }
 
-// ---- products ------------------------------------------------------------------------
-
-struct ProductArgs {
-  const uint8_t* a;
-  int64_t lda;
-  const uint8_t* a_scale;
-  int64_t a_scale_ld;
-  const uint8_t* b;
-  int64_t ldb;
-  const uint8_t* b_scale;
-  int64_t b_scale_ld;
-  const float* bias;
-  void* c;
-  int64_t ldc;
-  int64_t m, n;
-  int32_t blocks;  // of 128 columns
-  int32_t tiles_n;
-};
-
-// The scaled product of a fragment: 16 rows of each operand over one block. Either operand's
-// lane i holds row i % 16 and the 32 bytes of its place i / 16 in the block; any order of the
-// block's bytes serves that both share. D: lane i holds rows 4 (i / 16) .. + 3 of the first
-// operand against row i % 16 of the second.
-__device__ __forceinline__ f32x4 mfma(i32x8 a, i32x8 b, f32x4 c, int a_byte, int b_byte) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, a_byte, 0, b_byte);
-}
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
-// Eight codes and their scale as bfloat16, exactly (a code has 4 significant bits).
-__device__ __forceinline__ bf16x8 expand(int lo, int hi, float scale) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-  return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3),
-                                 __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// The scale that a row's codes are expanded with: half of theirs, as 448 x 2^120 (what a
-// block of magnitudes up to the largest float32 may round to) is past bfloat16. Sums take
-// kExpanded back in the epilogue.
-__device__ __forceinline__ float half_power(int byte) { return __uint_as_float((uint32_t)(byte - 1) << 23); }
-constexpr float kExpanded = 4.f;
-
-// The same product summed in float32 throughout, in units of 1 / kExpanded.
-__device__ __forceinline__ f32x4 mfma_exact(i32x8 a, i32x8 b, f32x4 c, float a_scale, float b_scale) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(expand(a[2 * q], a[2 * q + 1], a_scale),
-                                                expand(b[2 * q], b[2 * q + 1], b_scale), c, 0, 0, 0);
-  return c;
-}
-
-// 64 x 64 outputs of 4 waves, 32 x 32 each, fragments read from memory.
-template <typename OUT>
-__global__ __launch_bounds__(256) void float8_gemm_kernel(ProductArgs g) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t m0 = (int64_t)(blockIdx.x / g.tiles_n) * 64 + (wave >> 1) * 32;
-  const int64_t n0 = (int64_t)(blockIdx.x % g.tiles_n) * 64 + (wave & 1) * 32;
-  const int i16 = lane & 15, G = lane >> 4;
-  f32x4 acc[2][2] = {};
-  int64_t row[2], col[2];
-  for (int f = 0; f < 2; ++f) {
-    row[f] = min(m0 + f * 16 + i16, g.m - 1);
-    col[f] = min(n0 + f * 16 + i16, g.n - 1);
-  }
-  for (int kb = 0; kb < g.blocks; ++kb) {
-    i32x8 a[2], b[2];
-    int as[2], bs[2];
-    for (int f = 0; f < 2; ++f) {
-      const i32x4* pa = reinterpret_cast<const i32x4*>(g.a + row[f] * g.lda + kb * kTile + 32 * G);
-      const i32x4* pb = reinterpret_cast<const i32x4*>(g.b + col[f] * g.ldb + kb * kTile + 32 * G);
-      a[f] = __builtin_shufflevector(pa[0], pa[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      b[f] = __builtin_shufflevector(pb[0], pb[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      as[f] = g.a_scale[kb * g.a_scale_ld + row[f]];
-      bs[f] = g.b_scale[kb * g.b_scale_ld + col[f]];
-    }
-    for (int i = 0; i < 2; ++i)
-      for (int j = 0; j < 2; ++j)
-        acc[i][j] = sizeof(OUT) == 4
-                        ? mfma_exact(b[j], a[i], acc[i][j], half_power(bs[j]), half_power(as[i]))
-                        : mfma(b[j], a[i], acc[i][j], bs[j], as[i]);
-  }
-  OUT* c = reinterpret_cast<OUT*>(g.c);
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < 2; ++j)
-      for (int e = 0; e < 4; ++e) {
-        const int64_t r = m0 + i * 16 + i16, q = n0 + j * 16 + 4 * G + e;
-        if (r < g.m && q < g.n) 
-          c[r * g.ldc + q] = (OUT)((sizeof(OUT) == 4 ? kExpanded : 1.f) * acc[i][j][e] + (g.bias ? g.bias[q] : 0.f));
-      }
-}
-
-template <typename OUT>
-int launch_product(ProductArgs g, hipStream_t stream) {
-  const int64_t tm = ceil_div(g.m, 64), tn = ceil_div(g.n, 64);
-  DIONW_REQUIRE(tm * tn < INT32_MAX, "float8_gemm: too many tiles");
-  g.tiles_n = (int32_t)tn;
-  hipLaunchKernelGGL(float8_gemm_kernel<OUT>, dim3((unsigned)(tm * tn)), dim3(256), 0, stream, g);
-  return check_launch("float8_gemm");
-}
-
 }  // namespace
 }  // namespace dionw
 
@@ -352,7 +231,7 @@ extern "C" {
 int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
                           int32_t tiles, void* data, int64_t data_ld, void* scale,
                           int64_t scale_ld, void* data_t, int64_t data_t_ld, void* scale_t,
-                          int64_t scale_t_ld, float* sums, hipStream_t stream) {
+                          int64_t scale_t_ld, int32_t expand_t, float* sums, hipStream_t stream) {
   DIONW_REQUIRE(elem == kF16 || elem == kBF16 || elem == kF32, "float8_quantize: bad element type %d", elem);
   DIONW_REQUIRE(rows >= 0 && cols >= 0, "float8_quantize: negative extent");
   if (rows == 0 || cols == 0) return kOk;
@@ -362,20 +241,38 @@ int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t col
     return !d || (s && d_ld >= round_up(c, kTile) && d_ld % 16 == 0 && s_ld >= r && aligned16(d));
   };
   DIONW_REQUIRE(fits(data, data_ld, scale, scale_ld, rows, cols) &&
-                    fits(data_t, data_t_ld, scale_t, scale_t_ld, cols, rows),
+                    fits(data_t, data_t_ld, expand_t ? x : scale_t, expand_t ? cols : scale_t_ld, cols, rows),
                 "float8_quantize: an output is too small or not aligned");
   const int64_t tr = ceil_div(rows, kTile), tc = ceil_div(cols, kTile);
   DIONW_REQUIRE(tr < INT32_MAX / tc, "float8_quantize: too many tiles");
   const int64_t size = elem == kF32 ? 4 : 2;
   QuantizeArgs q{x,       rows,     cols,    ld,
                  static_cast<uint8_t*>(data),   data_ld,   static_cast<uint8_t*>(scale),   scale_ld,
-                 static_cast<uint8_t*>(data_t), data_t_ld, static_cast<uint8_t*>(scale_t), scale_t_ld,
+                 static_cast<uint8_t*>(data_t), expand_t ? 2 * data_t_ld : data_t_ld,
+                 static_cast<uint8_t*>(scale_t), scale_t_ld,
                  sums,    (int32_t)tc,
-                 aligned16(x) && ld * size % 16 == 0};
+                 aligned16(x) && ld * size % 16 == 0, expand_t};
   const unsigned grid = (unsigned)(tr * tc);
   if (elem == kF16) return launch_quantize<_Float16>(q, tiles != 0, grid, stream);
   if (elem == kBF16) return launch_quantize<__bf16>(q, tiles != 0, grid, stream);
   return launch_quantize<float>(q, tiles != 0, grid, stream);
+}
+
+int dionw_float8_expand(const void* data, int64_t data_ld, const void* scale, int64_t scale_ld,
+                        int64_t rows, int64_t depth, void* out, int64_t out_ld,
+                        hipStream_t stream) {
+  DIONW_REQUIRE(rows >= 0 && depth >= 0 && depth % kTile == 0, "float8_expand: bad extents");
+  if (rows == 0 || depth == 0) return kOk;
+  DIONW_REQUIRE(data && scale && out && aligned16(data) && aligned16(out) && data_ld >= depth &&
+                    data_ld % 16 == 0 && out_ld >= depth && out_ld % 8 == 0 && scale_ld >= rows,
+                "float8_expand: a matrix is too small or not aligned");
+  const int64_t chunks = depth / 16;
+  DIONW_REQUIRE(rows <= (int64_t)INT32_MAX * 256 / chunks, "float8_expand: too many elements");
+  hipLaunchKernelGGL(float8_expand_kernel, dim3((unsigned)ceil_div(rows * chunks, 256)), dim3(256), 0,
+                     stream, static_cast<const uint8_t*>(data), data_ld,
+                     static_cast<const uint8_t*>(scale), scale_ld, rows, chunks,
+                     static_cast<__bf16*>(out), out_ld);
+  return check_launch("float8_expand");
 }
 
 int dionw_sum_parts(const float* parts, int64_t count, int64_t cols, int32_t elem, void* out,
@@ -397,30 +294,6 @@ int dionw_sum_parts(const float* parts, int64_t count, int64_t cols, int32_t ele
   else
     DIONW_REQUIRE(false, "sum_parts: bad element type %d", elem);
   return check_launch("sum_parts");
-}
-
-int dionw_float8_gemm(int64_t m, int64_t n, int64_t depth, const void* a, int64_t lda,
-                      const void* a_scale, int64_t a_scale_ld, const void* b, int64_t ldb,
-                      const void* b_scale, int64_t b_scale_ld, const float* bias, int32_t elem,
-                      void* c, int64_t ldc, hipStream_t stream) {
-  DIONW_REQUIRE(m >= 0 && n >= 0 && depth >= 0 && depth % kTile == 0,
-                "float8_gemm: bad extents %lld x %lld x %lld", (long long)m, (long long)n,
-                (long long)depth);
-  DIONW_REQUIRE(elem == kF16 || elem == kBF16 || elem == kF32, "float8_gemm: bad element type %d", elem);
-  if (m == 0 || n == 0) return kOk;
-  DIONW_REQUIRE(c && ldc >= n, "float8_gemm: bad output");
-  DIONW_REQUIRE(depth == 0 || (a && a_scale && b && b_scale), "float8_gemm: null operand");
-  DIONW_REQUIRE(depth / kTile < INT32_MAX, "float8_gemm: depth too large");
-  DIONW_REQUIRE(lda >= depth && ldb >= depth && lda % 16 == 0 && ldb % 16 == 0 && aligned16(a) &&
-                    aligned16(b) && a_scale_ld >= m && b_scale_ld >= n,
-                "float8_gemm: operands need rows of at least their depth at multiples of 16 bytes "
-                "and a scale for each row");
-  ProductArgs g{static_cast<const uint8_t*>(a), lda, static_cast<const uint8_t*>(a_scale), a_scale_ld,
-                static_cast<const uint8_t*>(b), ldb, static_cast<const uint8_t*>(b_scale), b_scale_ld,
-                bias, c, ldc, m, n, (int32_t)(depth / kTile), 0};
-  if (elem == kF16) return launch_product<_Float16>(g, stream);
-  if (elem == kBF16) return launch_product<__bf16>(g, stream);
-  return launch_product<float>(g, stream);
 }
 
 }  // extern "C"

@@ -2,8 +2,8 @@
 
 The optimizer keeps float32 master weights; the layer here is a way to run the model over
 them: weights, activations and gradients are quantized to e4m3 (4 exponent bits, 3 fraction
-bits, largest 448) where a product reads them, and products sum in float32 on the scaled
-8-bit matrix instructions. Scales are powers of two, so that scaling rounds nothing.
+bits, largest 448) where a product reads them, and 16-bit results come from the scaled
+8-bit matrix instructions, float32 ones (weight gradients) from bfloat16 ones on the same values. Scales are powers of two, so that scaling rounds nothing.
 
 - ``float8_linear(x, weight, bias)``: ``x @ weight.T + bias``, differentiable. x and the
   gradient are quantized with a scale per row and 128 columns (for the weight's gradient, per
@@ -40,8 +40,8 @@ class Float8Matrix:
     Attributes:
         data: float8_e4m3fn codes ``[rows, depth]``, ``depth`` being ``cols`` rounded up to
             128; the columns past ``cols`` hold zeros.
-        scale: uint8 ``[depth / 128, at least rows]``: the exponent bytes of the float32
-            scales, by column block.
+        scale: uint8 ``[depth / 128, rows rounded up to 16 or more]``: the exponent bytes of
+            the float32 scales, by column block.
         cols: The number of columns.
 
     Raises:
@@ -65,6 +65,8 @@ class Float8Matrix:
         if scale.shape[0] != depth // TILE or scale.shape[1] < data.shape[0]:
             raise ValueError(f"the scales of {data.shape[0]} rows are [{depth // TILE}, rows or more], "
                              f"got {tuple(scale.shape)}")
+        if scale.shape[1] % 16:
+            raise ValueError(f"the scales of a column block lie at a multiple of 16, got {scale.shape[1]}")
         if not (data.is_contiguous() and scale.is_contiguous()) or data.device != scale.device:
             raise ValueError("a Float8Matrix's tensors are contiguous and on one device")
 
@@ -92,6 +94,33 @@ def _empty(rows: int, cols: int, device: torch.device) -> Float8Matrix:
         torch.empty(depth // TILE, -(-rows // 16) * 16, dtype=torch.uint8, device=device), cols)
 
 
+def _expanded(rows: int, cols: int, device: torch.device) -> Tensor:
+    return torch.empty(rows, -(-cols // TILE) * TILE, dtype=torch.bfloat16, device=device)
+
+
+def _expand(q: Float8Matrix) -> Tensor:
+    """The matrix as a product summed in float32 reads it: bfloat16 halves of the values."""
+    rows, depth = q.data.shape
+    out = _expanded(rows, depth, q.device)
+    _lib.call("dionw_float8_expand", q.data.data_ptr(), depth, q.scale.data_ptr(), q.scale.shape[1],
+              rows, depth, out.data_ptr(), depth, _lib.stream_handle(q.device))
+    return out
+
+
+def _product(m: int, n: int, depth: int, a: tuple[int, int | None, int], b: tuple[int, int | None, int],
+             bias: Tensor | None, dtype: torch.dtype, device: torch.device) -> Tensor:
+    """``a b.T + bias`` from the operands' addresses: (data, scale, scale pitch), the scale None
+    for expanded operands."""
+    expanded, stream = int(a[1] is None), _lib.stream_handle(device)
+    out = torch.empty(m, n, dtype=dtype, device=device)
+    size = _lib.library().dionw_float8_gemm_workspace(expanded, m, n, depth)
+    space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _lib.call("dionw_float8_gemm", expanded, m, n, depth, a[0], depth, a[1], a[2], b[0], depth, b[1],
+              b[2], _lib.ptr(bias), _lib.elem_code(dtype), out.data_ptr(), n, _lib.ptr(space), size,
+              stream)
+    return out
+
+
 def _readable(x: Tensor) -> Tensor:
     """x as the kernels read it: rows of adjacent elements that do not overlap."""
     if x.dim() != 2 or x.dtype not in _DTYPES:
@@ -102,22 +131,28 @@ def _readable(x: Tensor) -> Tensor:
 
 
 def _quantize(x: Tensor, tiles: bool, rows: bool, columns: bool, sums: torch.dtype | None = None,
-              ) -> tuple[Float8Matrix | None, Float8Matrix | None, Tensor | None]:
-    """x quantized by rows, its transpose quantized by rows, and its column sums, as asked."""
+              *, expand: bool = False,
+              ) -> tuple[Float8Matrix | None, Float8Matrix | Tensor | None, Tensor | None]:
+    """x quantized by rows, its transpose quantized by rows (``expand``: its codes expanded, as a
+    product summed in float32 reads them), and its column sums, as asked."""
     x = _readable(x)
     m, n = x.shape
     stream = _lib.stream_handle(x.device)
     by_row = _empty(m, n, x.device) if rows else None
-    by_column = _empty(n, m, x.device) if columns else None
+    by_column: Float8Matrix | Tensor | None = None
+    if columns:
+        by_column = _expanded(n, m, x.device) if expand else _empty(n, m, x.device)
     parts = torch.empty(-(-m // TILE), n, device=x.device) if sums else None
     ld = x.stride(0) if m > 1 else n
 
-    def place(q: Float8Matrix | None) -> tuple[Any, ...]:
+    def place(q: Float8Matrix | Tensor | None) -> tuple[Any, ...]:
+        if isinstance(q, Tensor):
+            return q.data_ptr(), q.shape[1], None, 0
         return (None, 0, None, 0) if q is None else (
             q.data.data_ptr(), q.data.shape[1], q.scale.data_ptr(), q.scale.shape[1])
 
     _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, max(ld, n),
-              int(tiles), *place(by_row), *place(by_column), _lib.ptr(parts), stream)
+              int(tiles), *place(by_row), *place(by_column), int(expand), _lib.ptr(parts), stream)
     total = None
     if sums:
         total = torch.empty(n, dtype=sums, device=x.device)
@@ -138,7 +173,11 @@ def float8_quantize(x: Tensor, *, tiles: bool = False) -> Float8Matrix:
 
 def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, *,
                   dtype: torch.dtype = torch.bfloat16) -> Tensor:
-    """``a @ b.T + bias`` summed in float32 and rounded once to ``dtype``.
+    """``a @ b.T + bias`` rounded once to ``dtype``.
+
+    A float32 result is summed in float32 on operands expanded to bfloat16, which is exact. A
+    16-bit one runs on the 8-bit matrix instructions, which cut the products of each 8 columns to
+    13 bits below the exponent of the largest of them before they add (1e-5 to 6e-5 of the result).
 
     Raises:
         ValueError: For operands or a bias that do not fit each other, another dtype than
@@ -149,12 +188,14 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
         raise ValueError(f"float8_matmul takes matrices of one depth on one device, got {a.shape} on "
                          f"{a.device} and {b.shape} on {b.device}")
     bias = _bias(bias, n, a.device)
-    code, stream = _lib.elem_code(dtype), _lib.stream_handle(a.device)
-    out = torch.empty(m, n, dtype=dtype, device=a.device)
-    _lib.call("dionw_float8_gemm", m, n, a.data.shape[1], a.data.data_ptr(), a.data.shape[1],
-              a.scale.data_ptr(), a.scale.shape[1], b.data.data_ptr(), b.data.shape[1],
-              b.scale.data_ptr(), b.scale.shape[1], _lib.ptr(bias), code, out.data_ptr(), n, stream)
-    return out
+    _lib.elem_code(dtype)
+    depth = a.data.shape[1]
+    if dtype is torch.float32:
+        ea, eb = _expand(a), _expand(b)
+        return _product(m, n, depth, (ea.data_ptr(), None, 0), (eb.data_ptr(), None, 0), bias, dtype,
+                        a.device)
+    return _product(m, n, depth, (a.data.data_ptr(), a.scale.data_ptr(), a.scale.shape[1]),
+                    (b.data.data_ptr(), b.scale.data_ptr(), b.scale.shape[1]), bias, dtype, a.device)
 
 
 def _bias(bias: Tensor | None, n: int, device: torch.device) -> Tensor | None:
@@ -188,9 +229,17 @@ class _Linear(torch.autograd.Function):
         saved = list(ctx.saved_tensors)
         xt = Float8Matrix(*saved[:2], m) if need_w else None
         wt = Float8Matrix(*saved[-2:], n) if need_x else None
-        rows, columns, db = _quantize(dy, False, need_x, need_w, ctx.bias_dtype if need_b else None)
+        exact = ctx.dtypes[1] is torch.float32
+        rows, columns, db = _quantize(dy, False, need_x, need_w, ctx.bias_dtype if need_b else None,
+                                      expand=exact)
         dx = float8_matmul(rows, wt, dtype=ctx.dtypes[0]) if need_x else None
-        dw = float8_matmul(columns, xt, dtype=ctx.dtypes[1]) if need_w else None
+        dw = None
+        if need_w and exact:
+            ex = _expand(xt)
+            dw = _product(n, k, ex.shape[1], (columns.data_ptr(), None, 0), (ex.data_ptr(), None, 0),
+                          None, torch.float32, dy.device)
+        elif need_w:
+            dw = float8_matmul(columns, xt, dtype=ctx.dtypes[1])
         return dx, dw, db
 
 

@@ -346,26 +346,45 @@ int dionw_adamw_8bit_values(const int64_t* numels, const int64_t* first_blocks, 
  * into data/scale by rows, and into data_t/scale_t as the transpose [cols, rows]; either may
  * be NULL. One scale for each row (of the transpose: column of x) and block of 128, or for
  * each 128 x 128 tile when tiles != 0. Values that are not finite become NaN and leave their
- * block's scale alone. sums (may be NULL): float32 [ceil(rows / 128)][cols], the column sums
+ * block's scale alone. expand_t != 0: data_t takes bfloat16 halves of the values (see
+ * dionw_float8_expand; data_t_ld in elements) and scale_t is not used. sums (may be NULL): float32 [ceil(rows / 128)][cols], the column sums
  * of each 128 rows.
  */
 int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
                           int32_t tiles, void* data, int64_t data_ld, void* scale,
                           int64_t scale_ld, void* data_t, int64_t data_t_ld, void* scale_t,
-                          int64_t scale_t_ld, float* sums, dionw_stream_t stream);
+                          int64_t scale_t_ld, int32_t expand_t, float* sums,
+                          dionw_stream_t stream);
 
 /* out[c] = parts[0][c] + parts[1][c] + ... in order, in element code elem. */
 int dionw_sum_parts(const float* parts, int64_t count, int64_t cols, int32_t elem, void* out,
                     dionw_stream_t stream);
 
 /*
+ * The codes [rows][data_ld] of a quantized matrix expanded: bfloat16 halves of the values,
+ * out [rows][out_ld] (16-byte aligned, out_ld a multiple of 8), `depth` columns (a multiple
+ * of 128).
+ */
+int dionw_float8_expand(const void* data, int64_t data_ld, const void* scale, int64_t scale_ld,
+                        int64_t rows, int64_t depth, void* out, int64_t out_ld,
+                        dionw_stream_t stream);
+
+/*
  * C [m, n] = A B^T + bias for quantized A [m, depth] and B [n, depth] (depth: a multiple of
  * 128), summed in float32 and rounded once to element code elem; bias: n floats or NULL.
+ * expanded 0: codes with their scales (pitches a multiple of 16, 4-byte aligned), float16 or
+ * bfloat16 output; the products of each 8 columns are cut to 13 bits below the exponent of
+ * the largest of them before they are added. expanded 1: operands from dionw_float8_expand
+ * (or dionw_float8_quantize), float32 output, every product exact. Pitches in elements, rows
+ * of less than 8 MB at multiples of 16 bytes. workspace: float32 scratch of
+ * dionw_float8_gemm_workspace bytes (0: none needed).
  */
-int dionw_float8_gemm(int64_t m, int64_t n, int64_t depth, const void* a, int64_t lda,
-                      const void* a_scale, int64_t a_scale_ld, const void* b, int64_t ldb,
-                      const void* b_scale, int64_t b_scale_ld, const float* bias, int32_t elem,
-                      void* c, int64_t ldc, dionw_stream_t stream);
+size_t dionw_float8_gemm_workspace(int32_t expanded, int64_t m, int64_t n, int64_t depth);
+int dionw_float8_gemm(int32_t expanded, int64_t m, int64_t n, int64_t depth, const void* a,
+                      int64_t lda, const void* a_scale, int64_t a_scale_ld, const void* b,
+                      int64_t ldb, const void* b_scale, int64_t b_scale_ld, const float* bias,
+                      int32_t elem, void* c, int64_t ldc, void* workspace, size_t workspace_bytes,
+                      dionw_stream_t stream);
 
 /*
  * GPU EMA of float32 sources: shadow = lerp(shadow, source, weight), or a

@@ -78,18 +78,32 @@ def test_the_library_checks_its_arguments() -> None:
     """Rejected before anything is launched: no address here is one of a GPU."""
     def quantize(elem=2, rows=4, cols=200, ld=200, data=16, data_ld=256, scale=16, scale_ld=4, data_t=None):
         _lib.call("dionw_float8_quantize", elem, 16, rows, cols, ld, 0, data, data_ld, scale, scale_ld,
-                  data_t, 0, None, 0, None, None)
+                  data_t, 0, None, 0, 0, None, None)
 
     for bad in ({"elem": 3}, {"rows": -1}, {"ld": 199}, {"data": None}, {"data": 8}, {"data_ld": 255},
                 {"data_ld": 200}, {"scale": None}, {"scale_ld": 3}, {"data_t": 16}):
         with pytest.raises(ValueError):
             quantize(**bad)
 
-    def gemm(m=4, n=4, depth=256, a=16, lda=256, a_scale=16, a_scale_ld=4, b=16, elem=2, c=16, ldc=4):
-        _lib.call("dionw_float8_gemm", m, n, depth, a, lda, a_scale, a_scale_ld, b, 256, 16, 4, None,
-                  elem, c, ldc, None)
+    def gemm(m=4, n=4, depth=256, a=16, lda=256, a_scale=16, a_scale_ld=16, b=16, elem=1, c=16, ldc=4,
+             expanded=0, ldb=256, b_scale_ld=16):
+        _lib.call("dionw_float8_gemm", expanded, m, n, depth, a, lda, a_scale, a_scale_ld, b, ldb, 16,
+                  b_scale_ld, None, elem, c, ldc, None, 0, None)
 
     for bad in ({"m": -1}, {"depth": 200}, {"a": None}, {"a": 8}, {"lda": 128}, {"lda": 264},
-                {"a_scale": None}, {"a_scale_ld": 3}, {"b": None}, {"elem": 3}, {"c": None}, {"ldc": 3}):
+                {"a_scale": None}, {"a_scale_ld": 3}, {"a_scale_ld": 20}, {"a_scale": 18}, {"b": None},
+                {"elem": 2}, {"elem": 3}, {"expanded": 1}, {"c": None}, {"ldc": 3}, {"lda": 1 << 23}):
         with pytest.raises(ValueError):
             gemm(**bad)
+    # A depth that is split needs its workspace.
+    size = _lib.library().dionw_float8_gemm_workspace(0, 64, 64, 1 << 16)
+    assert size > 0
+    with pytest.raises(ValueError, match="workspace"):
+        gemm(m=64, n=64, depth=1 << 16, lda=1 << 16, ldb=1 << 16, a_scale_ld=64, b_scale_ld=64, ldc=64)
+
+    def expand(data=16, data_ld=256, scale_ld=4, depth=256, out_ld=256):
+        _lib.call("dionw_float8_expand", data, data_ld, 16, scale_ld, 4, depth, 16, out_ld, None)
+
+    for bad in ({"data": None}, {"data": 8}, {"data_ld": 128}, {"scale_ld": 3}, {"depth": 130}, {"out_ld": 255}):
+        with pytest.raises(ValueError):
+            expand(**bad)
