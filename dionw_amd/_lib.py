@@ -135,6 +135,22 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _p,
          ctypes.c_size_t, _p],
     ),
+    "dionw_float8_linear_sizes": (None, [_i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _psize]),
+    "dionw_float8_linear_forward": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i32, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p,
+         ctypes.c_size_t, _p],
+    ),
+    "dionw_float8_linear_backward": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i32, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _i32, _p, _p,
+         ctypes.c_size_t, _p],
+    ),
+    "dionw_float8_linear_kept_scratch": (ctypes.c_size_t, [_i32, _i64, _i64, _i64]),
+    "dionw_float8_linear_kept": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, ctypes.c_size_t, _p],
+    ),
     "dionw_ema_update": (ctypes.c_int, [_pp, _pp, _pi64, _i32, _f32, _i32, _p]),
 }
 

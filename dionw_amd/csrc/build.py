@@ -17,7 +17,7 @@ HERE = Path(__file__).resolve().parent
 PACKAGE = HERE.parent
 LIBRARY = PACKAGE / "libdionw_hip.so"
 SOURCES = ("errors.cpp", "momentum.hip", "select.hip", "normuon.hip", "adamw_ema.hip",
-           "adamw_8bit.hip", "float8.hip", "float8_gemm.hip", "gemm.hip")
+           "adamw_8bit.hip", "float8.hip", "float8_gemm.hip", "float8_linear.hip", "gemm.hip")
 ARCH = "gfx950"
 FLAGS = (
     f"--offload-arch={ARCH}",

@@ -21,23 +21,6 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
 }
 __device__ __forceinline__ float power(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// The bits of |v|, 0 where it is not finite (such values become NaN codes and leave the
-// block's scale alone).
-__device__ __forceinline__ uint32_t magnitude(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? b : 0u;
-}
-
-// Four codes of four values, rounded to nearest even; infinities become NaN.
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float inv) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
-}
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
-__device__ __forceinline__ float to_float(__bf16 v) { return (float)v; }
-
 // Codes are expanded to bfloat16 with half their scale, as 448 x 2^120 (what a block of
 // magnitudes up to the largest float32 may round to) is past bfloat16. Sums of products of
 // two expanded operands take kExpanded back.
@@ -52,6 +35,68 @@ __device__ __forceinline__ bf16x8 expand(uint32_t lo, uint32_t hi, float scale) 
   const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
   return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3),
                                  __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Two values of a thread as they lie in memory: one word of 16-bit ones, two of float32.
+template <typename T>
+struct Pair;
+template <typename T>
+struct Pair16 {
+  uint32_t w;
+  // magnitudes, two 16-bit integers
+  __device__ __forceinline__ uint32_t most() const { return w & 0x7FFF7FFFu; }
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                  __builtin_bit_cast(u16x2, b)));
+  }
+};
+template <>
+struct Pair<__bf16> : Pair16<__bf16> {
+  static constexpr uint32_t inf = 0x7F80u;
+  __device__ __forceinline__ static uint32_t bits(uint32_t m) { return m << 16; }
+  __device__ __forceinline__ float value(int k) const {
+    return __uint_as_float(k ? w & 0xFFFF0000u : w << 16);
+  }
+};
+template <>
+struct Pair<_Float16> : Pair16<_Float16> {
+  static constexpr uint32_t inf = 0x7C00u;
+  __device__ __forceinline__ static uint32_t bits(uint32_t m) {
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)m));
+  }
+  __device__ __forceinline__ float value(int k) const {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(k ? w >> 16 : w));
+  }
+};
+
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Codes of four values times 1 / scale, rounded to nearest even; infinities become NaN.
+__device__ __forceinline__ uint32_t codes4(uint32_t lo, uint32_t hi, float scale, __bf16) {
+  i16x2 o = {0, 0};
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(bf16x2, lo), scale, false);
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(bf16x2, hi), scale, true);
+  return __builtin_bit_cast(uint32_t, o);
+}
+__device__ __forceinline__ uint32_t codes4(uint32_t lo, uint32_t hi, float scale, _Float16) {
+  i16x2 o = {0, 0};
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(f16x2, lo), scale, false);
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(f16x2, hi), scale, true);
+  return __builtin_bit_cast(uint32_t, o);
+}
+__device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, float scale) {
+  i16x2 o = {0, 0};
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, __uint_as_float(a), __uint_as_float(b), scale, false);
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, __uint_as_float(c), __uint_as_float(d), scale, true);
+  return __builtin_bit_cast(uint32_t, o);
+}
+
+// The largest over a row of 16 lanes.
+template <int N>
+__device__ __forceinline__ uint32_t turned_row(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 | N, 0xF, 0xF, false);  // row_ror:N
 }
 
 }  // namespace dionw

@@ -19,79 +19,204 @@ namespace {
 // ---- quantization ------------------------------------------------------------------
 //
 // A workgroup takes a 128 x 128 tile: thread t the rows 8 (t / 16) .. + 7 and the columns
-// 8 (t % 16) .. + 7, read once and held in registers. From them come the codes by rows and,
-// through LDS, the codes of the transpose, each in whole 128-byte lines.
-// Bound: HBM, 2 or 4 bytes read and 1 or 2 written an element.
+// 8 (t % 16) .. + 7, read once and held as they are. From them come the codes by rows and,
+// through LDS, the codes of the transpose, each in whole 128-byte lines. Magnitudes are compared
+// as integers (16-bit ones two at a time), and v_cvt_scalef32_pk_fp8_* rounds two values a time,
+// scale included. Infinities and NaN become NaN codes by themselves; a thread whose maximum is one
+// of them takes its finite values' maxima on a path of its own.
+// Bound: HBM, 2 or 4 bytes read and 1 to 4 written an element.
+struct Output {
+  uint8_t* data;     // null: not asked for
+  int64_t ld;        // bytes
+  uint8_t* scale;    // codes only
+  int64_t scale_ld;
+  int32_t expanded;  // bfloat16 halves of the values instead of codes
+};
 struct QuantizeArgs {
   const void* x;
   int64_t rows, cols, ld;
-  uint8_t* data;      // [rows][data_ld] or null
-  int64_t data_ld;
-  uint8_t* scale;     // [blocks][scale_ld]
-  int64_t scale_ld;
-  uint8_t* data_t;    // the transpose: [cols][data_t_ld bytes] or null
-  int64_t data_t_ld;
-  uint8_t* scale_t;
-  int64_t scale_t_ld;
-  float* sums;        // [row tiles][cols]: each tile's column sums, or null
+  Output by_row, by_col;  // x, and its transpose
+  float* sums;            // [row tiles][cols]: each tile's column sums, or null
   int32_t tiles_c;
-  int32_t vec;        // rows start at multiples of 16 bytes
-  int32_t expand_t;   // the transpose in bfloat16, scales included
+  int32_t vec;            // rows start at multiples of 16 bytes
+};
+
+// A thread's 8 x 8 values and what the kernel asks of them.
+template <typename T>
+struct Square {  // 16-bit
+  using P = Pair<T>;
+  static constexpr int kRowMost = 4, kColMost = 4;  // words of maxima: two rows, two columns each
+  uint32_t w[8][4];
+  __device__ __forceinline__ void load(int i, const T* at) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[i][k] = v[k];
+  }
+  __device__ __forceinline__ void load(int i, const T* at, int64_t left) {
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = 2 * k < left ? u[2 * k] : 0, hi = 2 * k + 1 < left ? u[2 * k + 1] : 0;
+      w[i][k] = lo | hi << 16;
+    }
+  }
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) { return P::larger(a, b); }
+  __device__ __forceinline__ void maxima(uint32_t (&row)[4], uint32_t (&col)[4]) const {
+    uint32_t one[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) col[k] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[k] = w[i][k] & 0x7FFF7FFFu;
+        col[k] = larger(col[k], m[k]);
+      }
+      one[i] = larger(larger(m[0], m[1]), larger(m[2], m[3]));
+    }
+    // Two rows a word: the larger of each row's even and odd columns.
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      row[i] = larger(__builtin_amdgcn_perm(one[2 * i + 1], one[2 * i], 0x05040100u),
+                      __builtin_amdgcn_perm(one[2 * i + 1], one[2 * i], 0x07060302u));
+  }
+  __device__ __forceinline__ static bool odd(uint32_t m) {  // not finite
+    return (m & 0xFFFFu) >= P::inf || (m >> 16) >= P::inf;
+  }
+  // The float32 bits of maximum i of the words.
+  __device__ __forceinline__ static uint32_t bits(const uint32_t (&m)[4], int i) {
+    return P::bits(i & 1 ? m[i >> 1] >> 16 : m[i >> 1] & 0xFFFFu);
+  }
+  // The maxima of the finite values.
+  __device__ __forceinline__ void finite_maxima(uint32_t (&row)[4], uint32_t (&col)[4]) const {
+    Square kept;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = w[i][k] & 0x7FFFu, hi = w[i][k] & 0x7FFF0000u;
+        kept.w[i][k] = (lo < P::inf ? lo : 0u) | (hi < P::inf << 16 ? hi : 0u);
+      }
+    kept.maxima(row, col);
+  }
+  __device__ __forceinline__ u32x2 row_codes(int i, float scale) const {
+    return u32x2{codes4(w[i][0], w[i][1], scale, T{}), codes4(w[i][2], w[i][3], scale, T{})};
+  }
+  __device__ __forceinline__ u32x2 col_codes(int k, float scale) const {
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      p[i] = __builtin_amdgcn_perm(w[2 * i + 1][k >> 1], w[2 * i][k >> 1], k & 1 ? 0x07060302u : 0x05040100u);
+    return u32x2{codes4(p[0], p[1], scale, T{}), codes4(p[2], p[3], scale, T{})};
+  }
+  __device__ __forceinline__ float value(int i, int k) const { return P{w[i][k >> 1]}.value(k & 1); }
+};
+
+template <>
+struct Square<float> {
+  static constexpr int kRowMost = 8, kColMost = 8;
+  static constexpr uint32_t inf = 0x7F800000u;
+  uint32_t w[8][8];
+  __device__ __forceinline__ void load(int i, const float* at) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 v = reinterpret_cast<const u32x4*>(at)[h];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[i][4 * h + k] = v[k];
+    }
+  }
+  __device__ __forceinline__ void load(int i, const float* at, int64_t left) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[i][k] = k < left ? __float_as_uint(at[k]) : 0;
+  }
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+  __device__ __forceinline__ void maxima(uint32_t (&row)[8], uint32_t (&col)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) row[k] = col[k] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t m = w[i][k] & 0x7FFFFFFFu;
+        row[i] = max(row[i], m);
+        col[k] = max(col[k], m);
+      }
+  }
+  __device__ __forceinline__ static bool odd(uint32_t m) { return m >= inf; }
+  __device__ __forceinline__ static uint32_t bits(const uint32_t (&m)[8], int i) { return m[i]; }
+  __device__ __forceinline__ void finite_maxima(uint32_t (&row)[8], uint32_t (&col)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) row[k] = col[k] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t b = w[i][k] & 0x7FFFFFFFu, m = b < inf ? b : 0u;
+        row[i] = max(row[i], m);
+        col[k] = max(col[k], m);
+      }
+  }
+  __device__ __forceinline__ u32x2 row_codes(int i, float scale) const {
+    return u32x2{codes4(w[i][0], w[i][1], w[i][2], w[i][3], scale),
+                 codes4(w[i][4], w[i][5], w[i][6], w[i][7], scale)};
+  }
+  __device__ __forceinline__ u32x2 col_codes(int k, float scale) const {
+    return u32x2{codes4(w[0][k], w[1][k], w[2][k], w[3][k], scale),
+                 codes4(w[4][k], w[5][k], w[6][k], w[7][k], scale)};
+  }
+  __device__ __forceinline__ float value(int i, int k) const { return __uint_as_float(w[i][k]); }
 };
 
 template <typename T, bool TILES>
 __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
-  constexpr int kPitch = kTile + 16;
-  __shared__ __attribute__((aligned(16))) uint8_t turned[kTile * kPitch];
-  __shared__ uint32_t col_most[4][kTile];
+  using S = Square<T>;
+  constexpr int RM = S::kRowMost, CM = S::kColMost;
+  // Bytes of the transpose: 33 words a row, so that the 16 columns x 4 row groups of a wave's
+  // 8-byte writes spread over the banks.
+  constexpr int kPitch = 33;
+  __shared__ uint32_t turned[kTile * kPitch];
+  __shared__ uint32_t col_most[4][16][CM];
   __shared__ float col_sum[4][kTile];
   __shared__ uint8_t row_bytes[kTile], col_bytes[kTile];
   const int tid = threadIdx.x, wave = tid >> 6;
   const int64_t r0 = (int64_t)(blockIdx.x / q.tiles_c) * kTile;
   const int64_t c0 = (int64_t)(blockIdx.x % q.tiles_c) * kTile;
   const int tr = tid / 16 * 8, tc = tid % 16 * 8;  // the thread's first row and column
-  float v[8][8];
+  S v;
+  const T* at = reinterpret_cast<const T*>(q.x) + (r0 + tr) * q.ld + c0 + tc;
+  if (q.vec && r0 + tr + 8 <= q.rows && c0 + tc + 8 <= q.cols) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + tr + i, c = c0 + tc;
-    const T* at = reinterpret_cast<const T*>(q.x) + r * q.ld + c;
-    if (r < q.rows && q.vec && c + 8 <= q.cols) {
-      T raw[8];
-#pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-        reinterpret_cast<u32x4*>(raw)[k] = reinterpret_cast<const u32x4*>(at)[k];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = to_float(raw[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = r < q.rows && c + k < q.cols ? to_float(at[k]) : 0.f;
-    }
-  }
-  uint32_t row_most[8], most[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) row_most[i] = most[i] = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t b = magnitude(v[i][k]);
-      row_most[i] = max(row_most[i], b);
-      most[k] = max(most[k], b);
-    }
-#pragma unroll
-  for (int off = 8; off >= 1; off >>= 1)
+    for (int i = 0; i < 8; ++i) v.load(i, at + i * q.ld);
+  } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      row_most[i] = max(row_most[i], (uint32_t)__shfl_xor((int)row_most[i], off, kWave));
-  if (TILES || q.data_t) {
+      v.load(i, at + i * q.ld, r0 + tr + i < q.rows ? q.cols - c0 - tc : 0);
+  }
+  uint32_t row[RM], col[CM];
+  v.maxima(row, col);
+  uint32_t all = 0;
 #pragma unroll
-    for (int off = 32; off >= 16; off >>= 1)
+  for (int k = 0; k < CM; ++k) all = S::larger(all, col[k]);
+  if (S::odd(all)) v.finite_maxima(row, col);
+  if (!TILES) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        most[k] = max(most[k], (uint32_t)__shfl_xor((int)most[k], off, kWave));
+    for (int i = 0; i < RM; ++i) {
+      row[i] = S::larger(row[i], turned_row<8>(row[i]));
+      row[i] = S::larger(row[i], turned_row<4>(row[i]));
+      row[i] = S::larger(row[i], turned_row<2>(row[i]));
+      row[i] = S::larger(row[i], turned_row<1>(row[i]));
+    }
+  }
+  if (TILES || q.by_col.data) {
+#pragma unroll
+    for (int k = 0; k < CM; ++k) {
+      col[k] = S::larger(col[k], (uint32_t)__shfl_xor((int)col[k], 16, kWave));
+      col[k] = S::larger(col[k], (uint32_t)__shfl_xor((int)col[k], 32, kWave));
+    }
     if ((tid & 63) < 16)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) col_most[wave][tc + k] = most[k];
+      for (int k = 0; k < CM; ++k) col_most[wave][tid & 15][k] = col[k];
   }
   if (q.sums) {
     float s[8];
@@ -99,7 +224,7 @@ __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
     for (int k = 0; k < 8; ++k) {
       s[k] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[k] += v[i][k];
+      for (int i = 0; i < 8; ++i) s[k] += v.value(i, k);
     }
 #pragma unroll
     for (int off = 16; off <= 32; off <<= 1)
@@ -109,79 +234,73 @@ __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) col_sum[wave][tc + k] = s[k];
   }
-  uint32_t row_byte[8], col_byte[8];
-  if (TILES || q.data_t || q.sums) __syncthreads();
-  if (TILES || q.data_t) {
-    uint32_t all = 0;
+  if (TILES || q.by_col.data || q.sums) __syncthreads();
+  if (TILES || q.by_col.data) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) m = max(m, col_most[w][tc + k]);
-      col_byte[k] = scale_byte(m);
-      all = max(all, m);
-    }
-    if (TILES) {
-#pragma unroll
-      for (int off = 8; off >= 1; off >>= 1) all = max(all, (uint32_t)__shfl_xor((int)all, off, kWave));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) col_byte[k] = row_byte[k] = scale_byte(all);
-    }
+    for (int k = 0; k < CM; ++k)
+      col[k] = S::larger(S::larger(col_most[0][tid & 15][k], col_most[1][tid & 15][k]),
+                         S::larger(col_most[2][tid & 15][k], col_most[3][tid & 15][k]));
   }
-  if (!TILES)
+  uint32_t tile_byte = 0;
+  if (TILES) {
+    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row_byte[i] = scale_byte(row_most[i]);
+    for (int k = 0; k < 8; ++k) most = max(most, S::bits(col, k));
+    most = max(most, turned_row<8>(most));
+    most = max(most, turned_row<4>(most));
+    most = max(most, turned_row<2>(most));
+    most = max(most, turned_row<1>(most));
+    tile_byte = scale_byte(most);
+  }
   if (q.sums && tid < kTile && c0 + tid < q.cols)
     q.sums[r0 / kTile * q.cols + c0 + tid] =
         (col_sum[0][tid] + col_sum[1][tid]) + (col_sum[2][tid] + col_sum[3][tid]);
-  if (q.data) {
+  if (q.by_row.data) {
+    uint8_t* out = q.by_row.data + (r0 + tr) * q.by_row.ld;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float inv = power(254 - row_byte[i]);
-      u32x2 w;
-      w[0] = pack4(v[i][0], v[i][1], v[i][2], v[i][3], inv);
-      w[1] = pack4(v[i][4], v[i][5], v[i][6], v[i][7], inv);
-      if (r0 + tr + i < q.rows)
-        *reinterpret_cast<u32x2*>(q.data + (r0 + tr + i) * q.data_ld + c0 + tc) = w;
-      if (tid % 16 == 0) row_bytes[tr + i] = (uint8_t)row_byte[i];
+    for (int i = 0; i < 8; ++i, out += q.by_row.ld) {
+      const uint32_t byte = TILES ? tile_byte : scale_byte(S::bits(row, i));
+      const u32x2 w = v.row_codes(i, power(byte));
+      if (r0 + tr + i < q.rows) {
+        if (q.by_row.expanded)
+          *reinterpret_cast<bf16x8*>(out + 2 * (c0 + tc)) = expand(w[0], w[1], half_power(byte));
+        else
+          *reinterpret_cast<u32x2*>(out + c0 + tc) = w;
+      }
+      if (tid % 16 == 0) row_bytes[tr + i] = (uint8_t)byte;
     }
   }
-  if (q.data_t) {
+  if (q.by_col.data) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float inv = power(254 - col_byte[k]);
-      u32x2 w;
-      w[0] = pack4(v[0][k], v[1][k], v[2][k], v[3][k], inv);
-      w[1] = pack4(v[4][k], v[5][k], v[6][k], v[7][k], inv);
-      *reinterpret_cast<u32x2*>(turned + (tc + k) * kPitch + tr) = w;
+      const uint32_t byte = TILES ? tile_byte : scale_byte(S::bits(col, k));
+      const u32x2 w = v.col_codes(k, power(byte));
+      turned[(tc + k) * kPitch + tr / 4] = w[0];
+      turned[(tc + k) * kPitch + tr / 4 + 1] = w[1];
+      if (tid < 16) col_bytes[tc + k] = (uint8_t)byte;
     }
-    if (tid < 16)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) col_bytes[tc + k] = (uint8_t)col_byte[k];
   }
   __syncthreads();
-  if (q.data && tid < kTile && r0 + tid < q.scale_ld)
-    q.scale[c0 / kTile * q.scale_ld + r0 + tid] = row_bytes[tid];
-  if (q.data_t && q.expand_t) {
+  if (q.by_row.data && !q.by_row.expanded && tid < kTile && r0 + tid < q.by_row.scale_ld)
+    q.by_row.scale[c0 / kTile * q.by_row.scale_ld + r0 + tid] = row_bytes[tid];
+  if (!q.by_col.data) return;
+  if (!q.by_col.expanded && tid < kTile && c0 + tid < q.by_col.scale_ld)
+    q.by_col.scale[r0 / kTile * q.by_col.scale_ld + c0 + tid] = col_bytes[tid];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = j * 32 + tid / 8, at = tid % 8 * 16;
-      if (c0 + c >= q.cols) continue;
-      const u32x4 w = *reinterpret_cast<const u32x4*>(turned + c * kPitch + at);
-      const float scale = half_power(col_bytes[c]);
-      bf16x8* out = reinterpret_cast<bf16x8*>(q.data_t + (c0 + c) * q.data_t_ld + 2 * (r0 + at));
-      out[0] = expand(w[0], w[1], scale);
-      out[1] = expand(w[2], w[3], scale);
-    }
-  } else if (q.data_t) {
-    if (tid < kTile && c0 + tid < q.scale_t_ld)
-      q.scale_t[r0 / kTile * q.scale_t_ld + c0 + tid] = col_bytes[tid];
+  for (int j = 0; j < 4; ++j) {
+    const int c = j * 32 + tid / 8, word = tid % 8 * 4;
+    if (c0 + c >= q.cols) continue;
+    u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = j * 32 + tid / 8, at = tid % 8 * 16;
-      if (c0 + c < q.cols)
-        *reinterpret_cast<u32x4*>(q.data_t + (c0 + c) * q.data_t_ld + r0 + at) =
-            *reinterpret_cast<const u32x4*>(turned + c * kPitch + at);
+    for (int k = 0; k < 4; ++k) w[k] = turned[c * kPitch + word + k];
+    uint8_t* out = q.by_col.data + (c0 + c) * q.by_col.ld;
+    if (q.by_col.expanded) {
+      const float half = half_power(col_bytes[c]);
+      bf16x8* to = reinterpret_cast<bf16x8*>(out + 2 * (r0 + 4 * word));
+      to[0] = expand(w[0], w[1], half);
+      to[1] = expand(w[2], w[3], half);
+    } else {
+      *reinterpret_cast<u32x4*>(out + r0 + 4 * word) = w;
     }
   }
 }
@@ -201,15 +320,23 @@ __global__ __launch_bounds__(256) void float8_expand_kernel(const uint8_t* data,
   to[1] = expand(w[2], w[3], s);
 }
 
-// out[c] = the parts' sums in order.
+// out[c] = the parts' sums: 4 threads a column, a quarter of the parts each in order, then
+// (0 + 1) + (2 + 3).
 template <typename T>
 __global__ __launch_bounds__(256) void sum_parts_kernel(const float* parts, int64_t count,
                                                         int64_t cols, T* out) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+  __shared__ float quarter[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane, per = (count + 3) / 4;
+  const int64_t last = min(count, (w + 1) * per);
   float s = 0.f;
-  for (int64_t i = 0; i < count; ++i) s += parts[i * cols + c];
-  out[c] = (T)s;
+  if (c < cols)
+#pragma unroll 8
+    for (int64_t i = w * per; i < last; ++i) s += parts[i * cols + c];
+  quarter[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && c < cols)
+    out[c] = (T)((quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]));
 }
 
 template <typename T>
@@ -231,27 +358,34 @@ extern "C" {
 int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
                           int32_t tiles, void* data, int64_t data_ld, void* scale,
                           int64_t scale_ld, void* data_t, int64_t data_t_ld, void* scale_t,
-                          int64_t scale_t_ld, int32_t expand_t, float* sums, hipStream_t stream) {
+                          int64_t scale_t_ld, int32_t expanded, float* sums, hipStream_t stream) {
   DIONW_REQUIRE(elem == kF16 || elem == kBF16 || elem == kF32, "float8_quantize: bad element type %d", elem);
   DIONW_REQUIRE(rows >= 0 && cols >= 0, "float8_quantize: negative extent");
   if (rows == 0 || cols == 0) return kOk;
   DIONW_REQUIRE(data || data_t || sums, "float8_quantize: no output");
   DIONW_REQUIRE(x && ld >= cols, "float8_quantize: bad input");
-  auto fits = [](const void* d, int64_t d_ld, const void* s, int64_t s_ld, int64_t r, int64_t c) {
-    return !d || (s && d_ld >= round_up(c, kTile) && d_ld % 16 == 0 && s_ld >= r && aligned16(d));
+  const bool row_expanded = expanded & 1, col_expanded = expanded & 2;
+  auto fits = [](const void* d, int64_t d_ld, const void* s, int64_t s_ld, int64_t r, int64_t c, bool e) {
+    return !d || (d_ld >= round_up(c, kTile) && d_ld % 16 == 0 && aligned16(d) && (e || (s && s_ld >= r)));
   };
-  DIONW_REQUIRE(fits(data, data_ld, scale, scale_ld, rows, cols) &&
-                    fits(data_t, data_t_ld, expand_t ? x : scale_t, expand_t ? cols : scale_t_ld, cols, rows),
+  DIONW_REQUIRE(fits(data, data_ld, scale, scale_ld, rows, cols, row_expanded) &&
+                    fits(data_t, data_t_ld, scale_t, scale_t_ld, cols, rows, col_expanded),
                 "float8_quantize: an output is too small or not aligned");
   const int64_t tr = ceil_div(rows, kTile), tc = ceil_div(cols, kTile);
   DIONW_REQUIRE(tr < INT32_MAX / tc, "float8_quantize: too many tiles");
   const int64_t size = elem == kF32 ? 4 : 2;
-  QuantizeArgs q{x,       rows,     cols,    ld,
-                 static_cast<uint8_t*>(data),   data_ld,   static_cast<uint8_t*>(scale),   scale_ld,
-                 static_cast<uint8_t*>(data_t), expand_t ? 2 * data_t_ld : data_t_ld,
-                 static_cast<uint8_t*>(scale_t), scale_t_ld,
-                 sums,    (int32_t)tc,
-                 aligned16(x) && ld * size % 16 == 0, expand_t};
+  QuantizeArgs q{};
+  q.x = x;
+  q.rows = rows;
+  q.cols = cols;
+  q.ld = ld;
+  q.by_row = {static_cast<uint8_t*>(data), row_expanded ? 2 * data_ld : data_ld,
+              static_cast<uint8_t*>(scale), scale_ld, row_expanded};
+  q.by_col = {static_cast<uint8_t*>(data_t), col_expanded ? 2 * data_t_ld : data_t_ld,
+              static_cast<uint8_t*>(scale_t), scale_t_ld, col_expanded};
+  q.sums = sums;
+  q.tiles_c = (int32_t)tc;
+  q.vec = aligned16(x) && ld * size % 16 == 0;
   const unsigned grid = (unsigned)(tr * tc);
   if (elem == kF16) return launch_quantize<_Float16>(q, tiles != 0, grid, stream);
   if (elem == kBF16) return launch_quantize<__bf16>(q, tiles != 0, grid, stream);
@@ -280,8 +414,8 @@ int dionw_sum_parts(const float* parts, int64_t count, int64_t cols, int32_t ele
   DIONW_REQUIRE(count >= 0 && cols >= 0, "sum_parts: negative extent");
   if (cols == 0) return kOk;
   DIONW_REQUIRE(out && (parts || count == 0), "sum_parts: null pointer");
-  DIONW_REQUIRE(ceil_div(cols, 256) < INT32_MAX, "sum_parts: too many columns");
-  const dim3 grid((unsigned)ceil_div(cols, 256));
+  DIONW_REQUIRE(ceil_div(cols, 64) < INT32_MAX, "sum_parts: too many columns");
+  const dim3 grid((unsigned)ceil_div(cols, 64));
   if (elem == kF16)
     hipLaunchKernelGGL(sum_parts_kernel<_Float16>, grid, dim3(256), 0, stream, parts, count, cols,
                        static_cast<_Float16*>(out));

@@ -17,8 +17,10 @@ An input that is not finite becomes NaN and leaves its block's scale alone.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Any, Final
 
 import torch
@@ -94,14 +96,10 @@ def _empty(rows: int, cols: int, device: torch.device) -> Float8Matrix:
         torch.empty(depth // TILE, -(-rows // 16) * 16, dtype=torch.uint8, device=device), cols)
 
 
-def _expanded(rows: int, cols: int, device: torch.device) -> Tensor:
-    return torch.empty(rows, -(-cols // TILE) * TILE, dtype=torch.bfloat16, device=device)
-
-
 def _expand(q: Float8Matrix) -> Tensor:
     """The matrix as a product summed in float32 reads it: bfloat16 halves of the values."""
     rows, depth = q.data.shape
-    out = _expanded(rows, depth, q.device)
+    out = torch.empty(rows, depth, dtype=torch.bfloat16, device=q.device)
     _lib.call("dionw_float8_expand", q.data.data_ptr(), depth, q.scale.data_ptr(), q.scale.shape[1],
               rows, depth, out.data_ptr(), depth, _lib.stream_handle(q.device))
     return out
@@ -130,29 +128,26 @@ def _readable(x: Tensor) -> Tensor:
     return x if adjacent and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
 
 
+def _pitch(x: Tensor) -> int:
+    """Elements between the rows of a readable matrix."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
 def _quantize(x: Tensor, tiles: bool, rows: bool, columns: bool, sums: torch.dtype | None = None,
-              *, expand: bool = False,
-              ) -> tuple[Float8Matrix | None, Float8Matrix | Tensor | None, Tensor | None]:
-    """x quantized by rows, its transpose quantized by rows (``expand``: its codes expanded, as a
-    product summed in float32 reads them), and its column sums, as asked."""
+              ) -> tuple[Float8Matrix | None, Float8Matrix | None, Tensor | None]:
+    """x quantized by rows, its transpose quantized by rows, and its column sums, as asked."""
     x = _readable(x)
     m, n = x.shape
     stream = _lib.stream_handle(x.device)
     by_row = _empty(m, n, x.device) if rows else None
-    by_column: Float8Matrix | Tensor | None = None
-    if columns:
-        by_column = _expanded(n, m, x.device) if expand else _empty(n, m, x.device)
+    by_column = _empty(n, m, x.device) if columns else None
     parts = torch.empty(-(-m // TILE), n, device=x.device) if sums else None
-    ld = x.stride(0) if m > 1 else n
-
-    def place(q: Float8Matrix | Tensor | None) -> tuple[Any, ...]:
-        if isinstance(q, Tensor):
-            return q.data_ptr(), q.shape[1], None, 0
+    def place(q: Float8Matrix | None) -> tuple[Any, ...]:
         return (None, 0, None, 0) if q is None else (
             q.data.data_ptr(), q.data.shape[1], q.scale.data_ptr(), q.scale.shape[1])
 
-    _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, max(ld, n),
-              int(tiles), *place(by_row), *place(by_column), int(expand), _lib.ptr(parts), stream)
+    _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, _pitch(x),
+              int(tiles), *place(by_row), *place(by_column), 0, _lib.ptr(parts), stream)
     total = None
     if sums:
         total = torch.empty(n, dtype=sums, device=x.device)
@@ -208,39 +203,78 @@ def _bias(bias: Tensor | None, n: int, device: torch.device) -> Tensor | None:
     return bias.detach().to(torch.float32).contiguous()
 
 
+@lru_cache(maxsize=256)
+def _sizes(x_code: int, w_code: int, m: int, n: int, k: int, need_x: bool, need_w: bool,
+           need_b: bool) -> tuple[int, int, int]:
+    """Bytes of what the forward saves and of both passes' scratch."""
+    sizes = (ctypes.c_size_t * 3)()
+    _lib.library().dionw_float8_linear_sizes(x_code, w_code, m, n, k, need_x, need_w, need_b, sizes)
+    return sizes[0], sizes[1], sizes[2]
+
+
+def _scratch(size: int, device: torch.device) -> Tensor | None:
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
 class _Linear(torch.autograd.Function):
     """y = x W^T + b; dx = dy W, dW = dy^T x, db = the sum of dy over the rows."""
 
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
-        need_x, need_w = ctx.needs_input_grad[:2]
-        xq, xt, _ = _quantize(x, False, True, need_w)
-        wq, wt, _ = _quantize(weight, True, True, need_x)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.dtypes, ctx.sizes = (x.dtype, weight.dtype), (x.shape[0], *weight.shape)
-        ctx.save_for_backward(*(t for q in (xt, wt) if q is not None for t in (q.data, q.scale)))
-        return float8_matmul(xq, wq, bias, dtype=x.dtype)
+        need_x, need_w, need_b = ctx.needs_input_grad
+        x, weight = _readable(x), _readable(weight)
+        m, k = x.shape
+        n, device, dtype = weight.shape[0], x.device, x.dtype
+        codes = _lib.elem_code(dtype), _lib.elem_code(weight.dtype)
+        stream = _lib.stream_handle(device)
+        keep, room, ctx.room = _sizes(*codes, m, n, k, need_x, need_w, need_b)
+        saved, scratch = _scratch(keep, device), _scratch(room, device)
+        y = torch.empty(m, n, dtype=dtype, device=device)
+        _lib.call("dionw_float8_linear_forward", codes[0], x.data_ptr(), _pitch(x), codes[1],
+                  weight.data_ptr(), _pitch(weight), _lib.ptr(_bias(bias, n, device)), m, n, k,
+                  need_x, need_w, y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
+        ctx.codes, ctx.sizes, ctx.dtypes = codes, (m, n, k), (dtype, weight.dtype)
+        ctx.bias_dtype = bias.dtype if need_b else None
+        ctx.save_for_backward(*([] if saved is None else [saved]))
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, dy: Tensor) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
         need_x, need_w, need_b = ctx.needs_input_grad
         m, n, k = ctx.sizes
-        saved = list(ctx.saved_tensors)
-        xt = Float8Matrix(*saved[:2], m) if need_w else None
-        wt = Float8Matrix(*saved[-2:], n) if need_x else None
-        exact = ctx.dtypes[1] is torch.float32
-        rows, columns, db = _quantize(dy, False, need_x, need_w, ctx.bias_dtype if need_b else None,
-                                      expand=exact)
-        dx = float8_matmul(rows, wt, dtype=ctx.dtypes[0]) if need_x else None
-        dw = None
-        if need_w and exact:
-            ex = _expand(xt)
-            dw = _product(n, k, ex.shape[1], (columns.data_ptr(), None, 0), (ex.data_ptr(), None, 0),
-                          None, torch.float32, dy.device)
-        elif need_w:
-            dw = float8_matmul(columns, xt, dtype=ctx.dtypes[1])
+        dy, device = _readable(dy), dy.device
+        saved = ctx.saved_tensors[0] if ctx.saved_tensors else None
+        scratch = _scratch(ctx.room, device)
+        dx = torch.empty(m, k, dtype=ctx.dtypes[0], device=device) if need_x else None
+        dw = torch.empty(n, k, dtype=ctx.dtypes[1], device=device) if need_w else None
+        db = torch.empty(n, dtype=ctx.bias_dtype, device=device) if need_b else None
+        _lib.call("dionw_float8_linear_backward", ctx.codes[0], dy.data_ptr(), _pitch(dy), ctx.codes[1],
+                  m, n, k, need_x, need_w, _lib.ptr(saved), _lib.ptr(dx), _lib.ptr(dw),
+                  _lib.elem_code(ctx.bias_dtype) if need_b else 0, _lib.ptr(db), _lib.ptr(scratch),
+                  ctx.room, _lib.stream_handle(device))
         return dx, dw, db
+
+
+@lru_cache(maxsize=256)
+def _kept_scratch(code: int, m: int, n: int, k: int) -> int:
+    return _lib.library().dionw_float8_linear_kept_scratch(code, m, n, k)
+
+
+def _kept_linear(x: Tensor, weight: Float8Matrix, bias: Tensor | None) -> Tensor:
+    x = _readable(x)
+    m, k = x.shape
+    data, scale, device = weight.data, weight.scale, x.device
+    n, code = data.shape[0], _lib.elem_code(x.dtype)
+    stream = _lib.stream_handle(device)
+    bias = _bias(bias, n, device)
+    room = _kept_scratch(code, m, n, k)
+    scratch = _scratch(room, device)
+    y = torch.empty(m, n, dtype=x.dtype, device=device)
+    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), _pitch(x), data.data_ptr(), data.shape[1],
+              scale.data_ptr(), scale.shape[1], _lib.ptr(bias), m, n, k, y.data_ptr(),
+              _lib.ptr(scratch), room, stream)
+    return y
 
 
 def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None = None) -> Tensor:
@@ -265,7 +299,7 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ValueError("a Float8Matrix weight is for inference: pass the float weight where "
                              "gradients are needed, or call under torch.no_grad()")
-        out = float8_matmul(float8_quantize(flat), weight, bias, dtype=x.dtype)
+        out = _kept_linear(flat, weight, bias)
     else:
         _bias(bias, weight.shape[0], x.device)
         out = _Linear.apply(flat, weight, bias)

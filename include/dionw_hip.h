@@ -346,17 +346,18 @@ int dionw_adamw_8bit_values(const int64_t* numels, const int64_t* first_blocks, 
  * into data/scale by rows, and into data_t/scale_t as the transpose [cols, rows]; either may
  * be NULL. One scale for each row (of the transpose: column of x) and block of 128, or for
  * each 128 x 128 tile when tiles != 0. Values that are not finite become NaN and leave their
- * block's scale alone. expand_t != 0: data_t takes bfloat16 halves of the values (see
- * dionw_float8_expand; data_t_ld in elements) and scale_t is not used. sums (may be NULL): float32 [ceil(rows / 128)][cols], the column sums
+ * block's scale alone. expanded: bit 0 for data, bit 1 for data_t: they take bfloat16 halves of
+ * the values (see dionw_float8_expand; pitches in elements) and the scales are not used. sums (may be NULL): float32 [ceil(rows / 128)][cols], the column sums
  * of each 128 rows.
  */
 int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
                           int32_t tiles, void* data, int64_t data_ld, void* scale,
                           int64_t scale_ld, void* data_t, int64_t data_t_ld, void* scale_t,
-                          int64_t scale_t_ld, int32_t expand_t, float* sums,
+                          int64_t scale_t_ld, int32_t expanded, float* sums,
                           dionw_stream_t stream);
 
-/* out[c] = parts[0][c] + parts[1][c] + ... in order, in element code elem. */
+/* out[c] = parts[0][c] + parts[1][c] + ..., a quarter of them at a time, in a fixed order, in
+ * element code elem. */
 int dionw_sum_parts(const float* parts, int64_t count, int64_t cols, int32_t elem, void* out,
                     dionw_stream_t stream);
 
@@ -385,6 +386,39 @@ int dionw_float8_gemm(int32_t expanded, int64_t m, int64_t n, int64_t depth, con
                       int64_t ldb, const void* b_scale, int64_t b_scale_ld, const float* bias,
                       int32_t elem, void* c, int64_t ldc, void* workspace, size_t workspace_bytes,
                       dionw_stream_t stream);
+
+/*
+ * A linear layer on 8-bit operands: y [m, n] = x [m, k] W [n, k]^T + bias in x's element code
+ * (x_elem), from float x and W (pitches in elements). x is quantized by rows, W by tiles.
+ * saved (NULL where both needs are 0) keeps, for the backward, W's transpose (need_x) and x's
+ * (need_w) in codes. The backward gives dx (x_elem) = dy W when need_x, dw (w_elem) = dy^T x
+ * when need_w, dy quantized by rows and by columns, and db (bias_elem) = the column sums of dy
+ * when db is not NULL; float32 results are summed in float32, 16-bit ones on the 8-bit
+ * instructions (dionw_float8_gemm). dionw_float8_linear_sizes writes the bytes of saved and of
+ * the two calls' scratch.
+ */
+void dionw_float8_linear_sizes(int32_t x_elem, int32_t w_elem, int64_t m, int64_t n, int64_t k,
+                               int32_t need_x, int32_t need_w, int32_t need_b, size_t* sizes);
+int dionw_float8_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int32_t w_elem,
+                                const void* w, int64_t w_ld, const float* bias, int64_t m,
+                                int64_t n, int64_t k, int32_t need_x, int32_t need_w, void* y,
+                                void* saved, void* scratch, size_t scratch_bytes,
+                                dionw_stream_t stream);
+int dionw_float8_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, int32_t w_elem,
+                                 int64_t m, int64_t n, int64_t k, int32_t need_x, int32_t need_w,
+                                 const void* saved, void* dx, void* dw, int32_t bias_elem,
+                                 void* db, void* scratch, size_t scratch_bytes,
+                                 dionw_stream_t stream);
+
+/*
+ * The same y from a kept W: codes [n][w_ld] with their scales [ceil(k / 128)][w_scale_ld]. Up
+ * to 16 rows of x are quantized by the product itself, in one launch and no scratch.
+ */
+size_t dionw_float8_linear_kept_scratch(int32_t x_elem, int64_t m, int64_t n, int64_t k);
+int dionw_float8_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const void* w,
+                             int64_t w_ld, const void* w_scale, int64_t w_scale_ld,
+                             const float* bias, int64_t m, int64_t n, int64_t k, void* y,
+                             void* scratch, size_t scratch_bytes, dionw_stream_t stream);
 
 /*
  * GPU EMA of float32 sources: shadow = lerp(shadow, source, weight), or a
