@@ -155,17 +155,17 @@ def adamw_8bit_step(group: dict[str, Any], pack: AdamWPack) -> None:
     grads: list[int] = []
     held: list[Tensor] = []  # converted tensors, alive until the launch is queued
     copies: list[tuple[Tensor, Tensor]] = []
-    float32 = torch.float32
-    device = pack.exp_avg.device
+    float32, device, index = torch.float32, pack.exp_avg.device, pack.exp_avg.get_device()
     for place, param in enumerate(pack.params):
         grad = param.grad
         if grad is None:
             continue
         if param.dtype is not float32:
             raise TypeError(f"the HIP AdamW takes float32 parameters, got {param.dtype}")
-        if grad.device != device or param.device != device or grad.shape != param.shape:
+        if (grad.get_device() != index or param.get_device() != index or grad.shape != param.shape
+                or param.numel() != pack.numels[place]):
             raise ValueError("an 8-bit AdamW parameter and its gradient lie on the state's device "
-                             "and have one shape")
+                             "and have one shape, the one the state was made for")
         if grad.dtype is not float32 or not grad.is_contiguous():
             grad = grad.to(float32).contiguous()
             held.append(grad)

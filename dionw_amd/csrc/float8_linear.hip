@@ -202,17 +202,23 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
   }
 }
 
+// R rows' fragments a wave and W waves a workgroup: many fragments take 64 rows each (x is read and
+// quantized once for them), few the most workgroups. us in a chain of launches (an empty one takes
+// 4), R W = 1 8 / 2 8 / 4 4: 1024 x 4096 5.3 / 8.1 / 13.5, 4096 x 4096 6.8 / 8.7 / 14.1, 4096 x 14336 15.0 /
+// 24.3 / 41.5, 6144 x 4096 9.6 / 9.2 / 14.4, 8192 x 4096 10.5 / 9.9 / 14.8, 10240 x 4096 13.3 / 14.9 / 15.2,
+// 14336 x 4096 (8 rows of x) 20.4 / 17.4 / 16.7, 128256 x 4096 112 / 100 / 96, with 16 rows 181 / 138 / 119.
 template <typename T>
 int launch_few(const FewArgs& g, hipStream_t stream) {
-  constexpr int kWide = sizeof(T) == 4 ? 8 : 16;  // float32 blocks take too many registers for 16 waves
   const int fragments = (g.n + 15) / 16;
   const bool whole = g.k % kTile == 0 && aligned16(g.x) && g.x_ld * (int64_t)sizeof(T) % 16 == 0;
   if (!whole)
     hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, false>), dim3(fragments), dim3(512), 0, stream, g);
-  else if (fragments <= 1024)
-    hipLaunchKernelGGL((float8_few_kernel<T, 1, kWide, true>), dim3(fragments), dim3(kWide * 64), 0, stream, g);
-  else
+  else if (fragments < 320 || (fragments > 512 && fragments < 768))
+    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, true>), dim3(fragments), dim3(512), 0, stream, g);
+  else if (fragments <= 512)
     hipLaunchKernelGGL((float8_few_kernel<T, 2, 8, true>), dim3((fragments + 1) / 2), dim3(512), 0, stream, g);
+  else
+    hipLaunchKernelGGL((float8_few_kernel<T, 4, 4, true>), dim3((fragments + 3) / 4), dim3(256), 0, stream, g);
   return check_launch("float8_few");
 }
 

@@ -262,16 +262,26 @@ def _kept_scratch(code: int, m: int, n: int, k: int) -> int:
 
 
 def _kept_linear(x: Tensor, weight: Float8Matrix, bias: Tensor | None) -> Tensor:
-    x = _readable(x)
-    m, k = x.shape
-    data, scale, device = weight.data, weight.scale, x.device
-    n, code = data.shape[0], _lib.elem_code(x.dtype)
+    data, scale, k, dtype = weight.data, weight.scale, weight.cols, x.dtype
+    device, shape = data.device, x.shape
+    n, depth = data.shape
+    if not shape or shape[-1] != k or x.device != device or dtype not in _DTYPES:
+        raise ValueError(f"float8_linear takes float x [..., {k}] on {device} for this weight, got "
+                         f"{dtype} {tuple(shape)} on {x.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError("a Float8Matrix weight is for inference: pass the float weight where "
+                         "gradients are needed, or call under torch.no_grad()")
     stream = _lib.stream_handle(device)
+    if len(shape) != 2:
+        x = x.reshape(math.prod(shape[:-1]), k)
+    if not x.is_contiguous():
+        x = _readable(x)
+    m, code = x.shape[0], _lib.elem_code(dtype)
     bias = _bias(bias, n, device)
     room = _kept_scratch(code, m, n, k)
     scratch = _scratch(room, device)
-    y = torch.empty(m, n, dtype=x.dtype, device=device)
-    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), _pitch(x), data.data_ptr(), data.shape[1],
+    y = torch.empty((*shape[:-1], n), dtype=dtype, device=device)
+    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), _pitch(x), data.data_ptr(), depth,
               scale.data_ptr(), scale.shape[1], _lib.ptr(bias), m, n, k, y.data_ptr(),
               _lib.ptr(scratch), room, stream)
     return y
@@ -289,21 +299,19 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
         ValueError: For shapes or types that do not fit, tensors off the GPU, or an x that
             requires a gradient beside a ``Float8Matrix``.
     """
-    if x.dim() == 0 or x.shape[-1] != weight.shape[-1] or len(weight.shape) != 2:
+    if isinstance(weight, Float8Matrix):
+        return _kept_linear(x, weight, bias)
+    shape = x.shape
+    if not shape or weight.dim() != 2 or shape[-1] != weight.shape[1]:
         raise ValueError(f"float8_linear takes x [..., in] and a weight [out, in], got "
-                         f"{tuple(x.shape)} and {tuple(weight.shape)}")
+                         f"{tuple(shape)} and {tuple(weight.shape)}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    flat = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
-    if isinstance(weight, Float8Matrix):
-        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-            raise ValueError("a Float8Matrix weight is for inference: pass the float weight where "
-                             "gradients are needed, or call under torch.no_grad()")
-        out = _kept_linear(flat, weight, bias)
-    else:
-        _bias(bias, weight.shape[0], x.device)
-        out = _Linear.apply(flat, weight, bias)
-    return out.view(*x.shape[:-1], weight.shape[0])
+    _bias(bias, weight.shape[0], x.device)
+    if len(shape) == 2:
+        return _Linear.apply(x, weight, bias)
+    flat = x.reshape(math.prod(shape[:-1]), shape[-1])
+    return _Linear.apply(flat, weight, bias).view(*shape[:-1], weight.shape[0])
 
 
 class Float8Linear(nn.Linear):

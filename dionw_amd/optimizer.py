@@ -23,6 +23,8 @@ from __future__ import annotations
 from collections.abc import Callable, Iterable, Iterator
 from contextlib import contextmanager
 from contextvars import ContextVar
+from itertools import groupby
+from operator import itemgetter
 from typing import Any, TypeVar
 
 import torch
@@ -136,6 +138,7 @@ class Dion(IntegratedEMAOptimizer):
                              "beta1": betas[0], "beta2": betas[1]})
         self._packed: list[Bucket] | None = None
         self._adamw_packs: dict[int, list[AdamWPack]] = {}  # by group: the 8-bit ones
+        self._adamw_places: dict[Tensor, tuple[AdamWPack, int]] = {}  # their parameters
         # The key is left out where nothing asks for it, so that checkpoints stay the reference's.
         more = ({} if adamw_state is AdamWState.FLOAT32
                 else {ADAMW_STATE_KEY: AdamWState(adamw_state).value})
@@ -186,7 +189,10 @@ class Dion(IntegratedEMAOptimizer):
         # every parameter; matrix state appears with the buckets.
         if spec.kind is RouteKind.ADAMW:
             if spec.adamw_state is AdamWState.EIGHT_BIT:
-                self._adamw_packs[len(self.param_groups) - 1] = pack_adamw(params, self.state)
+                packs = pack_adamw(params, self.state)
+                self._adamw_packs[len(self.param_groups) - 1] = packs
+                self._adamw_places.update((param, (pack, place)) for pack in packs
+                                          for place, param in enumerate(pack.params))
                 return
             for param in params:
                 init_adamw_state(param, self.state[param])
@@ -232,24 +238,20 @@ class Dion(IntegratedEMAOptimizer):
             ValueError: Without a parameter, for one that no 8-bit AdamW group of this
                 optimizer holds, or for parameters of several devices.
         """
-        held = {id(p): (pack, place) for packs in self._adamw_packs.values() for pack in packs
-                for place, p in enumerate(pack.params)}
         params = list(params)
-        if not params or any(id(p) not in held for p in params):
+        held = [self._adamw_places.get(p) for p in params]
+        if not params or None in held:
             raise ValueError("adamw_moments takes parameters of this optimizer's 8-bit AdamW "
                              f"groups ({ADAMW_STATE_KEY!r}: {AdamWState.EIGHT_BIT.value!r})")
-        device = params[0].device
-        if any(p.device != device for p in params):
+        device = held[0][0].exp_avg.device
+        if any(pack.exp_avg.device != device for pack, _ in held):
             raise ValueError("adamw_moments takes parameters of one device")
-        total = sum(p.numel() for p in params)
+        total = sum(pack.numels[place] for pack, place in held)
         exp_avg, rms = torch.empty(total, device=device), torch.empty(total, device=device)
-        at = start = 0
-        while start < len(params):
-            pack, places, size = held[id(params[start])][0], [], 0
-            while start < len(params) and held[id(params[start])][0] is pack:
-                places.append(held[id(params[start])][1])
-                size += params[start].numel()
-                start += 1
+        at = 0
+        for pack, run in groupby(held, key=itemgetter(0)):  # a launch for tensors of one pack
+            places = [place for _, place in run]
+            size = sum(pack.numels[place] for place in places)
             if size:
                 pack.moments(places, exp_avg[at:at + size], rms[at:at + size])
             at += size
