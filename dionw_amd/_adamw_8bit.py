@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes
 from collections.abc import Sequence
 from enum import Enum
+from operator import attrgetter
 from typing import Any, Final
 
 import torch
@@ -38,6 +39,8 @@ from dionw_amd.ema._fusion import ACTIVE_EMA
 __all__ = ["AdamWPack", "AdamWState", "adamw_8bit_step", "pack_adamw"]
 
 BLOCK: Final = 256  # elements that share a scale
+_FLOAT32: Final = {torch.float32}
+_DTYPE, _SHAPE = attrgetter("dtype"), attrgetter("shape")
 
 
 class AdamWState(Enum):
@@ -52,6 +55,7 @@ class AdamWPack:
 
     Attributes:
         params: The tensors, ordered as in their group.
+        numels, shapes: Their sizes when the state was made.
         first_blocks: Each tensor's first 256-element block.
     """
 
@@ -59,6 +63,7 @@ class AdamWPack:
         device = params[0].device
         self.params = list(params)
         self.numels = [p.numel() for p in self.params]
+        self.shapes = [p.shape for p in self.params]
         self.first_blocks = []
         blocks = 0
         for numel in self.numels:
@@ -83,9 +88,7 @@ class AdamWPack:
 
     def tables_of(self, places: list[int]) -> tuple[Any, Any, Any]:
         """Host tables of sizes, first blocks and ids of the tensors at ``places``."""
-        if places == self.every:
-            return self.tables
-        return self._tables(places)
+        return self.tables if places == self.every else self._tables(places)
 
     def views(self, place: int) -> dict[str, Tensor]:
         """The state entries of the tensor at ``place``."""
@@ -149,44 +152,39 @@ def adamw_8bit_step(group: dict[str, Any], pack: AdamWPack) -> None:
         TypeError: For a parameter that is not float32.
         ValueError: For a gradient of another device or size than its parameter.
     """
-    places: list[int] = []
-    params: list[Tensor] = []
-    targets: list[int] = []
-    grads: list[int] = []
-    held: list[Tensor] = []  # converted tensors, alive until the launch is queued
+    device = pack.exp_avg.device
     copies: list[tuple[Tensor, Tensor]] = []
-    float32, device, index = torch.float32, pack.exp_avg.device, pack.exp_avg.get_device()
-    for place, param in enumerate(pack.params):
-        grad = param.grad
-        if grad is None:
-            continue
-        if param.dtype is not float32:
-            raise TypeError(f"the HIP AdamW takes float32 parameters, got {param.dtype}")
-        if (grad.get_device() != index or param.get_device() != index or grad.shape != param.shape
-                or param.numel() != pack.numels[place]):
-            raise ValueError("an 8-bit AdamW parameter and its gradient lie on the state's device "
-                             "and have one shape, the one the state was made for")
-        if grad.dtype is not float32 or not grad.is_contiguous():
-            grad = grad.to(float32).contiguous()
-            held.append(grad)
-        target = param
-        if not param.is_contiguous():
-            # The state is in row-major order: step a row-major copy and write it back.
-            target = param.data.contiguous()
-            copies.append((param.data, target))
-        places.append(place)
-        params.append(param)
-        targets.append(target.data_ptr())
-        grads.append(grad.data_ptr())
+    params, places = pack.params, pack.every
+    grads = [param.grad for param in params]
+    if any(grad is None for grad in grads):
+        places = [place for place in places if grads[place] is not None]
+        params = [params[place] for place in places]
+        grads = [grads[place] for place in places]
     if not places:
         return
+    dtypes = set(map(_DTYPE, params))
+    if dtypes != _FLOAT32:
+        raise TypeError(f"the HIP AdamW takes float32 parameters, got {dtypes}")
+    shapes = pack.shapes if places is pack.every else [pack.shapes[place] for place in places]
+    if (set(map(Tensor.get_device, params)) | set(map(Tensor.get_device, grads))
+            != {pack.exp_avg.get_device()}
+            or list(map(_SHAPE, grads)) != shapes or list(map(_SHAPE, params)) != shapes):
+        raise ValueError("an 8-bit AdamW parameter and its gradient lie on the state's device "
+                         "and have the shape that the state was made for")
+    if set(map(_DTYPE, grads)) != _FLOAT32 or not all(map(Tensor.is_contiguous, grads)):
+        grads = [grad.to(torch.float32).contiguous() for grad in grads]
+    targets: Sequence[Tensor] = params
+    if not all(map(Tensor.is_contiguous, params)):
+        # The state is in row-major order: step row-major copies and write them back.
+        targets = [param.data.contiguous() for param in params]
+        copies = [(param.data, target) for param, target in zip(params, targets)
+                  if not param.is_contiguous()]
     count = len(places)
-    pointers = ctypes.c_void_p * count
     ema = ACTIVE_EMA.get()
     shadows = ema.fusable_shadows(params) if ema is not None and not copies else None
     beta1, beta2 = group["betas"]
     numels, first_blocks, ids = pack.tables_of(places)
-    _lib.call("dionw_adamw_8bit", pointers(*targets), pointers(*grads),
+    _lib.call("dionw_adamw_8bit", _lib.ptr_array(targets), _lib.ptr_array(grads),
               None if shadows is None else _lib.ptr_array(shadows), numels, first_blocks, ids,
               count, pack.blocks, len(pack.params), pack.exp_avg.data_ptr(),
               pack.exp_avg_scale.data_ptr(), pack.rms.data_ptr(), pack.rms_scale.data_ptr(),

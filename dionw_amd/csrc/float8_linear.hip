@@ -9,15 +9,19 @@ namespace {
 
 // ---- a few rows ----------------------------------------------------------------------
 //
-// y = x W^T + b for up to 16 rows of x (the tokens being decoded): every byte of W passes once,
-// from memory to registers, and x is quantized on the way, so that the call is one launch. A
-// workgroup takes 16 R rows of W; its waves take the blocks of 128 columns in turn and add their
+// y = x W^T + b for 16 rows of x at a time (the tokens being decoded): every byte of W passes
+// once, from memory to registers, and x is quantized on the way, so that the call is one launch.
+// A workgroup takes 16 R rows of W; its waves take the blocks of 128 columns in turn and add their
 // sums through LDS, in a fixed order. Of a block, a lane holds one token's (or weight row's)
 // chunks of 16 at places G = lane / 16 and 4 + G, so that each load of a wave covers 64 bytes of
 // 16 rows; the block's largest magnitude is one of 4 lanes', two exchanges. A wave reads the next
 // block while it multiplies one.
 // Bound: HBM, n k bytes of W; the smallest calls: launch and the latency of two dependent reads.
-constexpr int kFew = 16;
+//
+// 16-bit calls of more rows quantize x first and go through the tiles. float32 ones would expand W
+// for that, 5 bytes of traffic for each of its codes, so up to 64 rows they run as groups of 16 here,
+// W coming from the caches after the first.
+constexpr int kFew = 16, kFewFloat = 64;
 
 struct FewArgs {
   const void* x;
@@ -118,8 +122,8 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
   __shared__ f32x4 sums[W][R][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int G = lane >> 4, i16 = lane & 15;
-  const int n0 = blockIdx.x * 16 * R;
-  const T* x = reinterpret_cast<const T*>(g.x) + min(i16, g.m - 1) * g.x_ld;
+  const int n0 = blockIdx.x * 16 * R, token = blockIdx.y * 16 + i16;
+  const T* x = reinterpret_cast<const T*>(g.x) + min(token, g.m - 1) * g.x_ld;
   const uint8_t* w[R];
   int row[R];
 #pragma unroll
@@ -184,14 +188,14 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
 #pragma unroll
     for (int v = 1; v < W; ++v) s += sums[v][t][lane];
     const int n = n0 + 16 * t + 4 * G;
-    if (i16 >= g.m || n >= g.n) continue;
+    if (token >= g.m || n >= g.n) continue;
     typedef T t4 __attribute__((ext_vector_type(4)));
     typedef T t4any __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     t4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       o[e] = (T)((kExact ? kExpanded : 1.f) * s[e] + (g.bias ? g.bias[min(n + e, g.n - 1)] : 0.f));
-    T* y = reinterpret_cast<T*>(g.y) + (int64_t)i16 * g.n + n;
+    T* y = reinterpret_cast<T*>(g.y) + (int64_t)token * g.n + n;
     if (n + 4 <= g.n) {
       *reinterpret_cast<t4any*>(y) = o;
     } else {
@@ -210,15 +214,16 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
 template <typename T>
 int launch_few(const FewArgs& g, hipStream_t stream) {
   const int fragments = (g.n + 15) / 16;
+  const unsigned groups = (unsigned)(g.m + 15) / 16;
   const bool whole = g.k % kTile == 0 && aligned16(g.x) && g.x_ld * (int64_t)sizeof(T) % 16 == 0;
   if (!whole)
-    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, false>), dim3(fragments), dim3(512), 0, stream, g);
+    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, false>), dim3(fragments, groups), dim3(512), 0, stream, g);
   else if (fragments < 320 || (fragments > 512 && fragments < 768))
-    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, true>), dim3(fragments), dim3(512), 0, stream, g);
+    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, true>), dim3(fragments, groups), dim3(512), 0, stream, g);
   else if (fragments <= 512)
-    hipLaunchKernelGGL((float8_few_kernel<T, 2, 8, true>), dim3((fragments + 1) / 2), dim3(512), 0, stream, g);
+    hipLaunchKernelGGL((float8_few_kernel<T, 2, 8, true>), dim3((fragments + 1) / 2, groups), dim3(512), 0, stream, g);
   else
-    hipLaunchKernelGGL((float8_few_kernel<T, 4, 4, true>), dim3((fragments + 3) / 4), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((float8_few_kernel<T, 4, 4, true>), dim3((fragments + 3) / 4, groups), dim3(256), 0, stream, g);
   return check_launch("float8_few");
 }
 
@@ -389,7 +394,7 @@ int dionw_float8_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
 }
 
 size_t dionw_float8_linear_kept_scratch(int32_t x_elem, int64_t m, int64_t n, int64_t k) {
-  if (m <= kFew && k > 0) return 0;
+  if (m <= (x_elem == kF32 ? kFewFloat : kFew) && k > 0) return 0;
   Parts room{nullptr};
   if (x_elem == kF32) {
     Forward f(room, true, m, n, k);
@@ -413,7 +418,7 @@ int dionw_float8_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const 
                     aligned16(scratch),
                 "float8_linear: an operand is too small or not aligned");
   const Matrix weight{const_cast<void*>(w), const_cast<void*>(w_scale), n, depth, w_scale_ld};
-  if (m <= kFew && k > 0) {
+  if (m <= (x_elem == kF32 ? kFewFloat : kFew) && k > 0) {
     DIONW_REQUIRE(depth / kTile < INT32_MAX / 2, "float8_linear: depth too large");
     const FewArgs g{x, x_ld, static_cast<const uint8_t*>(w), w_ld, static_cast<const uint8_t*>(w_scale),
                     w_scale_ld, bias, y, k, (int32_t)m, (int32_t)n, (int32_t)(depth / kTile)};
