@@ -25,6 +25,7 @@ from dionw_amd.float8 import (
     float8_linear,
     float8_matmul,
     float8_quantize,
+    float8_quantize_both,
 )
 from dionw_amd.matrix_update import (
     DION3_UPDATE,
@@ -78,5 +79,6 @@ __all__ = [
     "float8_linear",
     "float8_matmul",
     "float8_quantize",
+    "float8_quantize_both",
     "param_groups",
 ]

@@ -24,7 +24,9 @@ __device__ __forceinline__ float power(uint32_t byte) { return __uint_as_float(b
 // Codes are expanded to bfloat16 with half their scale, as 448 x 2^120 (what a block of
 // magnitudes up to the largest float32 may round to) is past bfloat16. Sums of products of
 // two expanded operands take kExpanded back.
-__device__ __forceinline__ float half_power(uint32_t byte) { return __uint_as_float((byte - 1) << 23); }
+__device__ __forceinline__ float half_power(uint32_t byte) {
+  return __uint_as_float((max(byte, 1u) - 1) << 23);  // exponent 0 scales by 2^-127
+}
 constexpr float kExpanded = 4.f;
 
 // Eight codes and their scale as bfloat16, exactly (a code has 4 significant bits).

@@ -10,7 +10,7 @@ bits, largest 448) where a product reads them, and 16-bit results come from the 
   column and 128 rows), the weight with one per 128 x 128 tile, whose transpose holds the same
   values. ``weight`` may also be a ``Float8Matrix`` (inference with the 8-bit copy alone).
 - ``Float8Linear``: ``nn.Linear`` with that product.
-- ``float8_quantize`` / ``float8_matmul``: its parts.
+- ``float8_quantize`` / ``float8_quantize_both`` / ``float8_matmul``: its parts.
 
 An input that is not finite becomes NaN and leaves its block's scale alone.
 """
@@ -29,7 +29,8 @@ from torch.autograd.function import once_differentiable
 
 from dionw_amd import _lib
 
-__all__ = ["Float8Linear", "Float8Matrix", "float8_linear", "float8_matmul", "float8_quantize"]
+__all__ = ["Float8Linear", "Float8Matrix", "float8_linear", "float8_matmul", "float8_quantize",
+           "float8_quantize_both"]
 
 TILE: Final = 128  # columns (and rows) that share a scale
 _DTYPES: Final = (torch.float16, torch.bfloat16, torch.float32)
@@ -43,7 +44,7 @@ class Float8Matrix:
         data: float8_e4m3fn codes ``[rows, depth]``, ``depth`` being ``cols`` rounded up to
             128; the columns past ``cols`` hold zeros.
         scale: uint8 ``[depth / 128, rows rounded up to 16 or more]``: the exponent bytes of
-            the float32 scales, by column block.
+            the (normal) float32 scales, 1 to 254, by column block.
         cols: The number of columns.
 
     Raises:
@@ -133,27 +134,20 @@ def _pitch(x: Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _quantize(x: Tensor, tiles: bool, rows: bool, columns: bool, sums: torch.dtype | None = None,
-              ) -> tuple[Float8Matrix | None, Float8Matrix | None, Tensor | None]:
-    """x quantized by rows, its transpose quantized by rows, and its column sums, as asked."""
+def _quantize(x: Tensor, tiles: bool, both: bool) -> tuple[Float8Matrix, Float8Matrix | None]:
+    """x quantized by rows, and its transpose quantized by rows where both are asked for."""
     x = _readable(x)
     m, n = x.shape
     stream = _lib.stream_handle(x.device)
-    by_row = _empty(m, n, x.device) if rows else None
-    by_column = _empty(n, m, x.device) if columns else None
-    parts = torch.empty(-(-m // TILE), n, device=x.device) if sums else None
+    by_row = _empty(m, n, x.device)
+    by_column = _empty(n, m, x.device) if both else None
     def place(q: Float8Matrix | None) -> tuple[Any, ...]:
         return (None, 0, None, 0) if q is None else (
             q.data.data_ptr(), q.data.shape[1], q.scale.data_ptr(), q.scale.shape[1])
 
     _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, _pitch(x),
-              int(tiles), *place(by_row), *place(by_column), 0, _lib.ptr(parts), stream)
-    total = None
-    if sums:
-        total = torch.empty(n, dtype=sums, device=x.device)
-        _lib.call("dionw_sum_parts", parts.data_ptr(), parts.shape[0], n, _lib.elem_code(sums),
-                  total.data_ptr(), stream)
-    return by_row, by_column, total
+              int(tiles), *place(by_row), *place(by_column), 0, None, stream)
+    return by_row, by_column
 
 
 def float8_quantize(x: Tensor, *, tiles: bool = False) -> Float8Matrix:
@@ -163,7 +157,18 @@ def float8_quantize(x: Tensor, *, tiles: bool = False) -> Float8Matrix:
     Raises:
         ValueError: For another shape or type, or a tensor off the GPU.
     """
-    return _quantize(x.detach(), tiles, True, False)[0]
+    return _quantize(x.detach(), tiles, False)[0]
+
+
+def float8_quantize_both(x: Tensor, *, tiles: bool = False) -> tuple[Float8Matrix, Float8Matrix]:
+    """``float8_quantize`` of x and of its transpose, from one reading of x: what a product and its
+    gradients take. With ``tiles`` both hold the same values.
+
+    Raises:
+        ValueError: For another shape or type, or a tensor off the GPU.
+    """
+    by_row, by_column = _quantize(x.detach(), tiles, True)
+    return by_row, by_column
 
 
 def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, *,

@@ -238,9 +238,8 @@ class Dion(IntegratedEMAOptimizer):
             ValueError: Without a parameter, for one that no 8-bit AdamW group of this
                 optimizer holds, or for parameters of several devices.
         """
-        params = list(params)
         held = [self._adamw_places.get(p) for p in params]
-        if not params or None in held:
+        if not held or None in held:
             raise ValueError("adamw_moments takes parameters of this optimizer's 8-bit AdamW "
                              f"groups ({ADAMW_STATE_KEY!r}: {AdamWState.EIGHT_BIT.value!r})")
         device = held[0][0].exp_avg.device

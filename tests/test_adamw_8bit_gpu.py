@@ -297,6 +297,29 @@ def test_a_saved_state_resumes_bit_for_bit(tmp_path) -> None:
             assert torch.equal(p, q)
 
 
+def test_a_saved_state_with_an_ema_resumes_bit_for_bit() -> None:
+    params = _tensors([(30, 40), 777])
+    opt = _optimizer(params, ema=EMAConfig(decay=0.9))
+    for k in range(3):
+        _grads(params, k)
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    twin = _optimizer(twins, ema=EMAConfig(decay=0.9))
+    twin.load_state_dict(saved)
+    for k in range(3, 6):
+        _grads(params, k)
+        for p, q in zip(params, twins):
+            q.grad = p.grad.clone()
+        opt.step()
+        twin.step()
+        for p, q in zip(params, twins):
+            assert torch.equal(p, q)
+            assert torch.equal(opt.state[p]["ema_shadow"], twin.state[q]["ema_shadow"])
+    # Two optimizers that share a loaded dict share no state.
+    assert twin.state[twins[0]]["exp_avg"].data_ptr() != opt.state[params[0]]["exp_avg"].data_ptr()
+
+
 def test_states_of_another_kind_are_refused() -> None:
     params = _tensors([100])
     eight = _optimizer(params)

@@ -19,8 +19,8 @@ from dionw_amd import (
     float8_linear,
     float8_matmul,
     float8_quantize,
+    float8_quantize_both,
 )
-from dionw_amd.float8 import _quantize
 from tests import float8_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -60,7 +60,7 @@ SHAPES = [(1, 1), (1, 128), (128, 1), (127, 129), (128, 128), (200, 300), (3, 10
 @pytest.mark.parametrize("tiles", [False, True])
 def test_quantization_is_the_definitions(shape, dtype, tiles) -> None:
     x = _random(*shape, 1, dtype)
-    rows, columns, sums = _quantize(x, tiles, True, True, torch.float32)
+    rows, columns = float8_quantize_both(x, tiles=tiles)
     for got, source in ((rows, x), (columns, x.t())):
         values, byte = oracle.quantize(source, oracle.TILE if tiles else 1)
         assert got.shape == tuple(source.shape)
@@ -68,8 +68,17 @@ def test_quantization_is_the_definitions(shape, dtype, tiles) -> None:
         assert torch.equal(got.values().cpu().double(), values)
         assert not got.data[:, got.cols:].view(torch.uint8).any()
     assert torch.equal(float8_quantize(x, tiles=tiles).data.view(torch.uint8), rows.data.view(torch.uint8))
-    exact = x.double().sum(0)
-    bound = (shape[0] + 1) * 2.0 ** -24 * x.double().abs().sum(0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_biass_gradient_is_the_sum_of_the_rows(shape, dtype) -> None:
+    dy = _random(*shape, 1, dtype)
+    x, w = torch.ones(shape[0], 8, device="cuda", dtype=dtype), torch.ones(shape[1], 8, device="cuda")
+    b = torch.zeros(shape[1], device="cuda", requires_grad=True)
+    (sums,) = torch.autograd.grad(float8_linear(x, w, b), (b,), dy)
+    exact = dy.double().sum(0)
+    bound = (shape[0] + 1) * 2.0 ** -24 * dy.double().abs().sum(0)
     assert bool(((sums.double() - exact).abs() <= bound).all())
 
 
@@ -194,6 +203,28 @@ def test_the_layer_trains(size, dtype) -> None:
     _check(w.grad, oracle.quantize(dy.t())[0], oracle.quantize(x.t())[0])
     exact = dy.double().sum(0)
     assert bool(((b.grad.double() - exact).abs() <= (m + 1) * 2.0 ** -24 * dy.double().abs().sum(0)).all())
+
+
+@pytest.mark.parametrize("kinds", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.bfloat16),
+                                   (torch.float32, torch.float16)], ids=str)
+def test_weights_and_biases_of_16_bits(kinds) -> None:
+    """Gradients come in the weight's and the bias's own types."""
+    dtype, held = kinds
+    m, k, n = 300, 260, 130
+    x = _random(m, k, 7, spread=0.5).to(dtype).requires_grad_()
+    w = (_random(n, k, 8, spread=0.3) * k ** -0.5).to(held).requires_grad_()
+    b = torch.randn(n, device="cuda").to(held).requires_grad_()
+    dy = (_random(m, n, 9, spread=0.5) * 1e-2).to(dtype)
+    y = float8_linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert (dx.dtype, dw.dtype, db.dtype) == (dtype, held, held)
+    (xq, _), (wq, _) = oracle.quantize(x), oracle.quantize(w, oracle.TILE)
+    _check(y, xq, wq, b)
+    _check(dx, oracle.quantize(dy)[0], wq.T.contiguous())
+    _check(dw, oracle.quantize(dy.t())[0], oracle.quantize(x.t())[0])
+    exact = dy.double().sum(0)
+    bound = (m + 1) * 2.0 ** -24 * dy.double().abs().sum(0)
+    assert bool(((db.double() - exact).abs() <= bound + UNIT[held] * (exact.abs() + bound)).all())
 
 
 def test_only_the_gradients_asked_for() -> None:
