@@ -10,6 +10,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+// 16 bytes of a row that may start at any element: the hardware takes such loads whole.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kTile = 128;  // columns (and rows) that share a scale
 

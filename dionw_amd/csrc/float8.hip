@@ -38,7 +38,6 @@ struct QuantizeArgs {
   Output by_row, by_col;  // x, and its transpose
   float* sums;            // [row tiles][cols]: each tile's column sums, or null
   int32_t tiles_c;
-  int32_t vec;            // rows start at multiples of 16 bytes
 };
 
 // A thread's 8 x 8 values and what the kernel asks of them.
@@ -48,7 +47,7 @@ struct Square {  // 16-bit
   static constexpr int kRowMost = 4, kColMost = 4;  // words of maxima: two rows, two columns each
   uint32_t w[8][4];
   __device__ __forceinline__ void load(int i, const T* at) {
-    const u32x4 v = *reinterpret_cast<const u32x4*>(at);
+    const u32x4 v = *reinterpret_cast<const u32x4_any*>(at);
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[i][k] = v[k];
   }
@@ -121,7 +120,7 @@ struct Square<float> {
   __device__ __forceinline__ void load(int i, const float* at) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const u32x4 v = reinterpret_cast<const u32x4*>(at)[h];
+      const u32x4 v = *reinterpret_cast<const u32x4_any*>(at + 4 * h);
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[i][4 * h + k] = v[k];
     }
@@ -203,7 +202,7 @@ __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
   const int tr = tid / 16 * 8, tc = tid % 16 * 8;  // the thread's first row and column
   S v;
   const T* at = reinterpret_cast<const T*>(q.x) + (r0 + tr) * q.ld + c0 + tc;
-  if (q.vec && r0 + tr + 8 <= q.rows && c0 + tc + 8 <= q.cols) {
+  if (r0 + tr + 8 <= q.rows && c0 + tc + 8 <= q.cols) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v.load(i, at + i * q.ld);
   } else {
@@ -335,7 +334,7 @@ __global__ __launch_bounds__(256) void float8_quantize_rows_kernel(QuantizeArgs 
   if (row >= q.rows) return;  // a row's 16 lanes together
   Line<T> v;
   const T* at = reinterpret_cast<const T*>(q.x) + row * q.ld + c;
-  if (q.vec && c + 8 <= q.cols) v.load(at);
+  if (c + 8 <= q.cols) v.load(at);
   else v.load(at, q.cols - c);
   uint32_t most = v.most();
   most = max(most, turned_row<8>(most));
@@ -428,7 +427,6 @@ int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t col
                 "float8_quantize: an output is too small or not aligned");
   const int64_t tr = ceil_div(rows, kTile), tc = ceil_div(cols, kTile);
   DIONW_REQUIRE(tr < INT32_MAX / tc, "float8_quantize: too many tiles");
-  const int64_t size = elem == kF32 ? 4 : 2;
   QuantizeArgs q{};
   q.x = x;
   q.rows = rows;
@@ -440,7 +438,6 @@ int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t col
               static_cast<uint8_t*>(scale_t), scale_t_ld, col_expanded};
   q.sums = sums;
   q.tiles_c = (int32_t)tc;
-  q.vec = aligned16(x) && ld * size % 16 == 0;
   const unsigned grid = (unsigned)(tr * tc);
   if (elem == kF16) return launch_quantize<_Float16>(q, tiles != 0, grid, stream);
   if (elem == kBF16) return launch_quantize<__bf16>(q, tiles != 0, grid, stream);

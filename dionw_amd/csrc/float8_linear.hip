@@ -41,8 +41,7 @@ template <typename T>
 struct Values {
   static constexpr int kWords = 8 * sizeof(T);
   uint32_t w[kWords];
-  // `left`: columns from the block's first one on, at least 1 (WHOLE: 128, at a multiple of 16
-  // bytes).
+  // `left`: columns from the block's first one on, at least 1 (WHOLE: 128).
   template <bool WHOLE>
   __device__ __forceinline__ void load(const T* block, int G, int left) {
     constexpr int kHalf = kWords / 2;
@@ -52,7 +51,7 @@ struct Values {
       if constexpr (WHOLE) {
 #pragma unroll
         for (int v = 0; v < kHalf / 4; ++v) {
-          const u32x4 r = reinterpret_cast<const u32x4*>(block + c)[v];
+          const u32x4 r = *reinterpret_cast<const u32x4_any*>(block + c + 16 / sizeof(T) * v);
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[h * kHalf + 4 * v + e] = r[e];
         }
@@ -143,7 +142,10 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
       b.w[r][1] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w[r] + (int64_t)kb * kTile + 64));
       b.byte[r] = g.w_scale[kb * g.w_scale_ld + row[r]];
     }
-    b.x.template load<WHOLE>(x + (int64_t)kb * kTile, G, (int)min((int64_t)kTile, g.k - (int64_t)kb * kTile));
+    if (WHOLE || kb < g.blocks - 1)
+      b.x.template load<true>(x + (int64_t)kb * kTile, G, kTile);
+    else
+      b.x.template load<false>(x + (int64_t)kb * kTile, G, (int)(g.k - (int64_t)kb * kTile));
   };
   f32x4 acc[R];
 #pragma unroll
@@ -211,20 +213,23 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
 // 4), R W = 1 8 / 2 8 / 4 4: 1024 x 4096 5.3 / 8.1 / 13.5, 4096 x 4096 6.8 / 8.7 / 14.1, 4096 x 14336 15.0 /
 // 24.3 / 41.5, 6144 x 4096 9.6 / 9.2 / 14.4, 8192 x 4096 10.5 / 9.9 / 14.8, 10240 x 4096 13.3 / 14.9 / 15.2,
 // 14336 x 4096 (8 rows of x) 20.4 / 17.4 / 16.7, 128256 x 4096 112 / 100 / 96, with 16 rows 181 / 138 / 119.
-template <typename T>
+template <typename T, bool WHOLE>
 int launch_few(const FewArgs& g, hipStream_t stream) {
   const int fragments = (g.n + 15) / 16;
   const unsigned groups = (unsigned)(g.m + 15) / 16;
-  const bool whole = g.k % kTile == 0 && aligned16(g.x) && g.x_ld * (int64_t)sizeof(T) % 16 == 0;
-  if (!whole)
-    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, false>), dim3(fragments, groups), dim3(512), 0, stream, g);
-  else if (fragments < 320 || (fragments > 512 && fragments < 768))
-    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, true>), dim3(fragments, groups), dim3(512), 0, stream, g);
+  if (fragments < 320 || (fragments > 512 && fragments < 768))
+    hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, WHOLE>), dim3(fragments, groups), dim3(512), 0, stream, g);
   else if (fragments <= 512)
-    hipLaunchKernelGGL((float8_few_kernel<T, 2, 8, true>), dim3((fragments + 1) / 2, groups), dim3(512), 0, stream, g);
+    hipLaunchKernelGGL((float8_few_kernel<T, 2, 8, WHOLE>), dim3((fragments + 1) / 2, groups), dim3(512), 0, stream, g);
   else
-    hipLaunchKernelGGL((float8_few_kernel<T, 4, 4, true>), dim3((fragments + 3) / 4, groups), dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((float8_few_kernel<T, 4, 4, WHOLE>), dim3((fragments + 3) / 4, groups), dim3(256), 0, stream, g);
   return check_launch("float8_few");
+}
+
+// WHOLE: the depth is a multiple of 128, so that no block needs its columns counted.
+template <typename T>
+int launch_few(const FewArgs& g, hipStream_t stream) {
+  return g.k % kTile ? launch_few<T, false>(g, stream) : launch_few<T, true>(g, stream);
 }
 
 // ---- scratch ---------------------------------------------------------------------------
