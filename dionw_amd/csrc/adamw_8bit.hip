@@ -28,7 +28,9 @@
 // parameter is NaN at this step or the next) and takes no part in its block's scales.
 //
 // Bound: HBM, 16 B an element (p read and written, g read, two codes read and written)
-// against 28 with float32 moments.
+// against 28 with float32 moments. A wave loads 4 blocks of 256 before its first store, the
+// division of work that streams the float32 pass best. 525 M elements: 1464 us (5.74 TB/s; the
+// float32 pass 2580), 38.6 M: 112 us; the moments' values (2 B read, 8 written) 965 and 66 us.
 #include "common.h"
 
 #include <cmath>
