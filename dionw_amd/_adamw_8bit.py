@@ -40,7 +40,8 @@ __all__ = ["AdamWPack", "AdamWState", "adamw_8bit_step", "pack_adamw"]
 
 BLOCK: Final = 256  # elements that share a scale
 _FLOAT32: Final = {torch.float32}
-_DTYPE, _SHAPE = attrgetter("dtype"), attrgetter("shape")
+_DTYPE, _SHAPE, _GRAD = attrgetter("dtype"), attrgetter("shape"), attrgetter("grad")
+_NONE: Final = type(None)
 
 
 class AdamWState(Enum):
@@ -155,8 +156,8 @@ def adamw_8bit_step(group: dict[str, Any], pack: AdamWPack) -> None:
     device = pack.exp_avg.device
     copies: list[tuple[Tensor, Tensor]] = []
     params, places = pack.params, pack.every
-    grads = [param.grad for param in params]
-    if any(grad is None for grad in grads):
+    grads = list(map(_GRAD, params))
+    if _NONE in set(map(type, grads)):
         places = [place for place in places if grads[place] is not None]
         params = [params[place] for place in places]
         grads = [grads[place] for place in places]

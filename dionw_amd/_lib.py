@@ -215,7 +215,7 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
 
 def ptr_array(tensors: Sequence[torch.Tensor]) -> ctypes.Array[ctypes.c_void_p]:
     """A host array of the tensors' device addresses."""
-    return (ctypes.c_void_p * max(len(tensors), 1))(*[t.data_ptr() for t in tensors])
+    return (ctypes.c_void_p * max(len(tensors), 1))(*map(torch.Tensor.data_ptr, tensors))
 
 
 def int64_array(values: Sequence[int]) -> ctypes.Array[ctypes.c_int64]:

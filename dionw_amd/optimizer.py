@@ -238,19 +238,22 @@ class Dion(IntegratedEMAOptimizer):
             ValueError: Without a parameter, for one that no 8-bit AdamW group of this
                 optimizer holds, or for parameters of several devices.
         """
-        held = [self._adamw_places.get(p) for p in params]
+        held = list(map(self._adamw_places.get, params))
         if not held or None in held:
             raise ValueError("adamw_moments takes parameters of this optimizer's 8-bit AdamW "
                              f"groups ({ADAMW_STATE_KEY!r}: {AdamWState.EIGHT_BIT.value!r})")
+        packs = set(map(itemgetter(0), held))
         device = held[0][0].exp_avg.device
-        if any(pack.exp_avg.device != device for pack, _ in held):
+        if any(pack.exp_avg.device != device for pack in packs):
             raise ValueError("adamw_moments takes parameters of one device")
-        total = sum(pack.numels[place] for pack, place in held)
+        runs = []  # a launch for each run of tensors of one pack: (pack, places, elements)
+        for pack, run in groupby(held, key=itemgetter(0)) if len(packs) > 1 else [(held[0][0], held)]:
+            places = list(map(itemgetter(1), run))
+            runs.append((pack, places, sum(map(pack.numels.__getitem__, places))))
+        total = sum(size for _, _, size in runs)
         exp_avg, rms = torch.empty(total, device=device), torch.empty(total, device=device)
         at = 0
-        for pack, run in groupby(held, key=itemgetter(0)):  # a launch for tensors of one pack
-            places = [place for _, place in run]
-            size = sum(pack.numels[place] for place in places)
+        for pack, places, size in runs:
             if size:
                 pack.moments(places, exp_avg[at:at + size], rms[at:at + size])
             at += size
