@@ -14,6 +14,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kTile = 128;  // columns (and rows) that share a scale
+// A product's operand has rows of fewer bytes: a tile's rows are addressed with 32-bit offsets.
+constexpr int64_t kRowBytes = 1 << 23;
 
 // The scale's exponent byte of a block whose largest finite magnitude has the bits `largest`
 // (at least 1: the scale and its reciprocal are normal).

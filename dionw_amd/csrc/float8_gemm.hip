@@ -110,7 +110,7 @@ __device__ __forceinline__ i32x8 chunks(const unsigned char* lo, const unsigned 
 // the tile's `side` repeated. Even waves load the first operand's and odd ones the second's
 // (several the same bytes), so that every wave issues one load. A block's bytes run to a
 // multiple of 16, so a lane's 4 are in bounds; past the last it takes the last 4. All of them
-// lie within 2^32 bytes, as there are 128 codes to each.
+// lie within 2^32 bytes (checked).
 struct ScaleLoad {
 #ifdef __HIP_DEVICE_COMPILE__
   __amdgpu_buffer_rsrc_t rsrc;
@@ -814,7 +814,7 @@ int dionw_float8_gemm(int32_t expanded, int64_t m, int64_t n, int64_t depth, con
   DIONW_REQUIRE(c && ldc >= n, "float8_gemm: bad output");
   const int64_t size = expanded ? 2 : 1, row = depth * size;
   // A tile's rows are addressed with 32-bit offsets from its first one.
-  DIONW_REQUIRE(lda >= depth && ldb >= depth && lda * size < (1 << 23) && ldb * size < (1 << 23),
+  DIONW_REQUIRE(lda >= depth && ldb >= depth && lda * size < kRowBytes && ldb * size < kRowBytes,
                 "float8_gemm: operands need rows of at least their depth, of less than 8 MB");
   DIONW_REQUIRE(lda * size % 16 == 0 && ldb * size % 16 == 0 && aligned16(a) && aligned16(b),
                 "float8_gemm: operands need rows at multiples of 16 bytes");
@@ -824,6 +824,8 @@ int dionw_float8_gemm(int32_t expanded, int64_t m, int64_t n, int64_t depth, con
   };
   DIONW_REQUIRE(expanded || depth == 0 || (scaled(a_scale, a_scale_ld, m) && scaled(b_scale, b_scale_ld, n)),
                 "float8_gemm: codes need a scale for each row, at a pitch that is a multiple of 16");
+  DIONW_REQUIRE(expanded || std::max(a_scale_ld, b_scale_ld) <= UINT32_MAX / std::max<int64_t>(row / 128, 1),
+                "float8_gemm: a matrix's scales need to lie within 4 GB");
   const Plan p = depth ? plan(m, n, row / 128) : Plan{kSmall, 1, 1};
   DIONW_REQUIRE(p.splits == 1 ||
                     (workspace && workspace_bytes >= (size_t)p.splits * m * n * sizeof(float) &&

@@ -331,6 +331,11 @@ int product(bool expanded, const Matrix& a, const Matrix& b, const float* bias, 
                            stream);
 }
 
+// Whether an operand of that many columns is one the products take, for results of type `elem`.
+bool fits_row(int64_t cols, int32_t elem) {
+  return cols < kRowBytes && round_up(cols, kTile) * (elem == kF32 ? 2 : 1) < kRowBytes;
+}
+
 bool good_elem(int32_t e) { return e == kF16 || e == kBF16 || e == kF32; }
 
 }  // namespace
@@ -359,6 +364,9 @@ int dionw_float8_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int
   DIONW_REQUIRE(good_elem(x_elem) && good_elem(w_elem), "float8_linear: bad element type");
   DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0, "float8_linear: negative extent");
   DIONW_REQUIRE(saved || !(need_x || need_w) || n == 0 || k == 0, "float8_linear: no room to save");
+  // The gradients sum over n and m: refused here rather than after the forward pass.
+  DIONW_REQUIRE((!need_x || fits_row(n, x_elem)) && (!need_w || fits_row(m, w_elem)),
+                "float8_linear: a gradient's product takes rows of less than 8 MB");
   DIONW_REQUIRE(aligned16(saved) && aligned16(scratch), "float8_linear: buffers need 16-byte alignment");
   Parts kept{static_cast<uint8_t*>(saved)}, room{static_cast<uint8_t*>(scratch)};
   const bool exact = x_elem == kF32;

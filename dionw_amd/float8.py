@@ -301,8 +301,9 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     ``Float8Matrix`` for inference.
 
     Raises:
-        ValueError: For shapes or types that do not fit, tensors off the GPU, or an x that
-            requires a gradient beside a ``Float8Matrix``.
+        ValueError: For shapes or types that do not fit, tensors off the GPU, an x that
+            requires a gradient beside a ``Float8Matrix``, or sums of 8 M products (4 M for a
+            float32 result) and more, a gradient's included.
     """
     if isinstance(weight, Float8Matrix):
         return _kept_linear(x, weight, bias)

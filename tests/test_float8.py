@@ -95,6 +95,8 @@ def test_the_library_checks_its_arguments() -> None:
                 {"elem": 2}, {"elem": 3}, {"expanded": 1}, {"c": None}, {"ldc": 3}, {"lda": 1 << 23}):
         with pytest.raises(ValueError):
             gemm(**bad)
+    with pytest.raises(ValueError, match="4 GB"):  # 2 blocks' scales at a pitch of 2 GB
+        gemm(a_scale_ld=1 << 31)
     # A depth that is split needs its workspace.
     size = _lib.library().dionw_float8_gemm_workspace(0, 64, 64, 1 << 16)
     assert size > 0
@@ -107,3 +109,16 @@ def test_the_library_checks_its_arguments() -> None:
     for bad in ({"data": None}, {"data": 8}, {"data_ld": 128}, {"scale_ld": 3}, {"depth": 130}, {"out_ld": 255}):
         with pytest.raises(ValueError):
             expand(**bad)
+
+
+def test_a_forward_refuses_what_its_gradients_could_not_sum() -> None:
+    """Products take rows of less than 8 MB: a layer whose gradients need longer ones says so first."""
+    def forward(m, n, w_elem, need_x, need_w):
+        _lib.call("dionw_float8_linear_forward", 1, 16, 128, w_elem, 16, 128, None, m, n, 128, need_x,
+                  need_w, 16, 16, None, 0, None)
+
+    for bad in ((1 << 23, 4, 1, 0, 1), (1 << 22, 4, 2, 0, 1), (4, 1 << 23, 1, 1, 0), (1 << 62, 4, 1, 0, 1)):
+        with pytest.raises(ValueError, match="8 MB"):
+            forward(*bad)
+    with pytest.raises(ValueError, match="scratch"):
+        forward(1 << 22, 4, 1, 0, 1)
