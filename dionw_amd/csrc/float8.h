@@ -17,6 +17,28 @@ constexpr int kTile = 128;  // columns (and rows) that share a scale
 // A product's operand has rows of fewer bytes: a tile's rows are addressed with 32-bit offsets.
 constexpr int64_t kRowBytes = 1 << 23;
 
+// Codes with their scales, or (scale null) expanded codes; data null: nothing.
+struct Matrix {
+  void* data;
+  void* scale;
+  int64_t rows, depth, scale_ld;
+};
+
+// What dionw_float8_quantize does to one matrix.
+struct Quantization {
+  int32_t elem;
+  const void* x;
+  int64_t rows, cols, ld;
+  Matrix by_row, by_col;
+  float* sums;
+};
+// x by rows and columns and w by tiles, in one launch.
+int quantize_pair(const Quantization& x, const Quantization& w, hipStream_t stream);
+// x by rows and columns, and beside it, in the same launch, the codes of `from` expanded into `to`
+// where it has room.
+int quantize_and_expand(const Quantization& x, const Matrix (&from)[2], const Matrix (&to)[2],
+                        hipStream_t stream);
+
 // The scale's exponent byte of a block whose largest finite magnitude has the bits `largest`
 // (at least 1: the scale and its reciprocal are normal).
 __device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {

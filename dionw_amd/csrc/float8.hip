@@ -16,6 +16,9 @@
 namespace dionw {
 namespace {
 
+// The most workgroups of 256 a launch takes (2^32 threads).
+constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;
+
 // ---- quantization ------------------------------------------------------------------
 //
 // A workgroup takes a 128 x 128 tile: thread t the rows 8 (t / 16) .. + 7 and the columns
@@ -187,20 +190,29 @@ struct Line {
   __device__ __forceinline__ u32x2 codes(float scale) const { return s.row_codes(0, scale); }
 };
 
-template <typename T, bool TILES>
-__global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
-  using S = Square<T>;
-  constexpr int RM = S::kRowMost, CM = S::kColMost;
+// A workgroup's LDS.
+struct Shared {
   // Bytes of the transpose: 33 words a row, so that the 16 columns x 4 row groups of a wave's
   // 8-byte writes spread over the banks.
-  constexpr int kPitch = 33;
-  __shared__ uint32_t turned[kTile * kPitch];
-  __shared__ uint32_t col_most[4][16][CM];
-  __shared__ float col_sum[4][kTile];
-  __shared__ uint8_t row_bytes[kTile], col_bytes[kTile];
+  static constexpr int pitch = 33;
+  uint32_t turned[kTile * pitch];
+  uint32_t col_most[4][16][8];
+  float col_sum[4][kTile];
+  uint8_t row_bytes[kTile], col_bytes[kTile];
+};
+
+template <typename T, bool TILES>
+__device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t tile, Shared& shared) {
+  using S = Square<T>;
+  constexpr int RM = S::kRowMost, CM = S::kColMost, kPitch = Shared::pitch;
+  auto& turned = shared.turned;
+  auto& col_most = shared.col_most;
+  auto& col_sum = shared.col_sum;
+  auto& row_bytes = shared.row_bytes;
+  auto& col_bytes = shared.col_bytes;
   const int tid = threadIdx.x, wave = tid >> 6;
-  const int64_t r0 = (int64_t)(blockIdx.x / q.tiles_c) * kTile;
-  const int64_t c0 = (int64_t)(blockIdx.x % q.tiles_c) * kTile;
+  const int64_t r0 = (int64_t)(tile / q.tiles_c) * kTile;
+  const int64_t c0 = (int64_t)(tile % q.tiles_c) * kTile;
   const int tr = tid / 16 * 8, tc = tid % 16 * 8;  // the thread's first row and column
   S v;
   const T* at = reinterpret_cast<const T*>(q.x) + (r0 + tr) * q.ld + c0 + tc;
@@ -324,6 +336,12 @@ __global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
   }
 }
 
+template <typename T, bool TILES>
+__global__ __launch_bounds__(256) void float8_quantize_kernel(QuantizeArgs q) {
+  __shared__ Shared shared;
+  quantize_tile<T, TILES>(q, blockIdx.x, shared);
+}
+
 // The same codes and scales by rows alone: 16 lanes take a row's block of 128, a workgroup 16
 // rows' blocks, so that a matrix of a hundred rows still fills the GPU, and nothing goes through
 // LDS. us in a chain of launches, here / on 128 x 128 tiles: float16 100 x 14336 4.2 / 6.2, 8192 x
@@ -355,18 +373,50 @@ __global__ __launch_bounds__(256) void float8_quantize_rows_kernel(QuantizeArgs 
 }
 
 // Codes to bfloat16 halves of their values, 16 a thread.
-__global__ __launch_bounds__(256) void float8_expand_kernel(const uint8_t* data, int64_t data_ld,
-                                                            const uint8_t* scale, int64_t scale_ld,
-                                                            int64_t rows, int64_t chunks,
-                                                            __bf16* out, int64_t out_ld) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = at / chunks, c = (at - row * chunks) * 16;
-  if (row >= rows) return;
-  const u32x4 w = *reinterpret_cast<const u32x4*>(data + row * data_ld + c);
-  const float s = half_power(scale[c / kTile * scale_ld + row]);
-  bf16x8* to = reinterpret_cast<bf16x8*>(out + row * out_ld + c);
+struct ExpandArgs {
+  const uint8_t* data;
+  int64_t data_ld;
+  const uint8_t* scale;
+  int64_t scale_ld, rows, chunks;  // chunks: 16 codes each, of a row
+  __bf16* out;
+  int64_t out_ld;
+};
+__device__ __forceinline__ void expand_codes(const ExpandArgs& g, uint32_t block) {
+  const int64_t at = (int64_t)block * 256 + threadIdx.x;
+  const int64_t row = at / g.chunks, c = (at - row * g.chunks) * 16;
+  if (row >= g.rows) return;
+  const u32x4 w = *reinterpret_cast<const u32x4*>(g.data + row * g.data_ld + c);
+  const float s = half_power(g.scale[c / kTile * g.scale_ld + row]);
+  bf16x8* to = reinterpret_cast<bf16x8*>(g.out + row * g.out_ld + c);
   to[0] = expand(w[0], w[1], s);
   to[1] = expand(w[2], w[3], s);
+}
+__global__ __launch_bounds__(256) void float8_expand_kernel(ExpandArgs g) {
+  expand_codes(g, blockIdx.x);
+}
+
+// What a linear layer's pass quantizes and expands, in one launch: a small layer's parts hide each
+// other's latency.
+template <typename TX, typename TW>
+__global__ __launch_bounds__(256) void float8_quantize_pair_kernel(QuantizeArgs x, QuantizeArgs w,
+                                                                   uint32_t x_tiles) {
+  __shared__ Shared shared;
+  if (blockIdx.x < x_tiles)
+    quantize_tile<TX, false>(x, blockIdx.x, shared);
+  else
+    quantize_tile<TW, true>(w, blockIdx.x - x_tiles, shared);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void float8_quantize_expand_kernel(QuantizeArgs x, ExpandArgs a,
+                                                                     ExpandArgs b, uint32_t x_tiles,
+                                                                     uint32_t a_end) {
+  __shared__ Shared shared;
+  if (blockIdx.x < x_tiles)
+    quantize_tile<T, false>(x, blockIdx.x, shared);
+  else if (blockIdx.x < a_end)
+    expand_codes(a, blockIdx.x - x_tiles);
+  else
+    expand_codes(b, blockIdx.x - a_end);
 }
 
 // out[c] = the parts' sums: 4 threads a column, a quarter of the parts each in order, then
@@ -390,11 +440,9 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* parts, int6
 
 template <typename T>
 int launch_quantize(const QuantizeArgs& q, bool tiles, unsigned grid, hipStream_t stream) {
-  if (!tiles && !q.by_col.data && !q.sums) {
-    const int64_t groups = ceil_div(q.rows, 16);
-    DIONW_REQUIRE(groups < INT32_MAX / q.tiles_c, "float8_quantize: too many tiles");
-    hipLaunchKernelGGL(float8_quantize_rows_kernel<T>, dim3((unsigned)(groups * q.tiles_c)), dim3(256),
-                       0, stream, q);
+  if (!tiles && !q.by_col.data && !q.sums && ceil_div(q.rows, 16) * q.tiles_c <= kMostGroups) {
+    hipLaunchKernelGGL(float8_quantize_rows_kernel<T>, dim3((unsigned)(ceil_div(q.rows, 16) * q.tiles_c)),
+                       dim3(256), 0, stream, q);
     return check_launch("float8_quantize_rows");
   }
   if (tiles)
@@ -404,7 +452,110 @@ int launch_quantize(const QuantizeArgs& q, bool tiles, unsigned grid, hipStream_
   return check_launch("float8_quantize");
 }
 
+bool good_elem(int32_t e) { return e == kF16 || e == kBF16 || e == kF32; }
+
+// Checks a quantization; `tiles`: its workgroups, 0 where there is nothing to do.
+int prepare(const Quantization& j, QuantizeArgs& q, int64_t& tiles) {
+  tiles = 0;
+  DIONW_REQUIRE(good_elem(j.elem), "float8_quantize: bad element type %d", j.elem);
+  DIONW_REQUIRE(j.rows >= 0 && j.cols >= 0, "float8_quantize: negative extent");
+  if (j.rows == 0 || j.cols == 0) return kOk;
+  DIONW_REQUIRE(j.by_row.data || j.by_col.data || j.sums, "float8_quantize: no output");
+  DIONW_REQUIRE(j.x && j.ld >= j.cols, "float8_quantize: bad input");
+  auto fits = [](const Matrix& o, bool expanded, int64_t r, int64_t c) {
+    return !o.data || (o.depth >= round_up(c, kTile) && o.depth % 16 == 0 && aligned16(o.data) &&
+                       (expanded || o.scale_ld >= r));
+  };
+  const bool row_expanded = !j.by_row.scale, col_expanded = !j.by_col.scale;
+  DIONW_REQUIRE(fits(j.by_row, row_expanded, j.rows, j.cols) && fits(j.by_col, col_expanded, j.cols, j.rows),
+                "float8_quantize: an output is too small or not aligned");
+  const int64_t tr = ceil_div(j.rows, kTile), tc = ceil_div(j.cols, kTile);
+  DIONW_REQUIRE(tr <= kMostGroups / tc, "float8_quantize: too many tiles");
+  auto output = [](const Matrix& o, bool expanded) {
+    return Output{static_cast<uint8_t*>(o.data), expanded ? 2 * o.depth : o.depth,
+                  static_cast<uint8_t*>(o.scale), o.scale_ld, expanded};
+  };
+  q = {};
+  q.x = j.x;
+  q.rows = j.rows;
+  q.cols = j.cols;
+  q.ld = j.ld;
+  q.by_row = output(j.by_row, row_expanded);
+  q.by_col = output(j.by_col, col_expanded);
+  q.sums = j.sums;
+  q.tiles_c = (int32_t)tc;
+  tiles = tr * tc;
+  return kOk;
+}
+
+int prepare(const void* data, int64_t data_ld, const void* scale, int64_t scale_ld, int64_t rows,
+            int64_t depth, void* out, int64_t out_ld, ExpandArgs& g, int64_t& blocks) {
+  blocks = 0;
+  DIONW_REQUIRE(rows >= 0 && depth >= 0 && depth % kTile == 0, "float8_expand: bad extents");
+  if (rows == 0 || depth == 0) return kOk;
+  DIONW_REQUIRE(data && scale && out && aligned16(data) && aligned16(out) && data_ld >= depth &&
+                    data_ld % 16 == 0 && out_ld >= depth && out_ld % 8 == 0 && scale_ld >= rows,
+                "float8_expand: a matrix is too small or not aligned");
+  g = {static_cast<const uint8_t*>(data), data_ld, static_cast<const uint8_t*>(scale), scale_ld, rows,
+       depth / 16, static_cast<__bf16*>(out), out_ld};
+  DIONW_REQUIRE(rows <= kMostGroups * 256 / g.chunks, "float8_expand: too many elements");
+  blocks = ceil_div(rows * g.chunks, 256);
+  return kOk;
+}
+
+template <typename TX>
+int launch_pair(const QuantizeArgs& x, int64_t x_tiles, int32_t w_elem, const QuantizeArgs& w,
+                int64_t w_tiles, hipStream_t stream) {
+  const dim3 grid((unsigned)(x_tiles + w_tiles));
+  if (w_elem == kF16)
+    hipLaunchKernelGGL((float8_quantize_pair_kernel<TX, _Float16>), grid, dim3(256), 0, stream, x, w,
+                       (uint32_t)x_tiles);
+  else if (w_elem == kBF16)
+    hipLaunchKernelGGL((float8_quantize_pair_kernel<TX, __bf16>), grid, dim3(256), 0, stream, x, w,
+                       (uint32_t)x_tiles);
+  else
+    hipLaunchKernelGGL((float8_quantize_pair_kernel<TX, float>), grid, dim3(256), 0, stream, x, w,
+                       (uint32_t)x_tiles);
+  return check_launch("float8_quantize_pair");
+}
+
 }  // namespace
+
+int quantize_pair(const Quantization& x, const Quantization& w, hipStream_t stream) {
+  QuantizeArgs qx{}, qw{};
+  int64_t x_tiles, w_tiles;
+  DIONW_TRY(prepare(x, qx, x_tiles));
+  DIONW_TRY(prepare(w, qw, w_tiles));
+  if (x_tiles + w_tiles == 0) return kOk;
+  DIONW_REQUIRE(x_tiles + w_tiles <= kMostGroups, "float8_quantize: too many tiles");
+  if (x.elem == kF16) return launch_pair<_Float16>(qx, x_tiles, w.elem, qw, w_tiles, stream);
+  if (x.elem == kBF16) return launch_pair<__bf16>(qx, x_tiles, w.elem, qw, w_tiles, stream);
+  return launch_pair<float>(qx, x_tiles, w.elem, qw, w_tiles, stream);
+}
+
+int quantize_and_expand(const Quantization& x, const Matrix (&from)[2], const Matrix (&to)[2],
+                        hipStream_t stream) {
+  QuantizeArgs q{};
+  ExpandArgs g[2] = {};
+  int64_t tiles = 0, blocks[2] = {0, 0};
+  if (x.by_row.data || x.by_col.data || x.sums) DIONW_TRY(prepare(x, q, tiles));
+  for (int i = 0; i < 2; ++i)
+    if (to[i].data)
+      DIONW_TRY(prepare(from[i].data, from[i].depth, from[i].scale, from[i].scale_ld, from[i].rows,
+                        from[i].depth, to[i].data, to[i].depth, g[i], blocks[i]));
+  const int64_t total = tiles + blocks[0] + blocks[1];
+  if (total == 0) return kOk;
+  DIONW_REQUIRE(total <= kMostGroups, "float8_quantize: too many tiles");
+  auto launch = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)total), dim3(256), 0, stream, q, g[0], g[1], (uint32_t)tiles,
+                       (uint32_t)(tiles + blocks[0]));
+  };
+  if (x.elem == kF16) launch(float8_quantize_expand_kernel<_Float16>);
+  else if (x.elem == kBF16) launch(float8_quantize_expand_kernel<__bf16>);
+  else launch(float8_quantize_expand_kernel<float>);
+  return check_launch("float8_quantize_expand");
+}
+
 }  // namespace dionw
 
 using namespace dionw;
@@ -415,32 +566,17 @@ int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t col
                           int32_t tiles, void* data, int64_t data_ld, void* scale,
                           int64_t scale_ld, void* data_t, int64_t data_t_ld, void* scale_t,
                           int64_t scale_t_ld, int32_t expanded, float* sums, hipStream_t stream) {
-  DIONW_REQUIRE(elem == kF16 || elem == kBF16 || elem == kF32, "float8_quantize: bad element type %d", elem);
-  DIONW_REQUIRE(rows >= 0 && cols >= 0, "float8_quantize: negative extent");
-  if (rows == 0 || cols == 0) return kOk;
-  DIONW_REQUIRE(data || data_t || sums, "float8_quantize: no output");
-  DIONW_REQUIRE(x && ld >= cols, "float8_quantize: bad input");
   const bool row_expanded = expanded & 1, col_expanded = expanded & 2;
-  auto fits = [](const void* d, int64_t d_ld, const void* s, int64_t s_ld, int64_t r, int64_t c, bool e) {
-    return !d || (d_ld >= round_up(c, kTile) && d_ld % 16 == 0 && aligned16(d) && (e || (s && s_ld >= r)));
-  };
-  DIONW_REQUIRE(fits(data, data_ld, scale, scale_ld, rows, cols, row_expanded) &&
-                    fits(data_t, data_t_ld, scale_t, scale_t_ld, cols, rows, col_expanded),
-                "float8_quantize: an output is too small or not aligned");
-  const int64_t tr = ceil_div(rows, kTile), tc = ceil_div(cols, kTile);
-  DIONW_REQUIRE(tr < INT32_MAX / tc, "float8_quantize: too many tiles");
+  DIONW_REQUIRE((!data || row_expanded || scale) && (!data_t || col_expanded || scale_t),
+                "float8_quantize: codes need their scales");
+  const Quantization job{elem, x, rows, cols, ld,
+                         {data, row_expanded ? nullptr : scale, rows, data_ld, scale_ld},
+                         {data_t, col_expanded ? nullptr : scale_t, cols, data_t_ld, scale_t_ld}, sums};
   QuantizeArgs q{};
-  q.x = x;
-  q.rows = rows;
-  q.cols = cols;
-  q.ld = ld;
-  q.by_row = {static_cast<uint8_t*>(data), row_expanded ? 2 * data_ld : data_ld,
-              static_cast<uint8_t*>(scale), scale_ld, row_expanded};
-  q.by_col = {static_cast<uint8_t*>(data_t), col_expanded ? 2 * data_t_ld : data_t_ld,
-              static_cast<uint8_t*>(scale_t), scale_t_ld, col_expanded};
-  q.sums = sums;
-  q.tiles_c = (int32_t)tc;
-  const unsigned grid = (unsigned)(tr * tc);
+  int64_t count;
+  DIONW_TRY(prepare(job, q, count));
+  if (count == 0) return kOk;
+  const unsigned grid = (unsigned)count;
   if (elem == kF16) return launch_quantize<_Float16>(q, tiles != 0, grid, stream);
   if (elem == kBF16) return launch_quantize<__bf16>(q, tiles != 0, grid, stream);
   return launch_quantize<float>(q, tiles != 0, grid, stream);
@@ -449,17 +585,11 @@ int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t col
 int dionw_float8_expand(const void* data, int64_t data_ld, const void* scale, int64_t scale_ld,
                         int64_t rows, int64_t depth, void* out, int64_t out_ld,
                         hipStream_t stream) {
-  DIONW_REQUIRE(rows >= 0 && depth >= 0 && depth % kTile == 0, "float8_expand: bad extents");
-  if (rows == 0 || depth == 0) return kOk;
-  DIONW_REQUIRE(data && scale && out && aligned16(data) && aligned16(out) && data_ld >= depth &&
-                    data_ld % 16 == 0 && out_ld >= depth && out_ld % 8 == 0 && scale_ld >= rows,
-                "float8_expand: a matrix is too small or not aligned");
-  const int64_t chunks = depth / 16;
-  DIONW_REQUIRE(rows <= (int64_t)INT32_MAX * 256 / chunks, "float8_expand: too many elements");
-  hipLaunchKernelGGL(float8_expand_kernel, dim3((unsigned)ceil_div(rows * chunks, 256)), dim3(256), 0,
-                     stream, static_cast<const uint8_t*>(data), data_ld,
-                     static_cast<const uint8_t*>(scale), scale_ld, rows, chunks,
-                     static_cast<__bf16*>(out), out_ld);
+  ExpandArgs g{};
+  int64_t blocks;
+  DIONW_TRY(prepare(data, data_ld, scale, scale_ld, rows, depth, out, out_ld, g, blocks));
+  if (blocks == 0) return kOk;
+  hipLaunchKernelGGL(float8_expand_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, g);
   return check_launch("float8_expand");
 }
 

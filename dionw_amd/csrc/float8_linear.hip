@@ -245,12 +245,6 @@ struct Parts {
   }
 };
 
-struct Matrix {  // codes with their scales, or expanded codes
-  void* data;
-  void* scale;
-  int64_t rows, depth, scale_ld;
-};
-
 Matrix codes_in(Parts& p, int64_t rows, int64_t cols) {
   Matrix q{nullptr, nullptr, rows, round_up(cols, kTile), round_up(rows, 16)};
   q.data = p.take((size_t)(rows * q.depth));
@@ -309,21 +303,6 @@ struct Backward {
   }
 };
 
-// x by rows and its transpose by columns, into those of the two that have room.
-int quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld, bool tiles,
-             const Matrix& by_row, const Matrix& by_col, float* sums, hipStream_t stream) {
-  if (!by_row.data && !by_col.data && !sums) return kOk;
-  const int32_t expanded = (by_row.data && !by_row.scale ? 1 : 0) | (by_col.data && !by_col.scale ? 2 : 0);
-  return dionw_float8_quantize(elem, x, rows, cols, ld, tiles, by_row.data, by_row.depth, by_row.scale,
-                               by_row.scale_ld, by_col.data, by_col.depth, by_col.scale,
-                               by_col.scale_ld, expanded, sums, stream);
-}
-
-int expand_codes(const Matrix& from, const Matrix& to, hipStream_t stream) {
-  return dionw_float8_expand(from.data, from.depth, from.scale, from.scale_ld, from.rows, from.depth,
-                             to.data, to.depth, stream);
-}
-
 int product(bool expanded, const Matrix& a, const Matrix& b, const float* bias, int32_t elem, void* c,
             void* space, size_t bytes, hipStream_t stream) {
   return dionw_float8_gemm(expanded, a.rows, b.rows, a.depth, a.data, a.depth, a.scale, a.scale_ld,
@@ -373,8 +352,8 @@ int dionw_float8_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int
   Saved s(kept, m, n, k, need_x, need_w);
   Forward f(room, exact, m, n, k);
   DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float8_linear: scratch too small");
-  DIONW_TRY(quantize(x_elem, x, m, k, x_ld, false, f.x, s.xt, nullptr, stream));
-  DIONW_TRY(quantize(w_elem, w, n, k, w_ld, true, f.w, s.wt, nullptr, stream));
+  DIONW_TRY(quantize_pair({x_elem, x, m, k, x_ld, f.x, s.xt, nullptr},
+                          {w_elem, w, n, k, w_ld, f.w, s.wt, nullptr}, stream));
   return product(exact, f.x, f.w, bias, x_elem, y, f.product, f.product_bytes, stream);
 }
 
@@ -392,14 +371,13 @@ int dionw_float8_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
   Backward b(room, exact_x, exact_w, m, n, k, need_x, need_w, db != nullptr);
   DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float8_linear: scratch too small");
   DIONW_REQUIRE(saved || kept.used == 0, "float8_linear: nothing was saved");
-  DIONW_TRY(quantize(x_elem, dy, m, n, dy_ld, false, b.rows, b.cols, b.sums, stream));
+  DIONW_TRY(quantize_and_expand({x_elem, dy, m, n, dy_ld, b.rows, b.cols, b.sums}, {s.wt, s.xt},
+                                {b.wt, b.xt}, stream));
   if (need_x) {
-    if (exact_x) DIONW_TRY(expand_codes(s.wt, b.wt, stream));
     DIONW_TRY(product(exact_x, b.rows, exact_x ? b.wt : s.wt, nullptr, x_elem, dx, b.product,
                       b.product_bytes, stream));
   }
   if (need_w) {
-    if (exact_w) DIONW_TRY(expand_codes(s.xt, b.xt, stream));
     DIONW_TRY(product(exact_w, b.cols, exact_w ? b.xt : s.xt, nullptr, w_elem, dw, b.product,
                       b.product_bytes, stream));
   }
@@ -445,15 +423,15 @@ int dionw_float8_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const 
   if (exact) {
     Forward f(room, true, m, n, k);
     DIONW_REQUIRE(room.used <= scratch_bytes, "float8_linear: scratch too small");
-    DIONW_TRY(quantize(x_elem, x, m, k, x_ld, false, f.x, Matrix{}, nullptr, stream));
-    DIONW_TRY(expand_codes(weight, f.w, stream));
+    DIONW_TRY(quantize_and_expand({x_elem, x, m, k, x_ld, f.x, {}, nullptr}, {weight, {}}, {f.w, {}}, stream));
     return product(true, f.x, f.w, bias, x_elem, y, f.product, f.product_bytes, stream);
   }
   const Matrix rows = codes_in(room, m, k);
   const size_t bytes = dionw_float8_gemm_workspace(0, m, n, depth);
   void* space = room.take(bytes);
   DIONW_REQUIRE(room.used <= scratch_bytes, "float8_linear: scratch too small");
-  DIONW_TRY(quantize(x_elem, x, m, k, x_ld, false, rows, Matrix{}, nullptr, stream));
+  DIONW_TRY(dionw_float8_quantize(x_elem, x, m, k, x_ld, 0, rows.data, rows.depth, rows.scale, rows.scale_ld,
+                                  nullptr, 0, nullptr, 0, 0, nullptr, stream));
   return product(false, rows, weight, bias, x_elem, y, space, bytes, stream);
 }
 
