@@ -637,31 +637,46 @@ float8_gemm_kernel(ProductArgs g, int total) {
     quad_tile<CFG, CODES, OUT>(g, w);
 }
 
-// C = alpha (the ranges' sums in order) + bias.
+// C = alpha (the ranges' sums in order) + bias, 4 elements a thread, the loads of 4 ranges at once.
 template <typename OUT>
 __global__ __launch_bounds__(256) void join_splits_kernel(ProductArgs g, const float* parts, int splits) {
   const int64_t total = (int64_t)g.m * g.n, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= total) return;
   typedef float f4any __attribute__((ext_vector_type(4), aligned(4)));
-  float v[4];
-  if (at + 4 <= total) {
-    f4any s = *reinterpret_cast<const f4any*>(parts + at);
-    for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f4any*>(parts + k * total + at);
+  const bool whole = at + 4 <= total;
+  const uint32_t left = whole ? 4 : (uint32_t)(total - at);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < splits; k0 += 4) {
+    f32x4 v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = s[e];
-  } else {
+    for (int k = 0; k < 4; ++k) {
+      const float* from = parts + min(k0 + k, splits - 1) * total + at;
+      if (whole) {
+        v[k] = *reinterpret_cast<const f4any*>(from);
+      } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = 0.f;
-      for (int k = 0; k < splits && at + e < total; ++k) v[e] += parts[k * total + at + e];
+        for (uint32_t e = 0; e < 4; ++e) v[k][e] = e < left ? from[e] : 0.f;
+      }
     }
-  }
-  int64_t row = at / g.n;
-  int col = (int)(at - row * g.n);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (at + e < total)
-      reinterpret_cast<OUT*>(g.c)[row * g.ldc + col] = (OUT)(g.alpha * v[e] + (g.bias ? g.bias[col] : 0.f));
+    for (int k = 0; k < 4; ++k)
+      if (k0 + k < splits) s = k0 + k ? s + v[k] : v[k];
+  }
+  int64_t row = total <= UINT32_MAX ? (uint32_t)at / (uint32_t)g.n : at / g.n;
+  int col = (int)(at - row * g.n);
+  OUT* c = reinterpret_cast<OUT*>(g.c);
+  if (whole && col + 4 <= g.n) {
+    typedef OUT o4 __attribute__((ext_vector_type(4)));
+    typedef OUT o4any __attribute__((ext_vector_type(4), aligned(sizeof(OUT))));
+    o4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (OUT)(g.alpha * s[e] + (g.bias ? g.bias[col + e] : 0.f));
+    *reinterpret_cast<o4any*>(c + row * g.ldc + col) = o;
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) {
+    if (e < left) c[row * g.ldc + col] = (OUT)(g.alpha * s[e] + (g.bias ? g.bias[col] : 0.f));
     if (++col == g.n) {
       col = 0;
       ++row;
