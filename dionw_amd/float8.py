@@ -34,6 +34,7 @@ __all__ = ["Float8Linear", "Float8Matrix", "float8_linear", "float8_matmul", "fl
 
 TILE: Final = 128  # columns (and rows) that share a scale
 _DTYPES: Final = (torch.float16, torch.bfloat16, torch.float32)
+_CODES: Final = {dtype: _lib.elem_code(dtype) for dtype in _DTYPES}
 
 
 @dataclass(frozen=True, eq=False)
@@ -267,28 +268,34 @@ def _kept_scratch(code: int, m: int, n: int, k: int) -> int:
 
 
 def _kept_linear(x: Tensor, weight: Float8Matrix, bias: Tensor | None) -> Tensor:
+    # Decoding waits for the host here: every attribute is read once.
     data, scale, k, dtype = weight.data, weight.scale, weight.cols, x.dtype
-    device, shape = data.device, x.shape
+    device, shape, code = data.device, x.shape, _CODES.get(dtype)
     n, depth = data.shape
-    if not shape or shape[-1] != k or x.device != device or dtype not in _DTYPES:
+    if not shape or shape[-1] != k or x.device != device or code is None:
         raise ValueError(f"float8_linear takes float x [..., {k}] on {device} for this weight, got "
                          f"{dtype} {tuple(shape)} on {x.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("a Float8Matrix weight is for inference: pass the float weight where "
                          "gradients are needed, or call under torch.no_grad()")
     stream = _lib.stream_handle(device)
-    if len(shape) != 2:
-        x = x.reshape(math.prod(shape[:-1]), k)
+    if len(shape) == 2:
+        m, out = shape[0], (shape[0], n)
+    else:
+        m, out = math.prod(shape[:-1]), (*shape[:-1], n)
+        x = x.reshape(m, k)
+    pitch = k
     if not x.is_contiguous():
         x = _readable(x)
-    m, code = x.shape[0], _lib.elem_code(dtype)
-    bias = _bias(bias, n, device)
+        pitch = _pitch(x)
+    if bias is not None:
+        bias = _bias(bias, n, device)
     room = _kept_scratch(code, m, n, k)
-    scratch = _scratch(room, device)
-    y = torch.empty((*shape[:-1], n), dtype=dtype, device=device)
-    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), _pitch(x), data.data_ptr(), depth,
-              scale.data_ptr(), scale.shape[1], _lib.ptr(bias), m, n, k, y.data_ptr(),
-              _lib.ptr(scratch), room, stream)
+    scratch = _scratch(room, device) if room else None
+    y = x.new_empty(out)
+    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), pitch, data.data_ptr(), depth,
+              scale.data_ptr(), scale.shape[1], None if bias is None else bias.data_ptr(), m, n, k,
+              y.data_ptr(), _lib.ptr(scratch), room, stream)
     return y
 
 
