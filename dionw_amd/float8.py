@@ -199,14 +199,17 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
                     (b.data.data_ptr(), b.scale.data_ptr(), b.scale.shape[1]), bias, dtype, a.device)
 
 
-def _bias(bias: Tensor | None, n: int, device: torch.device) -> Tensor | None:
-    """The bias as the product reads it: contiguous float32."""
-    if bias is None:
-        return None
-    if bias.shape != (n,) or bias.dtype not in _DTYPES or bias.device != device:
+def _check_bias(bias: Tensor | None, n: int, device: torch.device) -> None:
+    if bias is not None and (bias.shape != (n,) or bias.dtype not in _DTYPES or bias.device != device):
         raise ValueError(f"the bias of {n} outputs is a float vector of that length on {device}, got "
                          f"{bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    return bias.detach().to(torch.float32).contiguous()
+
+
+def _bias(bias: Tensor | None, n: int, device: torch.device) -> Tensor | None:
+    """The bias as the product reads it: contiguous float32, which the caller holds until the
+    library call has returned (a temporary freed before it may be another thread's by then)."""
+    _check_bias(bias, n, device)
+    return None if bias is None else bias.detach().to(torch.float32).contiguous()
 
 
 @lru_cache(maxsize=256)
@@ -236,9 +239,10 @@ class _Linear(torch.autograd.Function):
         keep, room, ctx.room = _sizes(*codes, m, n, k, need_x, need_w, need_b)
         saved, scratch = _scratch(keep, device), _scratch(room, device)
         y = torch.empty(m, n, dtype=dtype, device=device)
+        added = _bias(bias, n, device)
         _lib.call("dionw_float8_linear_forward", codes[0], x.data_ptr(), _pitch(x), codes[1],
-                  weight.data_ptr(), _pitch(weight), _lib.ptr(_bias(bias, n, device)), m, n, k,
-                  need_x, need_w, y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
+                  weight.data_ptr(), _pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
+                  y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
         ctx.codes, ctx.sizes, ctx.dtypes = codes, (m, n, k), (dtype, weight.dtype)
         ctx.bias_dtype = bias.dtype if need_b else None
         ctx.save_for_backward(*([] if saved is None else [saved]))
@@ -320,7 +324,7 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
                          f"{tuple(shape)} and {tuple(weight.shape)}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    _bias(bias, weight.shape[0], x.device)
+    _check_bias(bias, weight.shape[0], x.device)
     if len(shape) == 2:
         return _Linear.apply(x, weight, bias)
     flat = x.reshape(math.prod(shape[:-1]), shape[-1])
