@@ -25,6 +25,7 @@ from typing import Any, Final
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from dionw_amd import _lib
@@ -35,6 +36,30 @@ __all__ = ["Float8Linear", "Float8Matrix", "float8_linear", "float8_matmul", "fl
 TILE: Final = 128  # columns (and rows) that share a scale
 _DTYPES: Final = (torch.float16, torch.bfloat16, torch.float32)
 _CODES: Final = {dtype: _lib.elem_code(dtype) for dtype in _DTYPES}
+
+
+# Cheap signs of what _check_unrecorded looks for: torch.jit.trace, and function modes, which
+# make_fx runs under (as harmless ones do).
+_tracing = torch._C._is_tracing
+_function_modes = torch._C._len_torch_function_stack
+
+
+def _check_unrecorded(*tensors: Tensor | None) -> None:
+    """Kernels run on addresses, which graph recorders and forward-mode derivatives do not see: a
+    recorded graph would return the outputs' memory as it was allocated, a tangent would be lost."""
+    if torch.jit.is_tracing() or (_function_modes() and _recorded_by_fx()):
+        raise ValueError("the 8-bit kernels cannot be recorded by torch.jit.trace or make_fx: the "
+                         "graph would lose them")
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("the 8-bit operators have no forward-mode derivative: call them on plain "
+                         "tensors, or use the backward pass")
+
+
+def _recorded_by_fx() -> bool:
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode  # takes a second to import
+
+    return get_proxy_mode() is not None
 
 
 @dataclass(frozen=True, eq=False)
@@ -137,6 +162,8 @@ def _pitch(x: Tensor) -> int:
 
 def _quantize(x: Tensor, tiles: bool, both: bool) -> tuple[Float8Matrix, Float8Matrix | None]:
     """x quantized by rows, and its transpose quantized by rows where both are asked for."""
+    if _tracing() or _function_modes():
+        _check_unrecorded()
     x = _readable(x)
     m, n = x.shape
     stream = _lib.stream_handle(x.device)
@@ -156,7 +183,8 @@ def float8_quantize(x: Tensor, *, tiles: bool = False) -> Float8Matrix:
     row and 128 columns, or (``tiles``) for each 128 x 128 tile.
 
     Raises:
-        ValueError: For another shape or type, or a tensor off the GPU.
+        ValueError: For another shape or type, a tensor off the GPU, or a call that
+            ``torch.jit.trace`` or ``make_fx`` records.
     """
     return _quantize(x.detach(), tiles, False)[0]
 
@@ -166,7 +194,8 @@ def float8_quantize_both(x: Tensor, *, tiles: bool = False) -> tuple[Float8Matri
     gradients take. With ``tiles`` both hold the same values.
 
     Raises:
-        ValueError: For another shape or type, or a tensor off the GPU.
+        ValueError: For another shape or type, a tensor off the GPU, or a call that
+            ``torch.jit.trace`` or ``make_fx`` records.
     """
     by_row, by_column = _quantize(x.detach(), tiles, True)
     return by_row, by_column
@@ -182,8 +211,11 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
 
     Raises:
         ValueError: For operands or a bias that do not fit each other, another dtype than
-            float16, bfloat16 or float32, or tensors off the GPU.
+            float16, bfloat16 or float32, tensors off the GPU, a forward-mode dual, or a call
+            that ``torch.jit.trace`` or ``make_fx`` records.
     """
+    if _tracing() or _function_modes() or forward_ad._current_level >= 0:
+        _check_unrecorded(bias)
     m, n = a.shape[0], b.shape[0]
     if a.cols != b.cols or a.device != b.device:
         raise ValueError(f"float8_matmul takes matrices of one depth on one device, got {a.shape} on "
@@ -312,11 +344,15 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     ``Float8Matrix`` for inference.
 
     Raises:
-        ValueError: For shapes or types that do not fit, tensors off the GPU, an x that
-            requires a gradient beside a ``Float8Matrix``, or sums of 8 M products (4 M for a
+        ValueError: For shapes or types that do not fit, tensors off the GPU, an x or bias that
+            requires a gradient beside a ``Float8Matrix``, forward-mode duals, calls that
+            ``torch.jit.trace`` or ``make_fx`` records, or sums of 8 M products (4 M for a
             float32 result) and more, a gradient's included.
     """
-    if isinstance(weight, Float8Matrix):
+    kept = isinstance(weight, Float8Matrix)
+    if _tracing() or _function_modes() or forward_ad._current_level >= 0:
+        _check_unrecorded(x, None if kept else weight, bias)
+    if kept:
         return _kept_linear(x, weight, bias)
     shape = x.shape
     if not shape or weight.dim() != 2 or shape[-1] != weight.shape[1]:

@@ -12,9 +12,18 @@ from typing import Any
 
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from dionw_amd import Float8Matrix, _lib, float8_linear
+from dionw_amd import (
+    Float8Matrix,
+    _lib,
+    float8_linear,
+    float8_matmul,
+    float8_quantize,
+    float8_quantize_both,
+)
 
 FORWARD = "dionw_float8_linear_forward"
 BIAS = 6  # the bias's place among the forward's arguments
@@ -72,3 +81,75 @@ def test_a_16_bit_bias_is_converted_once_and_held_during_the_call(weight, dtype,
         float8_linear(x, w, bias)
     assert held == [True]
     assert copies.count == 1
+
+
+def _float_weight(rows: int, cols: int) -> torch.Tensor:
+    return torch.ones(rows, cols)
+
+
+# Each of the operators as a function of a float x, for a weight [5, 200] made outside of it.
+OPERATORS = [
+    pytest.param(lambda x, w: float8_linear(x, w), _kept, id="kept"),
+    pytest.param(lambda x, w: float8_linear(x, w), _float_weight, id="linear"),
+    pytest.param(lambda x, w: float8_matmul(w, w, x[0, :5]), _kept, id="matmul"),
+]
+QUANTIZERS = [
+    pytest.param(lambda x, w: float8_quantize(x).data, _kept, id="quantize"),
+    pytest.param(lambda x, w: float8_quantize_both(x)[1].data, _kept, id="quantize both"),
+]
+
+
+@pytest.mark.parametrize(("operator", "weight"), OPERATORS)
+def test_forward_mode_duals_are_refused(operator, weight, calls) -> None:
+    """Their tangents would be dropped: a derivative of zero."""
+    w, x = weight(5, 200), torch.ones(3, 200)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad(), pytest.raises(ValueError, match="forward-mode"):
+                operator(dual, w)
+        assert not calls
+        operator(x, w)  # a plain tensor inside a level is served
+    assert calls
+
+
+def test_a_dual_bias_or_weight_is_refused(calls) -> None:
+    x, w, bias = torch.ones(3, 200), torch.ones(5, 200), torch.ones(5)
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (w, bias)]
+        for call in (lambda: float8_linear(x, dual[0]), lambda: float8_linear(x, w, dual[1]),
+                     lambda: float8_linear(x, _kept(5, 200), dual[1])):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+    assert not calls
+
+
+@pytest.mark.parametrize(("operator", "weight"), OPERATORS + QUANTIZERS)
+@pytest.mark.parametrize("recorder", ["make_fx", "make_fx before dispatch", "jit.trace"])
+def test_recorders_are_refused(recorder, operator, weight, calls) -> None:
+    """A recorded graph would hold the outputs' allocation and no kernel."""
+    w, x = weight(5, 200), torch.ones(3, 200)
+    with pytest.raises(ValueError, match="record"):
+        if recorder == "jit.trace":
+            torch.jit.trace(lambda x: operator(x, w), (x,), check_trace=False)
+        else:
+            make_fx(lambda x: operator(x, w), pre_dispatch="before" in recorder)(x)
+    assert not calls
+
+
+@pytest.mark.parametrize(("operator", "weight"), OPERATORS + QUANTIZERS)
+def test_modes_that_record_nothing_are_served(operator, weight, calls) -> None:
+    w, x = weight(5, 200), torch.ones(3, 200)
+    with torch.device("cpu"), _Copies(-1):
+        operator(x, w)
+    assert calls
+
+
+@pytest.mark.parametrize(("operator", "weight"), OPERATORS + QUANTIZERS)
+def test_compiled_functions_reach_the_library_every_time(operator, weight, calls) -> None:
+    w, x = weight(5, 200), torch.ones(3, 200)
+    compiled = torch.compile(lambda x: operator(x + 1, w), backend="eager")
+    compiled(x)
+    first = len(calls)
+    compiled(x)
+    assert first and len(calls) == 2 * first
