@@ -257,26 +257,33 @@ def _scratch(size: int, device: torch.device) -> Tensor | None:
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
+def _forward(x: Tensor, weight: Tensor, bias: Tensor | None, need_x: bool, need_w: bool,
+             need_b: bool) -> tuple[Tensor, Tensor | None, int]:
+    """y, what the gradients asked for need of x and W, and the bytes of the backward's scratch."""
+    x, weight = _readable(x), _readable(weight)
+    m, k = x.shape
+    n, device = weight.shape[0], x.device
+    x_code, w_code = _CODES[x.dtype], _CODES[weight.dtype]
+    stream = _lib.stream_handle(device)
+    keep, room, backward_room = _sizes(x_code, w_code, m, n, k, need_x, need_w, need_b)
+    saved, scratch = _scratch(keep, device), _scratch(room, device)
+    y = torch.empty(m, n, dtype=x.dtype, device=device)
+    added = _bias(bias, n, device)
+    _lib.call("dionw_float8_linear_forward", x_code, x.data_ptr(), _pitch(x), w_code,
+              weight.data_ptr(), _pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
+              y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
+    return y, saved, backward_room
+
+
 class _Linear(torch.autograd.Function):
     """y = x W^T + b; dx = dy W, dW = dy^T x, db = the sum of dy over the rows."""
 
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
-        need_x, need_w, need_b = ctx.needs_input_grad
-        x, weight = _readable(x), _readable(weight)
-        m, k = x.shape
-        n, device, dtype = weight.shape[0], x.device, x.dtype
-        codes = _lib.elem_code(dtype), _lib.elem_code(weight.dtype)
-        stream = _lib.stream_handle(device)
-        keep, room, ctx.room = _sizes(*codes, m, n, k, need_x, need_w, need_b)
-        saved, scratch = _scratch(keep, device), _scratch(room, device)
-        y = torch.empty(m, n, dtype=dtype, device=device)
-        added = _bias(bias, n, device)
-        _lib.call("dionw_float8_linear_forward", codes[0], x.data_ptr(), _pitch(x), codes[1],
-                  weight.data_ptr(), _pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
-                  y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
-        ctx.codes, ctx.sizes, ctx.dtypes = codes, (m, n, k), (dtype, weight.dtype)
-        ctx.bias_dtype = bias.dtype if need_b else None
+        y, saved, ctx.room = _forward(x, weight, bias, *ctx.needs_input_grad)
+        ctx.codes = _CODES[x.dtype], _CODES[weight.dtype]
+        ctx.sizes, ctx.dtypes = (x.shape[0], *weight.shape), (x.dtype, weight.dtype)
+        ctx.bias_dtype = bias.dtype if ctx.needs_input_grad[2] else None
         ctx.save_for_backward(*([] if saved is None else [saved]))
         return y
 
@@ -361,10 +368,14 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
     _check_bias(bias, weight.shape[0], x.device)
-    if len(shape) == 2:
-        return _Linear.apply(x, weight, bias)
-    flat = x.reshape(math.prod(shape[:-1]), shape[-1])
-    return _Linear.apply(flat, weight, bias).view(*shape[:-1], weight.shape[0])
+    flat = x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), shape[-1])
+    # Asked here: inside the function gradients are off, and what it is told of its inputs' needs
+    # does not know whether they were on.
+    if torch.is_grad_enabled():
+        y = _Linear.apply(flat, weight, bias)
+    else:
+        y = _forward(flat, weight, bias, False, False, False)[0]
+    return y if len(shape) == 2 else y.view(*shape[:-1], weight.shape[0])
 
 
 class Float8Linear(nn.Linear):

@@ -12,11 +12,13 @@ from typing import Any
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from dionw_amd import (
+    Float8Linear,
     Float8Matrix,
     _lib,
     float8_linear,
@@ -153,3 +155,33 @@ def test_compiled_functions_reach_the_library_every_time(operator, weight, calls
     first = len(calls)
     compiled(x)
     assert first and len(calls) == 2 * first
+
+
+SAVED = slice(10, 14)  # need_x, need_w, y, saved among the forward's arguments
+
+
+@pytest.mark.parametrize("grad", [torch.no_grad, torch.inference_mode])
+def test_a_forward_without_gradients_prepares_none(grad, calls) -> None:
+    """Parameters require gradients also where none are recorded: nothing is transposed or kept
+    then, and nothing refused that only a gradient could not do."""
+    x, layer = torch.ones(30, 200, requires_grad=True), Float8Linear(200, 50)
+    with grad():
+        y = layer(x)
+    ((name, args),) = calls
+    need_x, need_w, _, saved = args[SAVED]
+    assert name == FORWARD and (need_x, need_w, saved) == (False, False, None)
+    assert y.shape == (30, 50) and not y.requires_grad
+    calls.clear()
+    layer(x)
+    ((_, args),) = calls
+    need_x, need_w, _, saved = args[SAVED]
+    assert need_x and need_w and saved
+
+
+def test_a_first_pass_of_a_checkpoint_prepares_no_gradients(calls) -> None:
+    x, layer = torch.ones(30, 200, requires_grad=True), Float8Linear(200, 50)
+    y = torch.utils.checkpoint.checkpoint(layer, x, use_reentrant=True)
+    assert y.requires_grad
+    y.sum().backward()
+    assert [name for name, _ in calls] == [FORWARD, FORWARD, "dionw_float8_linear_backward"]
+    assert [bool(args[10] or args[11]) for _, args in calls[:2]] == [False, True]
