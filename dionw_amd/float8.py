@@ -211,8 +211,8 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
 
     Raises:
         ValueError: For operands or a bias that do not fit each other, another dtype than
-            float16, bfloat16 or float32, tensors off the GPU, a forward-mode dual, or a call
-            that ``torch.jit.trace`` or ``make_fx`` records.
+            float16, bfloat16 or float32, tensors off the GPU, a bias that requires a gradient,
+            a forward-mode dual, or a call that ``torch.jit.trace`` or ``make_fx`` records.
     """
     if _tracing() or _function_modes() or forward_ad._current_level >= 0:
         _check_unrecorded(bias)
@@ -220,6 +220,9 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
     if a.cols != b.cols or a.device != b.device:
         raise ValueError(f"float8_matmul takes matrices of one depth on one device, got {a.shape} on "
                          f"{a.device} and {b.shape} on {b.device}")
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("float8_matmul gives its bias no gradient: pass it detached, or use "
+                         "float8_linear on the float weight")
     bias = _bias(bias, n, a.device)
     _lib.elem_code(dtype)
     depth = a.data.shape[1]

@@ -185,3 +185,14 @@ def test_a_first_pass_of_a_checkpoint_prepares_no_gradients(calls) -> None:
     y.sum().backward()
     assert [name for name, _ in calls] == [FORWARD, FORWARD, "dionw_float8_linear_backward"]
     assert [bool(args[10] or args[11]) for _, args in calls[:2]] == [False, True]
+
+
+def test_a_product_refuses_a_bias_whose_gradient_it_would_drop(calls) -> None:
+    a, bias = _kept(5, 200), torch.ones(5, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        float8_matmul(a, a, bias)
+    assert not calls
+    float8_matmul(a, a, bias.detach())
+    with torch.no_grad():
+        float8_matmul(a, a, bias)
+    assert [name for name, _ in calls] == ["dionw_float8_gemm"] * 2
