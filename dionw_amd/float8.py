@@ -349,9 +349,10 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     """``x @ weight.T + bias`` in 8 bits, in x's type (float16, bfloat16 or float32).
 
     ``x`` is ``[..., in]``; its rows, all leading dimensions taken together, form the blocks of
-    128 of the weight's gradient. ``weight`` is ``[out, in]``: a float tensor, quantized at
-    every call (gradients flow to x, weight and bias, the weight's in its own type), or a
-    ``Float8Matrix`` for inference.
+    128 of the weight's gradient. Under ``torch.autocast`` x is cast to its type first, as for
+    ``nn.Linear``; the weight and the bias stay as they are. ``weight`` is ``[out, in]``: a float
+    tensor, quantized at every call (gradients flow to x, weight and bias, the weight's in its
+    own type), or a ``Float8Matrix`` for inference.
 
     Raises:
         ValueError: For shapes or types that do not fit, tensors off the GPU, an x or bias that
@@ -362,6 +363,8 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     kept = isinstance(weight, Float8Matrix)
     if _tracing() or _function_modes() or forward_ad._current_level >= 0:
         _check_unrecorded(x, None if kept else weight, bias)
+    if torch.is_autocast_enabled() and x.dtype in _CODES:
+        x = x.to(torch.get_autocast_dtype("cuda"))
     if kept:
         return _kept_linear(x, weight, bias)
     shape = x.shape

@@ -7,7 +7,7 @@ GPU ones would.
 from __future__ import annotations
 
 import gc
-from collections.abc import Callable
+from collections.abc import Callable, Iterator
 from typing import Any
 
 import pytest
@@ -196,3 +196,35 @@ def test_a_product_refuses_a_bias_whose_gradient_it_would_drop(calls) -> None:
     with torch.no_grad():
         float8_matmul(a, a, bias)
     assert [name for name, _ in calls] == ["dionw_float8_gemm"] * 2
+
+
+@pytest.fixture
+def autocast() -> Iterator[None]:
+    """The GPU's autocast to bfloat16, as ``torch.autocast("cuda", torch.bfloat16)`` sets it."""
+    before = torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda")
+    torch.set_autocast_dtype("cuda", torch.bfloat16)
+    torch.set_autocast_enabled("cuda", True)
+    yield
+    torch.set_autocast_enabled("cuda", before[0])
+    torch.set_autocast_dtype("cuda", before[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_autocast_casts_the_input_as_for_a_linear_layer(dtype, autocast, calls) -> None:
+    x, layer = torch.ones(30, 200, dtype=dtype, requires_grad=True), Float8Linear(200, 50)
+    y = layer(x)
+    assert y.dtype is torch.bfloat16 and calls[0][1][0] == _lib.BF16 and calls[0][1][3] == _lib.F32
+    y.sum().backward()
+    assert x.grad.dtype is dtype and layer.weight.grad.dtype is layer.bias.grad.dtype is torch.float32
+    calls.clear()
+    with torch.no_grad():
+        assert float8_linear(x, _kept(50, 200), layer.bias).dtype is torch.bfloat16
+    assert calls[0][1][0] == _lib.BF16
+
+
+def test_autocast_leaves_other_types_refused(autocast, calls) -> None:
+    for dtype in (torch.float64, torch.int32):
+        for w in (torch.ones(5, 200), _kept(5, 200)):
+            with pytest.raises(ValueError):
+                float8_linear(torch.ones(3, 200, dtype=dtype), w)
+    assert not calls

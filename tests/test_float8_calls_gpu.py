@@ -35,3 +35,23 @@ def test_rows_that_only_a_gradient_could_not_sum_are_served() -> None:
     with torch.no_grad():
         y = float8_linear(x, w)
         assert torch.equal(y[-2:], float8_linear(x[-2:], w)) and not y[:-2].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast_is_heeded(dtype) -> None:
+    """A float32 activation under autocast goes the way of a 16-bit one, and gets a float32 gradient."""
+    layer, kept_layer = Float8Linear(260, 130).cuda(), torch.nn.Linear(260, 130).cuda()
+    x, half = _random(300, 260, 1).requires_grad_(), _random(300, 260, 1).to(dtype).requires_grad_()
+    dy = _random(300, 130, 2).to(dtype)
+    with torch.autocast("cuda", dtype):
+        y = layer(x)
+        assert y.dtype is kept_layer(x).dtype is dtype
+        with torch.no_grad():
+            served = float8_linear(x, layer.quantized_weight(), layer.bias)
+    want = layer(half)
+    assert torch.equal(y, want)
+    with torch.no_grad():
+        assert torch.equal(served, float8_linear(half, layer.quantized_weight(), layer.bias))
+    got = torch.autograd.grad(y, (x, layer.weight, layer.bias), dy)
+    for g, w in zip(got, torch.autograd.grad(want, (half, layer.weight, layer.bias), dy)):
+        assert g.dtype is torch.float32 and torch.equal(g, w.float())
