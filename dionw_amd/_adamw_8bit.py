@@ -17,7 +17,7 @@ and every replica of a tensor round alike.
 from __future__ import annotations
 
 import ctypes
-from collections.abc import Sequence
+from collections.abc import Mapping, Sequence
 from enum import Enum
 from operator import attrgetter
 from typing import Any, Final
@@ -105,23 +105,36 @@ class AdamWPack:
             ADAMW_STEP_STATE: self.steps[place],
         }
 
+    def check(self, state: Mapping[Tensor, Mapping[str, Any]]) -> None:
+        """Refuse a state that ``adopt`` could not take.
+
+        Raises:
+            ValueError: If an entry is not a tensor of the parameter's size.
+        """
+        for place, param in enumerate(self.params):
+            entry = state.get(param, {})
+            for key, view in self.views(place).items():
+                held = entry.get(key)
+                if held is not None and (not isinstance(held, Tensor) or held.shape != view.shape):
+                    found = tuple(held.shape) if isinstance(held, Tensor) else type(held).__name__
+                    raise ValueError(f"the 8-bit AdamW state {key!r} is {found}, the parameter "
+                                     f"needs a tensor of shape {tuple(view.shape)}")
+
     def adopt(self, state: ParamState) -> None:
         """Point the tensors' state entries at the pack, copying in the values they held
         (a loaded checkpoint; torch's loader hands codes over as float32, which holds them
-        exactly), zeros where there are none.
+        exactly), zeros where there are none. A refused state changes nothing.
 
         Raises:
             ValueError: If an entry holds a state of another size.
         """
+        self.check(state)
         for place, param in enumerate(self.params):
             entry = state[param]
             for key, view in self.views(place).items():
                 held = entry.get(key)
                 if held is None:
                     view.zero_()
-                elif held.shape != view.shape:
-                    raise ValueError(f"the 8-bit AdamW state {key!r} has shape "
-                                     f"{tuple(held.shape)}, the parameter needs {tuple(view.shape)}")
                 elif held.data_ptr() != view.data_ptr() or held.dtype != view.dtype:
                     view.copy_(held)
                 entry[key] = view

@@ -218,9 +218,17 @@ class Dion(IntegratedEMAOptimizer):
 
         Raises:
             ValueError: If the saved groups differ in number or in a structural
-                key (route, fraction, heads, update options).
+                key (route, fraction, heads, update options), or 8-bit AdamW state is
+                of another size than its parameter; nothing is loaded then.
         """
         groups = refuse_structural_change(state_dict["param_groups"], self.param_groups)
+        if self._adamw_packs:
+            saved = {param: state_dict["state"].get(index, {})
+                     for old, live in zip(groups, self.param_groups)
+                     for index, param in zip(old["params"], live["params"])}
+            for packs in self._adamw_packs.values():
+                for pack in packs:
+                    pack.check(saved)
         super().load_state_dict({**state_dict, "param_groups": groups})
         self._repack()
         for packs in self._adamw_packs.values():
