@@ -7,7 +7,9 @@ as uint8 codes of an unsigned float with 4 exponent bits (bias 8) and 4 fraction
 bits. The state of a group's tensors on one device lies in one allocation of
 each kind (``AdamWPack``), every tensor at a multiple of 256 elements in
 row-major order, and ``optimizer.state[p]`` holds views; so a step passes the
-tensors' places instead of six pointers for each.
+tensors' places instead of six pointers for each. What a caller puts in a view's
+place is copied into the pack before the next step reads it, and a view that was
+removed starts again from zeros.
 
 The codes are rounded stochastically with bits from a hash of the step, the
 tensor's position in its group and the element's index: a run, a resumed run
@@ -19,7 +21,8 @@ from __future__ import annotations
 import ctypes
 from collections.abc import Mapping, Sequence
 from enum import Enum
-from operator import attrgetter
+from itertools import chain
+from operator import attrgetter, is_, itemgetter
 from typing import Any, Final
 
 import torch
@@ -42,6 +45,9 @@ BLOCK: Final = 256  # elements that share a scale
 _FLOAT32: Final = {torch.float32}
 _DTYPE, _SHAPE, _GRAD = attrgetter("dtype"), attrgetter("shape"), attrgetter("grad")
 _NONE: Final = type(None)
+_KEYS: Final = (EXP_AVG_STATE, EXP_AVG_SCALE_STATE, EXP_AVG_RMS_STATE, EXP_AVG_RMS_SCALE_STATE,
+                ADAMW_STEP_STATE)
+_VIEWS: Final = itemgetter(*_KEYS)
 
 
 class AdamWState(Enum):
@@ -49,6 +55,32 @@ class AdamWState(Enum):
 
     FLOAT32 = "float32"   # torch's layout: two float32 tensors like the parameter
     EIGHT_BIT = "8bit"    # one byte per element and moment, a scale per 256 elements
+
+
+def _noting(name: str) -> Any:
+    """A dict method that changes an entry, and notes it."""
+    change = getattr(dict, name)
+
+    def method(self: AdamWEntry, *args: Any, **kwargs: Any) -> Any:
+        self.noted[0] = True
+        return change(self, *args, **kwargs)
+
+    return method
+
+
+class AdamWEntry(dict[str, Any]):
+    """A tensor's ``optimizer.state`` entry, which notes that a view may have been replaced or
+    removed: a step asks one flag (comparing the views of 65 tensors would take 10 us of its 85)."""
+
+    noted: list[bool] = [False]  # its pack's; this one is that of a copied entry
+
+    def __setitem__(self, key: str, value: Any) -> None:
+        if key in _KEYS:
+            self.noted[0] = True
+        super().__setitem__(key, value)
+
+    __delitem__, __ior__, update, setdefault, pop, popitem, clear = map(
+        _noting, ("__delitem__", "__ior__", "update", "setdefault", "pop", "popitem", "clear"))
 
 
 class AdamWPack:
@@ -78,6 +110,11 @@ class AdamWPack:
         self.rms_scale = torch.zeros(blocks, device=device)
         self.steps = torch.zeros(count, device=device)
         self.scalars = torch.zeros(count, 4, device=device)  # rewritten by every step
+        # The tensors' state entries, what they held when they were adopted, and whether one of
+        # them has noted a change since.
+        self.entries: list[AdamWEntry] = []
+        self.held: list[Tensor] = []
+        self.noted = [False]
         # The whole pack's host tables: a step in which every tensor has a gradient uses them.
         self.every = list(range(count))
         self.tables = self._tables(self.every)
@@ -129,8 +166,13 @@ class AdamWPack:
             ValueError: If an entry holds a state of another size.
         """
         self.check(state)
+        entries = []
         for place, param in enumerate(self.params):
             entry = state[param]
+            if not (isinstance(entry, AdamWEntry) and entry.noted is self.noted):
+                entry = state[param] = AdamWEntry(entry)
+                entry.noted = self.noted
+            entries.append(entry)
             for key, view in self.views(place).items():
                 held = entry.get(key)
                 if held is None:
@@ -138,6 +180,22 @@ class AdamWPack:
                 elif held.data_ptr() != view.data_ptr() or held.dtype != view.dtype:
                     view.copy_(held)
                 entry[key] = view
+        self.entries, self.held = entries, list(chain.from_iterable(map(_VIEWS, entries)))
+        self.noted[0] = False
+
+    def holds(self, state: ParamState, *, same_entries: bool = False) -> bool:
+        """Whether the tensors' state entries are still the pack's views (values written into
+        them are the pack's). Replaced or cleared ones count as they do for float32 state, once
+        ``adopt`` has taken them up. ``same_entries``: the caller knows that ``state`` maps the
+        tensors to the entries that were adopted."""
+        if not same_entries and not all(map(is_, map(state.get, self.params), self.entries)):
+            return False
+        if self.noted[0]:
+            try:
+                self.noted[0] = not all(map(is_, chain.from_iterable(map(_VIEWS, self.entries)), self.held))
+            except KeyError:
+                pass
+        return not self.noted[0]
 
     def moments(self, places: list[int], exp_avg: Tensor, rms: Tensor) -> None:
         """Write the values of the tensors at ``places``, one after another."""

@@ -64,6 +64,7 @@ class StepGraph:
                                                               torch.cuda.current_device())
         # Packing zeroes and copies state: do it now, outside the recording.
         optimizer._buckets()
+        optimizer._sync_adamw()
         current = torch.cuda.current_stream(device)
         capture = torch.cuda.Stream(device)
         _workspace.share(device, current.cuda_stream, capture.cuda_stream)

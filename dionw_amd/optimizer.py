@@ -24,7 +24,7 @@ from collections.abc import Callable, Iterable, Iterator
 from contextlib import contextmanager
 from contextvars import ContextVar
 from itertools import groupby
-from operator import itemgetter
+from operator import is_, itemgetter
 from typing import Any, TypeVar
 
 import torch
@@ -139,6 +139,7 @@ class Dion(IntegratedEMAOptimizer):
         self._packed: list[Bucket] | None = None
         self._adamw_packs: dict[int, list[AdamWPack]] = {}  # by group: the 8-bit ones
         self._adamw_places: dict[Tensor, tuple[AdamWPack, int]] = {}  # their parameters
+        self._state_entries: list[dict[str, Any]] = []  # the state's dicts when last looked at
         # The key is left out where nothing asks for it, so that checkpoints stay the reference's.
         more = ({} if adamw_state is AdamWState.FLOAT32
                 else {ADAMW_STATE_KEY: AdamWState(adamw_state).value})
@@ -209,6 +210,8 @@ class Dion(IntegratedEMAOptimizer):
             raise ValueError("the parameter is not in the optimizer")
         if GroupSpec.of(owner).kind is RouteKind.MATRIX:
             self._buckets()
+        elif param in self._adamw_places:
+            self._sync_adamw()
         elif EXP_AVG_STATE not in self.state[param]:
             init_adamw_state(param, self.state[param])
 
@@ -235,6 +238,35 @@ class Dion(IntegratedEMAOptimizer):
             for pack in packs:
                 pack.adopt(self.state)
 
+    def state_dict(self) -> dict[str, Any]:
+        """The state, 8-bit AdamW entries that were replaced or cleared taken up first."""
+        self._sync_adamw()
+        state = super().state_dict()
+        if self._adamw_packs:  # plain dicts, which every loader takes
+            state["state"] = {index: dict(entry) for index, entry in state["state"].items()}
+        return state
+
+    def _sync_adamw(self) -> None:
+        """Take up 8-bit AdamW entries that were replaced or cleared in ``self.state``.
+
+        Raises:
+            ValueError: If one is of another size than its parameter.
+            RuntimeError: If there are any under graph capture.
+        """
+        if not self._adamw_packs:
+            return
+        entries = self._state_entries
+        same = len(entries) == len(self.state) and all(map(is_, self.state.values(), entries))
+        stale = [pack for packs in self._adamw_packs.values() for pack in packs
+                 if not pack.holds(self.state, same_entries=same)]
+        if stale and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("Dion.step under graph capture: 8-bit AdamW state was replaced or "
+                               "cleared; run one eager step first")
+        for pack in stale:
+            pack.adopt(self.state)
+        if stale or not same:
+            self._state_entries = list(self.state.values())
+
     def adamw_moments(self, params: Iterable[Tensor]) -> tuple[Tensor, Tensor]:
         """The moments that 8-bit AdamW state stands for (not in the reference).
 
@@ -250,6 +282,7 @@ class Dion(IntegratedEMAOptimizer):
         if not held or None in held:
             raise ValueError("adamw_moments takes parameters of this optimizer's 8-bit AdamW "
                              f"groups ({ADAMW_STATE_KEY!r}: {AdamWState.EIGHT_BIT.value!r})")
+        self._sync_adamw()
         packs = set(map(itemgetter(0), held))
         device = held[0][0].exp_avg.device
         if any(pack.exp_avg.device != device for pack in packs):
@@ -301,9 +334,11 @@ class Dion(IntegratedEMAOptimizer):
 
         Raises:
             RuntimeError: If the EMA weights are in the parameters.
+            ValueError: If 8-bit AdamW state was replaced by one of another size.
         """
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             self._check_capturable()
+        self._sync_adamw()
         with self._ema_cadence():
             loss = None
             if closure is not None:
