@@ -184,6 +184,8 @@ class Dion(IntegratedEMAOptimizer):
             check_parameter(param)
         group = {**param_group, "params": params}
         spec = GroupSpec.of({**self.defaults, **group})
+        if ADAMW_STATE_KEY in group:  # the value, as the defaults hold it and checkpoints carry it
+            group[ADAMW_STATE_KEY] = spec.adamw_state.value
         super().add_param_group(group)
         self._repack()
         # With AdamW state present from the start, an integrated EMA tracks

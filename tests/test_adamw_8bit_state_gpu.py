@@ -133,3 +133,19 @@ def test_replaced_entries_are_not_recorded_in_a_graph() -> None:
     graph.replay()
     graph.replay()
     assert float(opt.state[vector]["adamw_step"]) == 7
+
+
+def test_a_group_may_name_its_state_by_the_enum(tmp_path) -> None:
+    """The group then holds the value, as with the constructor's argument: a checkpoint of either
+    loads into the other, and needs no class of this package to be read."""
+    params = _tensors([300])
+    by_enum = Dion([{"params": params, "dion_route": "adamw", "adamw_state": AdamWState.EIGHT_BIT}], **HYPER)
+    twins = _tensors([300])
+    by_argument = _optimizer(twins)
+    _step(by_enum, params, by_argument, twins, 1)
+    _same(by_enum, params, by_argument, twins)
+    for source, target in ((by_enum, by_argument), (by_argument, by_enum)):
+        torch.save(source.state_dict(), tmp_path / "opt.pt")
+        saved = torch.load(tmp_path / "opt.pt", weights_only=True)
+        assert saved["param_groups"][0]["adamw_state"] == "8bit"
+        target.load_state_dict(saved)
