@@ -128,6 +128,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_i32, _p, _i64, _i64, _i64, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p],
     ),
     "dionw_float8_expand": (ctypes.c_int, [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "dionw_float8_gemm_plan": (ctypes.c_int, [_i32, _i64, _i64, _i64, _pi32, _pi32]),
     "dionw_float8_gemm_workspace": (ctypes.c_size_t, [_i32, _i64, _i64, _i64]),
     "dionw_sum_parts": (ctypes.c_int, [_p, _i64, _i64, _i32, _p, _p]),
     "dionw_float8_gemm": (

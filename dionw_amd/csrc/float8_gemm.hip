@@ -808,6 +808,16 @@ using namespace dionw;
 
 extern "C" {
 
+int dionw_float8_gemm_plan(int32_t expanded, int64_t m, int64_t n, int64_t depth, int32_t* side,
+                           int32_t* ranges) {
+  DIONW_REQUIRE(m > 0 && n > 0 && depth > 0 && depth % kTile == 0 && side && ranges,
+                "float8_gemm_plan: bad arguments");
+  const Plan p = plan(m, n, depth / kTile * (expanded ? 2 : 1));
+  *side = kSide[p.tile];
+  *ranges = p.splits;
+  return kOk;
+}
+
 size_t dionw_float8_gemm_workspace(int32_t expanded, int64_t m, int64_t n, int64_t depth) {
   if (m <= 0 || n <= 0 || depth <= 0 || depth % kTile) return 0;
   const Plan p = plan(m, n, depth / kTile * (expanded ? 2 : 1));

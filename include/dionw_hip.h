@@ -378,8 +378,12 @@ int dionw_float8_expand(const void* data, int64_t data_ld, const void* scale, in
  * the largest of them before they are added. expanded 1: operands from dionw_float8_expand
  * (or dionw_float8_quantize), float32 output, every product exact. Pitches in elements, rows
  * of less than 8 MB at multiples of 16 bytes. workspace: float32 scratch of
- * dionw_float8_gemm_workspace bytes (0: none needed).
+ * dionw_float8_gemm_workspace bytes (0: none needed). dionw_float8_gemm_plan writes what a product
+ * of these extents runs on: the side of its tiles (256, 128 or 64) and in how many ranges its depth
+ * is summed (1: whole).
  */
+int dionw_float8_gemm_plan(int32_t expanded, int64_t m, int64_t n, int64_t depth, int32_t* side,
+                           int32_t* ranges);
 size_t dionw_float8_gemm_workspace(int32_t expanded, int64_t m, int64_t n, int64_t depth);
 int dionw_float8_gemm(int32_t expanded, int64_t m, int64_t n, int64_t depth, const void* a,
                       int64_t lda, const void* a_scale, int64_t a_scale_ld, const void* b,
