@@ -26,3 +26,18 @@ def test_training_follows_float32_and_decoding_the_model() -> None:
     for i in range(16):
         alone = decoder(tokens[i:i + 1])
         assert torch.allclose(alone[0], together[i], rtol=0, atol=0.05 * float(together.abs().max()))
+
+
+def test_decoding_ranks_the_models_token_first() -> None:
+    """Where the model's first token leads by more than twice what the test above lets a logit
+    move, decoding from kept weights must rank it first; after 200 steps it does so somewhere."""
+    model, _ = example.train(200)
+    decoder = example.Decoder(model)
+    tokens, _ = example.sequence(64, torch.Generator().manual_seed(3))
+    with torch.no_grad():
+        together = model(tokens)
+    first, second = together.topk(2, -1).values.unbind(-1)
+    clear = first - second > 2 * 0.05 * together.abs().amax()
+    assert clear.any()
+    for i in clear.nonzero().flatten().tolist():
+        assert decoder(tokens[i:i + 1]).argmax() == together[i].argmax()
