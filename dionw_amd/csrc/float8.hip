@@ -363,13 +363,8 @@ __global__ __launch_bounds__(256) void float8_quantize_rows_kernel(QuantizeArgs 
   most = max(most, turned_row<1>(most));
   const uint32_t byte = scale_byte(most);
   const u32x2 w = v.codes(power(byte));
-  uint8_t* out = q.by_row.data + row * q.by_row.ld;
-  if (q.by_row.expanded) {
-    *reinterpret_cast<bf16x8*>(out + 2 * c) = expand(w[0], w[1], half_power(byte));
-  } else {
-    *reinterpret_cast<u32x2*>(out + c) = w;
-    if (lane == 0) q.by_row.scale[block * q.by_row.scale_ld + row] = (uint8_t)byte;
-  }
+  *reinterpret_cast<u32x2*>(q.by_row.data + row * q.by_row.ld + c) = w;
+  if (lane == 0) q.by_row.scale[block * q.by_row.scale_ld + row] = (uint8_t)byte;
 }
 
 // Codes to bfloat16 halves of their values, 16 a thread.
@@ -440,7 +435,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* parts, int6
 
 template <typename T>
 int launch_quantize(const QuantizeArgs& q, bool tiles, unsigned grid, hipStream_t stream) {
-  if (!tiles && !q.by_col.data && !q.sums && ceil_div(q.rows, 16) * q.tiles_c <= kMostGroups) {
+  if (!tiles && !q.by_row.expanded && !q.by_col.data && !q.sums && ceil_div(q.rows, 16) * q.tiles_c <= kMostGroups) {
     hipLaunchKernelGGL(float8_quantize_rows_kernel<T>, dim3((unsigned)(ceil_div(q.rows, 16) * q.tiles_c)),
                        dim3(256), 0, stream, q);
     return check_launch("float8_quantize_rows");

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from dionw_amd import Float8Linear, float8_linear
+from dionw_amd import Float8Linear, _lib, float8_linear, float8_quantize_both
 from tests.test_float8_gpu import _random
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +55,35 @@ def test_autocast_is_heeded(dtype) -> None:
     got = torch.autograd.grad(y, (x, layer.weight, layer.bias), dy)
     for g, w in zip(got, torch.autograd.grad(want, (half, layer.weight, layer.bias), dy)):
         assert g.dtype is torch.float32 and torch.equal(g, w.float())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tiles", [0, 1])
+@pytest.mark.parametrize("shape", [(1, 128), (130, 200), (257, 384)])
+def test_the_library_quantizes_into_expanded_values_and_sums(shape, tiles, dtype) -> None:
+    """The entry's outputs that the Python functions do not ask for: bfloat16 halves of the
+    values, which are exact in it, and the sums of each 128 rows' columns."""
+    (m, n), x = shape, _random(*shape, 1, dtype)
+    depth, depth_t = -(-n // 128) * 128, -(-m // 128) * 128
+    rows, columns = float8_quantize_both(x, tiles=bool(tiles))
+    for expanded in (1, 2, 3):
+        data = torch.empty(m, depth, dtype=torch.bfloat16 if expanded & 1 else torch.uint8, device="cuda")
+        data_t = torch.empty(n, depth_t, dtype=torch.bfloat16 if expanded & 2 else torch.uint8, device="cuda")
+        scale, scale_t = torch.empty_like(rows.scale), torch.empty_like(columns.scale)
+        sums = torch.empty(-(-m // 128), n, device="cuda")
+        _lib.call("dionw_float8_quantize", _lib.elem_code(dtype), x.data_ptr(), m, n, n, tiles,
+                  data.data_ptr(), depth, scale.data_ptr(), scale.shape[1], data_t.data_ptr(), depth_t,
+                  scale_t.data_ptr(), scale_t.shape[1], expanded, sums.data_ptr(), _lib.stream_handle(x.device))
+        for got, want, bit in ((data, rows, 1), (data_t, columns, 2)):
+            if expanded & bit:
+                assert torch.equal(2 * got[:, :want.cols].float(), want.values())
+                assert not got[:, want.cols:].any()
+            else:
+                assert torch.equal(got, want.data.view(torch.uint8))
+        exact = torch.stack([part.double().sum(0) for part in x.split(128)])
+        size = torch.stack([part.double().abs().sum(0) for part in x.split(128)])
+        assert bool(((sums.double() - exact).abs() <= 128 * 2.0 ** -24 * size).all())
+    alone = torch.empty(m, depth, dtype=torch.bfloat16, device="cuda")
+    _lib.call("dionw_float8_quantize", _lib.elem_code(dtype), x.data_ptr(), m, n, n, tiles,
+              alone.data_ptr(), depth, None, 0, None, 0, None, 0, 1, None, _lib.stream_handle(x.device))
+    assert torch.equal(2 * alone[:, :n].float(), rows.values())
