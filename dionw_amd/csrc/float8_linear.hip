@@ -19,9 +19,15 @@ namespace {
 // Bound: HBM, n k bytes of W; the smallest calls: launch and the latency of two dependent reads.
 //
 // 16-bit calls of more rows quantize x first and go through the tiles. float32 ones would expand W
-// for that, 5 bytes of traffic for each of its codes, so up to 64 rows they run as groups of 16 here,
-// W coming from the caches after the first.
-constexpr int kFew = 16, kFewFloat = 64;
+// for that, 5 bytes of traffic for each of its codes, so they run as groups of 16 here up to 32
+// rows, and up to 64 of at most 4096 columns, each group reading W again. us for 64 rows here / 65
+// through the tiles: 4096 x 1024 7.5 / 16, 4096 x 4096 19 / 27, 14336 x 4096 70 / 61, 28672 x 4096 126 /
+// 136; 1024 x 14336 34 / 28, 4096 x 14336 60 / 61, 6144 x 14336 122 / 87, 14336 x 14336 248 / 228. For 32
+// rows here, of 14336 columns: 34, 46, 61, 125.
+constexpr int kFew = 16, kFewFloat = 32, kFewFloatShallow = 64, kShallow = 4096;
+bool few_rows(int32_t elem, int64_t m, int64_t k) {
+  return k > 0 && m <= (elem != kF32 ? kFew : k <= kShallow ? kFewFloatShallow : kFewFloat);
+}
 
 struct FewArgs {
   const void* x;
@@ -208,18 +214,24 @@ __global__ __launch_bounds__(W * 64) void float8_few_kernel(FewArgs g) {
   }
 }
 
-// R rows' fragments a wave and W waves a workgroup: many fragments take 64 rows each (x is read and
-// quantized once for them), few the most workgroups. us in a chain of launches (an empty one takes
-// 4), R W = 1 8 / 2 8 / 4 4: 1024 x 4096 5.3 / 8.1 / 13.5, 4096 x 4096 6.8 / 8.7 / 14.1, 4096 x 14336 15.0 /
-// 24.3 / 41.5, 6144 x 4096 9.6 / 9.2 / 14.4, 8192 x 4096 10.5 / 9.9 / 14.8, 10240 x 4096 13.3 / 14.9 / 15.2,
-// 14336 x 4096 (8 rows of x) 20.4 / 17.4 / 16.7, 128256 x 4096 112 / 100 / 96, with 16 rows 181 / 138 / 119.
+// R rows' fragments a wave and W waves a workgroup: many fragments (counted for each group of 16
+// tokens) take 64 rows each (x is read and quantized once for them), few the most workgroups. us in
+// a chain of launches (an empty one takes 4), R W = 1 8 / 2 8 / 4 4, bfloat16, a row of x: 1024 x 4096
+// 5.3 / 8.1 / 13.5, 4096 x 4096 6.8 / 8.7 / 14.1, 4096 x 14336 15.0 / 24.3 / 41.5, 6144 x 4096 9.6 / 9.2 / 14.4,
+// 8192 x 4096 10.5 / 9.9 / 14.8, 10240 x 4096 13.3 / 14.9 / 15.2, 14336 x 4096 (8 rows of x) 20.4 / 17.4 /
+// 16.7, 128256 x 4096 112 / 100 / 96, with 16 rows 181 / 138 / 119. The type counts between 512 and 768
+// fragments alone, 10240 x 4096: 16 bits, 16 rows 20.1 / 19.3 / 16.6, 8 16.5 / 16.9 / 15.7 (the number
+// of rows is not asked, so that a row's sums do not depend on the rows beside it); float32, 1 row
+// 19.6 / 18.7 / 16.3, 16 33 / 29 / 20. float32 groups: 2 of 4096 x 4096 23 / 15.5 / 19, 2 of 8192 x 4096 44 /
+// 30 / 20, 4 of 4096 x 14336 135 / 91 / 60, 4 of 28672 x 4096 294 / 195 / 126.
 template <typename T, bool WHOLE>
 int launch_few(const FewArgs& g, hipStream_t stream) {
   const int fragments = (g.n + 15) / 16;
   const unsigned groups = (unsigned)(g.m + 15) / 16;
-  if (fragments < 320 || (fragments > 512 && fragments < 768))
+  const int64_t all = (int64_t)fragments * groups;
+  if (all < 320 || (sizeof(T) == 2 && all > 512 && all < 768))
     hipLaunchKernelGGL((float8_few_kernel<T, 1, 8, WHOLE>), dim3(fragments, groups), dim3(512), 0, stream, g);
-  else if (fragments <= 512)
+  else if (all <= 512)
     hipLaunchKernelGGL((float8_few_kernel<T, 2, 8, WHOLE>), dim3((fragments + 1) / 2, groups), dim3(512), 0, stream, g);
   else
     hipLaunchKernelGGL((float8_few_kernel<T, 4, 4, WHOLE>), dim3((fragments + 3) / 4, groups), dim3(256), 0, stream, g);
@@ -385,7 +397,7 @@ int dionw_float8_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
 }
 
 size_t dionw_float8_linear_kept_scratch(int32_t x_elem, int64_t m, int64_t n, int64_t k) {
-  if (m <= (x_elem == kF32 ? kFewFloat : kFew) && k > 0) return 0;
+  if (few_rows(x_elem, m, k)) return 0;
   Parts room{nullptr};
   if (x_elem == kF32) {
     Forward f(room, true, m, n, k);
@@ -409,7 +421,7 @@ int dionw_float8_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const 
                     aligned16(scratch),
                 "float8_linear: an operand is too small or not aligned");
   const Matrix weight{const_cast<void*>(w), const_cast<void*>(w_scale), n, depth, w_scale_ld};
-  if (m <= (x_elem == kF32 ? kFewFloat : kFew) && k > 0) {
+  if (few_rows(x_elem, m, k)) {
     DIONW_REQUIRE(depth / kTile < INT32_MAX / 2, "float8_linear: depth too large");
     const FewArgs g{x, x_ld, static_cast<const uint8_t*>(w), w_ld, static_cast<const uint8_t*>(w_scale),
                     w_scale_ld, bias, y, k, (int32_t)m, (int32_t)n, (int32_t)(depth / kTile)};

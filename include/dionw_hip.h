@@ -416,8 +416,8 @@ int dionw_float8_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
 
 /*
  * The same y from a kept W: codes [n][w_ld] with their scales [ceil(k / 128)][w_scale_ld]. Up
- * to 16 rows of x (64 float32 ones) are quantized by the product itself, in one launch and no
- * scratch.
+ * to 16 rows of x (32 float32 ones, 64 of at most 4096 columns) are quantized by the product
+ * itself, in one launch and no scratch.
  */
 size_t dionw_float8_linear_kept_scratch(int32_t x_elem, int64_t m, int64_t n, int64_t k);
 int dionw_float8_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const void* w,

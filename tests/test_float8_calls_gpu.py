@@ -5,8 +5,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from dionw_amd import Float8Linear, _lib, float8_linear, float8_quantize_both
+from dionw_amd import Float8Linear, _lib, float8_linear, float8_quantize, float8_quantize_both
 from tests.test_float8_gpu import _random
+from tests.test_float8_tiles_gpu import _check
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,14 @@ def test_the_library_quantizes_into_expanded_values_and_sums(shape, tiles, dtype
     _lib.call("dionw_float8_quantize", _lib.elem_code(dtype), x.data_ptr(), m, n, n, tiles,
               alone.data_ptr(), depth, None, 0, None, 0, None, 0, 1, None, _lib.stream_handle(x.device))
     assert torch.equal(2 * alone[:, :n].float(), rows.values())
+
+
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 64, 65])
+@pytest.mark.parametrize("size", [(4096, 99), (4100, 99), (640, 4200), (14336, 300), (4224, 9000)], ids=str)
+def test_float32_rows_on_a_kept_weight(rows, size) -> None:
+    """Around the numbers of rows and columns at which the kernel changes, and its shapes."""
+    k, n = size
+    x, w = _random(rows, k, 5, spread=0.5), _random(n, k, 6, spread=0.3) * k ** -0.5
+    bias = torch.randn(n, device="cuda")
+    kept = float8_quantize(w, tiles=True)
+    _check(float8_linear(x, kept, bias), float8_quantize(x).values(), kept.values(), bias)
