@@ -3,7 +3,8 @@
 The optimizer keeps float32 master weights; the layer here is a way to run the model over
 them: weights, activations and gradients are quantized to e4m3 (4 exponent bits, 3 fraction
 bits, largest 448) where a product reads them, and 16-bit results come from the scaled
-8-bit matrix instructions, float32 ones (weight gradients) from bfloat16 ones on the same values. Scales are powers of two, so that scaling rounds nothing.
+8-bit matrix instructions, float32 ones (weight gradients) from bfloat16 ones on the same
+values. Scales are powers of two, so that scaling rounds nothing.
 
 - ``float8_linear(x, weight, bias)``: ``x @ weight.T + bias``, differentiable. x and the
   gradient are quantized with a scale per row and 128 columns (for the weight's gradient, per
@@ -207,7 +208,8 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
 
     A float32 result is summed in float32 on operands expanded to bfloat16, which is exact. A
     16-bit one runs on the 8-bit matrix instructions, which cut the products of each 8 columns to
-    13 bits below the exponent of the largest of them before they add (1e-5 to 6e-5 of the result).
+    13 bits below the exponent of the largest of them before they add (1e-5 to 6e-5 of the result
+    on random data, more where large products cancel).
 
     Raises:
         ValueError: For operands or a bias that do not fit each other, another dtype than
@@ -352,7 +354,8 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     128 of the weight's gradient. Under ``torch.autocast`` x is cast to its type first, as for
     ``nn.Linear``; the weight and the bias stay as they are. ``weight`` is ``[out, in]``: a float
     tensor, quantized at every call (gradients flow to x, weight and bias, the weight's in its
-    own type), or a ``Float8Matrix`` for inference.
+    own type), or a ``Float8Matrix`` for inference. A 16-bit x sums as ``float8_matmul`` does for
+    its type; ``x.float()`` has the same codes and float32 sums.
 
     Raises:
         ValueError: For shapes or types that do not fit, tensors off the GPU, an x or bias that

@@ -347,8 +347,8 @@ int dionw_adamw_8bit_values(const int64_t* numels, const int64_t* first_blocks, 
  * be NULL. One scale for each row (of the transpose: column of x) and block of 128, or for
  * each 128 x 128 tile when tiles != 0. Values that are not finite become NaN and leave their
  * block's scale alone. expanded: bit 0 for data, bit 1 for data_t: they take bfloat16 halves of
- * the values (see dionw_float8_expand; pitches in elements) and the scales are not used. sums (may be NULL): float32 [ceil(rows / 128)][cols], the column sums
- * of each 128 rows.
+ * the values (see dionw_float8_expand; pitches in elements) and the scales are not used. sums (may
+ * be NULL): float32 [ceil(rows / 128)][cols], the column sums of each 128 rows.
  */
 int dionw_float8_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
                           int32_t tiles, void* data, int64_t data_ld, void* scale,

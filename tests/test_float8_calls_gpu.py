@@ -99,3 +99,19 @@ def test_float32_rows_on_a_kept_weight(rows, size) -> None:
     bias = torch.randn(n, device="cuda")
     kept = float8_quantize(w, tiles=True)
     _check(float8_linear(x, kept, bias), float8_quantize(x).values(), kept.values(), bias)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_float32_rows_have_the_codes_of_16_bit_ones_and_exact_sums(rows, dtype) -> None:
+    """Products that cancel: 448 x 448 and its opposite beside 1 x 1 in each 8 columns. A 16-bit
+    row may lose the small ones, the same row in float32 must not."""
+    x, w = torch.ones(rows, 256, device="cuda"), torch.ones(64, 256, device="cuda")
+    x[:, 0::8], x[:, 1::8] = 448.0, -448.0
+    w[:, 0::8], w[:, 1::8] = 448.0, 448.0
+    kept = float8_quantize(w, tiles=True)
+    half = x.to(dtype)
+    assert torch.equal(float8_quantize(half).data.view(torch.uint8), float8_quantize(x).data.view(torch.uint8))
+    for weight in (w, kept):
+        assert torch.equal(float8_linear(half.float(), weight), torch.full((rows, 64), 192.0, device="cuda"))
+        _check(float8_linear(half, weight), half.float(), w)
