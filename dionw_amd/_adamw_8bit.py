@@ -48,6 +48,8 @@ _NONE: Final = type(None)
 _KEYS: Final = (EXP_AVG_STATE, EXP_AVG_SCALE_STATE, EXP_AVG_RMS_STATE, EXP_AVG_RMS_SCALE_STATE,
                 ADAMW_STEP_STATE)
 _VIEWS: Final = itemgetter(*_KEYS)
+_KEY_SET: Final = frozenset(_KEYS)
+_set_item: Final = dict.__setitem__
 
 
 class AdamWState(Enum):
@@ -75,9 +77,9 @@ class AdamWEntry(dict[str, Any]):
     noted: list[bool] = [False]  # its pack's; this one is that of a copied entry
 
     def __setitem__(self, key: str, value: Any) -> None:
-        if key in _KEYS:
+        if key in _KEY_SET:
             self.noted[0] = True
-        super().__setitem__(key, value)
+        _set_item(self, key, value)
 
     __delitem__, __ior__, update, setdefault, pop, popitem, clear = map(
         _noting, ("__delitem__", "__ior__", "update", "setdefault", "pop", "popitem", "clear"))

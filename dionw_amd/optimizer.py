@@ -23,7 +23,7 @@ from __future__ import annotations
 from collections.abc import Callable, Iterable, Iterator
 from contextlib import contextmanager
 from contextvars import ContextVar
-from itertools import groupby
+from itertools import chain, groupby
 from operator import is_, itemgetter
 from typing import Any, TypeVar
 
@@ -257,17 +257,18 @@ class Dion(IntegratedEMAOptimizer):
         """
         if not self._adamw_packs:
             return
-        entries = self._state_entries
-        same = len(entries) == len(self.state) and all(map(is_, self.state.values(), entries))
-        stale = [pack for packs in self._adamw_packs.values() for pack in packs
-                 if not pack.holds(self.state, same_entries=same)]
+        packs = list(chain.from_iterable(self._adamw_packs.values()))
+        state, entries = self.state, self._state_entries
+        same = len(entries) == len(state) and all(map(is_, state.values(), entries))
+        if same and not any(pack.noted[0] for pack in packs):
+            return
+        stale = [pack for pack in packs if not pack.holds(state, same_entries=same)]
         if stale and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("Dion.step under graph capture: 8-bit AdamW state was replaced or "
                                "cleared; run one eager step first")
         for pack in stale:
-            pack.adopt(self.state)
-        if stale or not same:
-            self._state_entries = list(self.state.values())
+            pack.adopt(state)
+        self._state_entries = list(state.values())
 
     def adamw_moments(self, params: Iterable[Tensor]) -> tuple[Tensor, Tensor]:
         """The moments that 8-bit AdamW state stands for (not in the reference).
