@@ -1,0 +1,81 @@
+"""What the operators on tensors (quantized products, layer norm) share: how they read a tensor, what
+they refuse, and how they call the library."""
+
+from __future__ import annotations
+
+from typing import Any, Final
+
+import torch
+from torch import Tensor
+from torch.autograd import forward_ad
+
+from dionw_amd import _lib
+
+DTYPES: Final = (torch.float16, torch.bfloat16, torch.float32)
+CODES: Final = {dtype: _lib.elem_code(dtype) for dtype in DTYPES}
+
+# Cheap signs of what check_unrecorded looks for: torch.jit.trace, and function modes, which
+# make_fx runs under (as harmless ones do).
+tracing = torch._C._is_tracing
+function_modes = torch._C._len_torch_function_stack
+
+
+def check_unrecorded(*tensors: Tensor | None) -> None:
+    """Kernels run on addresses, which graph recorders and forward-mode derivatives do not see: a
+    recorded graph would return the outputs' memory as it was allocated, a tangent would be lost."""
+    if torch.jit.is_tracing() or (function_modes() and _recorded_by_fx()):
+        raise ValueError("the kernels cannot be recorded by torch.jit.trace or make_fx: the graph "
+                         "would lose them")
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("these operators have no forward-mode derivative: call them on plain "
+                         "tensors, or use the backward pass")
+
+
+def watched() -> bool:
+    """Whether check_unrecorded is worth its while."""
+    return tracing() or function_modes() or forward_ad._current_level >= 0
+
+
+def _recorded_by_fx() -> bool:
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode  # takes a second to import
+
+    return get_proxy_mode() is not None
+
+
+def readable(x: Tensor) -> Tensor:
+    """A matrix as the kernels read it: rows of adjacent elements that do not overlap."""
+    adjacent = x.shape[1] <= 1 or x.stride(1) == 1
+    return x if adjacent and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
+def pitch(x: Tensor) -> int:
+    """Elements between the rows of a readable matrix."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def check_vector(name: str, v: Tensor | None, n: int, device: torch.device) -> None:
+    if v is not None and (v.shape != (n,) or v.dtype not in DTYPES or v.device != device):
+        raise ValueError(f"the {name} of {n} outputs is a float vector of that length on {device}, got "
+                         f"{v.dtype} {tuple(v.shape)} on {v.device}")
+
+
+def float_bias(bias: Tensor | None, n: int, device: torch.device) -> Tensor | None:
+    """The bias as the products read it: contiguous float32, which the caller holds until the
+    library call has returned (a temporary freed before it may be another thread's by then)."""
+    check_vector("bias", bias, n, device)
+    return None if bias is None else bias.detach().to(torch.float32).contiguous()
+
+
+def scratch(size: int, device: torch.device) -> Tensor | None:
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def call(device: torch.device, name: str, *args: Any) -> None:
+    """``_lib.call`` with ``device`` the current one: a default stream has no device of its own."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args)

@@ -45,133 +45,6 @@ struct QuantizeArgs {
   int32_t tiles_c;
 };
 
-// A thread's 8 x 8 values and what the kernel asks of them.
-template <typename T>
-struct Square {  // 16-bit
-  using P = Pair<T>;
-  static constexpr int kRowMost = 4, kColMost = 4;  // words of maxima: two rows, two columns each
-  uint32_t w[8][4];
-  __device__ __forceinline__ void load(int i, const T* at) {
-    const u32x4 v = *reinterpret_cast<const u32x4_any*>(at);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[i][k] = v[k];
-  }
-  __device__ __forceinline__ void load(int i, const T* at, int64_t left) {
-    const uint16_t* u = reinterpret_cast<const uint16_t*>(at);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t lo = 2 * k < left ? u[2 * k] : 0, hi = 2 * k + 1 < left ? u[2 * k + 1] : 0;
-      w[i][k] = lo | hi << 16;
-    }
-  }
-  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) { return P::larger(a, b); }
-  __device__ __forceinline__ void maxima(uint32_t (&row)[4], uint32_t (&col)[4]) const {
-    uint32_t one[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) col[k] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t m[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[k] = w[i][k] & 0x7FFF7FFFu;
-        col[k] = larger(col[k], m[k]);
-      }
-      one[i] = larger(larger(m[0], m[1]), larger(m[2], m[3]));
-    }
-    // Two rows a word: the larger of each row's even and odd columns.
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      row[i] = larger(__builtin_amdgcn_perm(one[2 * i + 1], one[2 * i], 0x05040100u),
-                      __builtin_amdgcn_perm(one[2 * i + 1], one[2 * i], 0x07060302u));
-  }
-  __device__ __forceinline__ static bool odd(uint32_t m) {  // not finite
-    return (m & 0xFFFFu) >= P::inf || (m >> 16) >= P::inf;
-  }
-  // The float32 bits of maximum i of the words.
-  __device__ __forceinline__ static uint32_t bits(const uint32_t (&m)[4], int i) {
-    return P::bits(i & 1 ? m[i >> 1] >> 16 : m[i >> 1] & 0xFFFFu);
-  }
-  // The maxima of the finite values.
-  __device__ __forceinline__ void finite_maxima(uint32_t (&row)[4], uint32_t (&col)[4]) const {
-    Square kept;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t lo = w[i][k] & 0x7FFFu, hi = w[i][k] & 0x7FFF0000u;
-        kept.w[i][k] = (lo < P::inf ? lo : 0u) | (hi < P::inf << 16 ? hi : 0u);
-      }
-    kept.maxima(row, col);
-  }
-  __device__ __forceinline__ u32x2 row_codes(int i, float scale) const {
-    return u32x2{codes4(w[i][0], w[i][1], scale, T{}), codes4(w[i][2], w[i][3], scale, T{})};
-  }
-  __device__ __forceinline__ u32x2 col_codes(int k, float scale) const {
-    uint32_t p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      p[i] = __builtin_amdgcn_perm(w[2 * i + 1][k >> 1], w[2 * i][k >> 1], k & 1 ? 0x07060302u : 0x05040100u);
-    return u32x2{codes4(p[0], p[1], scale, T{}), codes4(p[2], p[3], scale, T{})};
-  }
-  __device__ __forceinline__ float value(int i, int k) const { return P{w[i][k >> 1]}.value(k & 1); }
-};
-
-template <>
-struct Square<float> {
-  static constexpr int kRowMost = 8, kColMost = 8;
-  static constexpr uint32_t inf = 0x7F800000u;
-  uint32_t w[8][8];
-  __device__ __forceinline__ void load(int i, const float* at) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x4 v = *reinterpret_cast<const u32x4_any*>(at + 4 * h);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[i][4 * h + k] = v[k];
-    }
-  }
-  __device__ __forceinline__ void load(int i, const float* at, int64_t left) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) w[i][k] = k < left ? __float_as_uint(at[k]) : 0;
-  }
-  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
-  __device__ __forceinline__ void maxima(uint32_t (&row)[8], uint32_t (&col)[8]) const {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) row[k] = col[k] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t m = w[i][k] & 0x7FFFFFFFu;
-        row[i] = max(row[i], m);
-        col[k] = max(col[k], m);
-      }
-  }
-  __device__ __forceinline__ static bool odd(uint32_t m) { return m >= inf; }
-  __device__ __forceinline__ static uint32_t bits(const uint32_t (&m)[8], int i) { return m[i]; }
-  __device__ __forceinline__ void finite_maxima(uint32_t (&row)[8], uint32_t (&col)[8]) const {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) row[k] = col[k] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t b = w[i][k] & 0x7FFFFFFFu, m = b < inf ? b : 0u;
-        row[i] = max(row[i], m);
-        col[k] = max(col[k], m);
-      }
-  }
-  __device__ __forceinline__ u32x2 row_codes(int i, float scale) const {
-    return u32x2{codes4(w[i][0], w[i][1], w[i][2], w[i][3], scale),
-                 codes4(w[i][4], w[i][5], w[i][6], w[i][7], scale)};
-  }
-  __device__ __forceinline__ u32x2 col_codes(int k, float scale) const {
-    return u32x2{codes4(w[0][k], w[1][k], w[2][k], w[3][k], scale),
-                 codes4(w[4][k], w[5][k], w[6][k], w[7][k], scale)};
-  }
-  __device__ __forceinline__ float value(int i, int k) const { return __uint_as_float(w[i][k]); }
-};
-
 // Eight values of a row, and the float32 bits of their largest finite magnitude.
 template <typename T>
 struct Line {

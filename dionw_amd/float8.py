@@ -30,37 +30,23 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from dionw_amd import _lib
+from dionw_amd._operands import (
+    CODES,
+    DTYPES,
+    check_unrecorded,
+    check_vector,
+    float_bias,
+    function_modes,
+    pitch,
+    readable,
+    scratch as _scratch,
+    tracing,
+)
 
 __all__ = ["Float8Linear", "Float8Matrix", "float8_linear", "float8_matmul", "float8_quantize",
            "float8_quantize_both"]
 
 TILE: Final = 128  # columns (and rows) that share a scale
-_DTYPES: Final = (torch.float16, torch.bfloat16, torch.float32)
-_CODES: Final = {dtype: _lib.elem_code(dtype) for dtype in _DTYPES}
-
-
-# Cheap signs of what _check_unrecorded looks for: torch.jit.trace, and function modes, which
-# make_fx runs under (as harmless ones do).
-_tracing = torch._C._is_tracing
-_function_modes = torch._C._len_torch_function_stack
-
-
-def _check_unrecorded(*tensors: Tensor | None) -> None:
-    """Kernels run on addresses, which graph recorders and forward-mode derivatives do not see: a
-    recorded graph would return the outputs' memory as it was allocated, a tangent would be lost."""
-    if torch.jit.is_tracing() or (_function_modes() and _recorded_by_fx()):
-        raise ValueError("the 8-bit kernels cannot be recorded by torch.jit.trace or make_fx: the "
-                         "graph would lose them")
-    if forward_ad._current_level >= 0 and any(
-            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        raise ValueError("the 8-bit operators have no forward-mode derivative: call them on plain "
-                         "tensors, or use the backward pass")
-
-
-def _recorded_by_fx() -> bool:
-    from torch.fx.experimental.proxy_tensor import get_proxy_mode  # takes a second to import
-
-    return get_proxy_mode() is not None
 
 
 @dataclass(frozen=True, eq=False)
@@ -149,22 +135,16 @@ def _product(m: int, n: int, depth: int, a: tuple[int, int | None, int], b: tupl
 
 def _readable(x: Tensor) -> Tensor:
     """x as the kernels read it: rows of adjacent elements that do not overlap."""
-    if x.dim() != 2 or x.dtype not in _DTYPES:
+    if x.dim() != 2 or x.dtype not in DTYPES:
         raise ValueError("8-bit quantization takes a float16, bfloat16 or float32 matrix, got "
                          f"{x.dtype} of shape {tuple(x.shape)}")
-    adjacent = x.shape[1] <= 1 or x.stride(1) == 1
-    return x if adjacent and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
-
-
-def _pitch(x: Tensor) -> int:
-    """Elements between the rows of a readable matrix."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    return readable(x)
 
 
 def _quantize(x: Tensor, tiles: bool, both: bool) -> tuple[Float8Matrix, Float8Matrix | None]:
     """x quantized by rows, and its transpose quantized by rows where both are asked for."""
-    if _tracing() or _function_modes():
-        _check_unrecorded()
+    if tracing() or function_modes():
+        check_unrecorded()
     x = _readable(x)
     m, n = x.shape
     stream = _lib.stream_handle(x.device)
@@ -174,7 +154,7 @@ def _quantize(x: Tensor, tiles: bool, both: bool) -> tuple[Float8Matrix, Float8M
         return (None, 0, None, 0) if q is None else (
             q.data.data_ptr(), q.data.shape[1], q.scale.data_ptr(), q.scale.shape[1])
 
-    _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, _pitch(x),
+    _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, pitch(x),
               int(tiles), *place(by_row), *place(by_column), 0, None, stream)
     return by_row, by_column
 
@@ -216,8 +196,8 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
             float16, bfloat16 or float32, tensors off the GPU, a bias that requires a gradient,
             a forward-mode dual, or a call that ``torch.jit.trace`` or ``make_fx`` records.
     """
-    if _tracing() or _function_modes() or forward_ad._current_level >= 0:
-        _check_unrecorded(bias)
+    if tracing() or function_modes() or forward_ad._current_level >= 0:
+        check_unrecorded(bias)
     m, n = a.shape[0], b.shape[0]
     if a.cols != b.cols or a.device != b.device:
         raise ValueError(f"float8_matmul takes matrices of one depth on one device, got {a.shape} on "
@@ -225,7 +205,7 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError("float8_matmul gives its bias no gradient: pass it detached, or use "
                          "float8_linear on the float weight")
-    bias = _bias(bias, n, a.device)
+    bias = float_bias(bias, n, a.device)
     _lib.elem_code(dtype)
     depth = a.data.shape[1]
     if dtype is torch.float32:
@@ -234,19 +214,6 @@ def float8_matmul(a: Float8Matrix, b: Float8Matrix, bias: Tensor | None = None, 
                         a.device)
     return _product(m, n, depth, (a.data.data_ptr(), a.scale.data_ptr(), a.scale.shape[1]),
                     (b.data.data_ptr(), b.scale.data_ptr(), b.scale.shape[1]), bias, dtype, a.device)
-
-
-def _check_bias(bias: Tensor | None, n: int, device: torch.device) -> None:
-    if bias is not None and (bias.shape != (n,) or bias.dtype not in _DTYPES or bias.device != device):
-        raise ValueError(f"the bias of {n} outputs is a float vector of that length on {device}, got "
-                         f"{bias.dtype} {tuple(bias.shape)} on {bias.device}")
-
-
-def _bias(bias: Tensor | None, n: int, device: torch.device) -> Tensor | None:
-    """The bias as the product reads it: contiguous float32, which the caller holds until the
-    library call has returned (a temporary freed before it may be another thread's by then)."""
-    _check_bias(bias, n, device)
-    return None if bias is None else bias.detach().to(torch.float32).contiguous()
 
 
 @lru_cache(maxsize=256)
@@ -258,24 +225,20 @@ def _sizes(x_code: int, w_code: int, m: int, n: int, k: int, need_x: bool, need_
     return sizes[0], sizes[1], sizes[2]
 
 
-def _scratch(size: int, device: torch.device) -> Tensor | None:
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-
-
 def _forward(x: Tensor, weight: Tensor, bias: Tensor | None, need_x: bool, need_w: bool,
              need_b: bool) -> tuple[Tensor, Tensor | None, int]:
     """y, what the gradients asked for need of x and W, and the bytes of the backward's scratch."""
     x, weight = _readable(x), _readable(weight)
     m, k = x.shape
     n, device = weight.shape[0], x.device
-    x_code, w_code = _CODES[x.dtype], _CODES[weight.dtype]
+    x_code, w_code = CODES[x.dtype], CODES[weight.dtype]
     stream = _lib.stream_handle(device)
     keep, room, backward_room = _sizes(x_code, w_code, m, n, k, need_x, need_w, need_b)
     saved, scratch = _scratch(keep, device), _scratch(room, device)
     y = torch.empty(m, n, dtype=x.dtype, device=device)
-    added = _bias(bias, n, device)
-    _lib.call("dionw_float8_linear_forward", x_code, x.data_ptr(), _pitch(x), w_code,
-              weight.data_ptr(), _pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
+    added = float_bias(bias, n, device)
+    _lib.call("dionw_float8_linear_forward", x_code, x.data_ptr(), pitch(x), w_code,
+              weight.data_ptr(), pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
               y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
     return y, saved, backward_room
 
@@ -286,7 +249,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
         y, saved, ctx.room = _forward(x, weight, bias, *ctx.needs_input_grad)
-        ctx.codes = _CODES[x.dtype], _CODES[weight.dtype]
+        ctx.codes = CODES[x.dtype], CODES[weight.dtype]
         ctx.sizes, ctx.dtypes = (x.shape[0], *weight.shape), (x.dtype, weight.dtype)
         ctx.bias_dtype = bias.dtype if ctx.needs_input_grad[2] else None
         ctx.save_for_backward(*([] if saved is None else [saved]))
@@ -303,7 +266,7 @@ class _Linear(torch.autograd.Function):
         dx = torch.empty(m, k, dtype=ctx.dtypes[0], device=device) if need_x else None
         dw = torch.empty(n, k, dtype=ctx.dtypes[1], device=device) if need_w else None
         db = torch.empty(n, dtype=ctx.bias_dtype, device=device) if need_b else None
-        _lib.call("dionw_float8_linear_backward", ctx.codes[0], dy.data_ptr(), _pitch(dy), ctx.codes[1],
+        _lib.call("dionw_float8_linear_backward", ctx.codes[0], dy.data_ptr(), pitch(dy), ctx.codes[1],
                   m, n, k, need_x, need_w, _lib.ptr(saved), _lib.ptr(dx), _lib.ptr(dw),
                   _lib.elem_code(ctx.bias_dtype) if need_b else 0, _lib.ptr(db), _lib.ptr(scratch),
                   ctx.room, _lib.stream_handle(device))
@@ -318,7 +281,7 @@ def _kept_scratch(code: int, m: int, n: int, k: int) -> int:
 def _kept_linear(x: Tensor, weight: Float8Matrix, bias: Tensor | None) -> Tensor:
     # Decoding waits for the host here: every attribute is read once.
     data, scale, k, dtype = weight.data, weight.scale, weight.cols, x.dtype
-    device, shape, code = data.device, x.shape, _CODES.get(dtype)
+    device, shape, code = data.device, x.shape, CODES.get(dtype)
     n, depth = data.shape
     if not shape or shape[-1] != k or x.device != device or code is None:
         raise ValueError(f"float8_linear takes float x [..., {k}] on {device} for this weight, got "
@@ -332,16 +295,16 @@ def _kept_linear(x: Tensor, weight: Float8Matrix, bias: Tensor | None) -> Tensor
     else:
         m, out = math.prod(shape[:-1]), (*shape[:-1], n)
         x = x.reshape(m, k)
-    pitch = k
+    ld = k
     if not x.is_contiguous():
         x = _readable(x)
-        pitch = _pitch(x)
+        ld = pitch(x)
     if bias is not None:
-        bias = _bias(bias, n, device)
+        bias = float_bias(bias, n, device)
     room = _kept_scratch(code, m, n, k)
     scratch = _scratch(room, device) if room else None
     y = x.new_empty(out)
-    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), pitch, data.data_ptr(), depth,
+    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), ld, data.data_ptr(), depth,
               scale.data_ptr(), scale.shape[1], None if bias is None else bias.data_ptr(), m, n, k,
               y.data_ptr(), _lib.ptr(scratch), room, stream)
     return y
@@ -364,9 +327,9 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
             float32 result) and more, a gradient's included.
     """
     kept = isinstance(weight, Float8Matrix)
-    if _tracing() or _function_modes() or forward_ad._current_level >= 0:
-        _check_unrecorded(x, None if kept else weight, bias)
-    if torch.is_autocast_enabled() and x.dtype in _CODES:
+    if tracing() or function_modes() or forward_ad._current_level >= 0:
+        check_unrecorded(x, None if kept else weight, bias)
+    if torch.is_autocast_enabled() and x.dtype in CODES:
         x = x.to(torch.get_autocast_dtype("cuda"))
     if kept:
         return _kept_linear(x, weight, bias)
@@ -376,7 +339,7 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
                          f"{tuple(shape)} and {tuple(weight.shape)}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    _check_bias(bias, weight.shape[0], x.device)
+    check_vector("bias", bias, weight.shape[0], x.device)
     flat = x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), shape[-1])
     # Asked here: inside the function gradients are off, and what it is told of its inputs' needs
     # does not know whether they were on.
