@@ -19,6 +19,14 @@ from dionw_amd._keys import (
 )
 from dionw_amd._adamw_8bit import AdamWState
 from dionw_amd.ema import EMAConfig, EMADevice, EMASchedule, IntegratedEMAOptimizer
+from dionw_amd.float4 import (
+    Float4Linear,
+    Float4Matrix,
+    float4_linear,
+    float4_matmul,
+    float4_quantize,
+    float4_quantize_both,
+)
 from dionw_amd.float8 import (
     Float8Linear,
     Float8Matrix,
@@ -27,6 +35,7 @@ from dionw_amd.float8 import (
     float8_quantize,
     float8_quantize_both,
 )
+from dionw_amd.layer_norm import LayerNorm, float4_layer_norm, layer_norm
 from dionw_amd.matrix_update import (
     DION3_UPDATE,
     MUON_UPDATE,
@@ -61,9 +70,12 @@ __all__ = [
     "EMAConfig",
     "EMADevice",
     "EMASchedule",
+    "Float4Linear",
+    "Float4Matrix",
     "Float8Linear",
     "Float8Matrix",
     "IntegratedEMAOptimizer",
+    "LayerNorm",
     "MatrixUpdate",
     "MomentumForm",
     "NewtonSchulz",
@@ -76,9 +88,15 @@ __all__ = [
     "RoutingReport",
     "RowNormalization",
     "__version__",
+    "float4_layer_norm",
+    "float4_linear",
+    "float4_matmul",
+    "float4_quantize",
+    "float4_quantize_both",
     "float8_linear",
     "float8_matmul",
     "float8_quantize",
     "float8_quantize_both",
+    "layer_norm",
     "param_groups",
 ]

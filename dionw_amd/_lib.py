@@ -152,6 +152,47 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         ctypes.c_int,
         [_i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, ctypes.c_size_t, _p],
     ),
+    "dionw_float4_quantize": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i64, _i64, _i32, _i64, _p, _p, _p, _i64, _p, _p, _i64, _p],
+    ),
+    "dionw_float4_values": (ctypes.c_int, [_p, _p, _i64, _i64, _i64, _p, _p]),
+    "dionw_float4_gemm_plan": (ctypes.c_int, [_i64, _i64, _i64, _pi32, _pi32]),
+    "dionw_float4_gemm_workspace": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "dionw_float4_gemm": (
+        ctypes.c_int,
+        [_i64, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _p, _i32, _p, _i64, _p, ctypes.c_size_t, _p],
+    ),
+    "dionw_float4_linear_sizes": (None, [_i64, _i64, _i64, _i32, _i32, _i32, _psize]),
+    "dionw_float4_linear_forward": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i32, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p,
+         ctypes.c_size_t, _p],
+    ),
+    "dionw_float4_linear_backward": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i32, _i64, _i64, _i64, _i32, _i32, _i64, _p, _p, _p, _p, _i32, _p, _p,
+         ctypes.c_size_t, _p],
+    ),
+    "dionw_float4_linear_kept_scratch": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "dionw_float4_linear_kept": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _p, _p, ctypes.c_size_t, _p],
+    ),
+    "dionw_layer_norm_forward": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i64, _i64, _i32, _p, _i32, _p, _f32, _p, _p, _p, _p],
+    ),
+    "dionw_layer_norm_float4": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _i64, _i64, _i32, _p, _i32, _p, _f32, _p, _p, _i64, _p],
+    ),
+    "dionw_layer_norm_backward_scratch": (ctypes.c_size_t, [_i64, _i64]),
+    "dionw_layer_norm_backward": (
+        ctypes.c_int,
+        [_i32, _p, _i64, _p, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _p, _i32, _p, _p,
+         ctypes.c_size_t, _p],
+    ),
     "dionw_ema_update": (ctypes.c_int, [_pp, _pp, _pi64, _i32, _f32, _i32, _p]),
 }
 

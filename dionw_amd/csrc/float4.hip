@@ -1,0 +1,463 @@
+// 4-bit floating-point matrices with a scale for each block of 32: quantization and reading back.
+//
+// A quantized matrix holds e2m1 codes (a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6) row-major, two a
+// byte, the first in its low half, its columns padded with zeros to a multiple of 256, and for every
+// row and block of 32 columns the exponent byte of a float32 power of two (255: the block is NaN).
+// Scaling by powers of two rounds nothing, and the matrix instructions multiply by them on the way.
+// Bytes are kept by column block, [blocks][rows], so that the rows of a tile lie side by side.
+//
+// A weight's bytes are equal within each 32 x 32 tile, so that its transpose holds the same values;
+// an activation's or a gradient's differ from row to row. Gradients are rounded stochastically: to
+// nearest, what is smaller than a quarter of its block's step is lost from every sum, in 4 bits a
+// large part of a gradient; up or down by chance the sums over many rows stay right on average.
+#include "float4.h"
+
+namespace dionw {
+namespace {
+
+// The most workgroups of 256 a launch takes (2^32 threads).
+constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;
+
+struct Output {
+  uint8_t* data;  // null: not asked for
+  int64_t ld;     // bytes
+  uint8_t* scale;
+  int64_t scale_ld;
+};
+struct QuantizeArgs {
+  const void* x;
+  int64_t rows, cols, ld;
+  Output by_row, by_col;  // x, and its transpose
+  float* sums;            // [tiles of 128 rows][cols]: each tile's column sums, or null
+  int32_t tiles_c;
+  int32_t far;            // 2^32 pairs of columns or more
+  Noise noise;
+};
+
+// ---- by rows and by columns ----------------------------------------------------------
+//
+// A workgroup takes a 128 x 128 tile: thread t the rows 8 (t / 16) .. + 7 and the columns
+// 8 (t % 16) .. + 7, read once and held as they are. A wave then holds 32 rows of 128 columns, so
+// that every block of either form is a wave's own: 4 lanes side by side hold a row's block, 4 of a
+// column of lanes a column's. Codes by rows go from registers to memory, those of the transpose
+// through LDS, each in 64-byte runs; the scales through LDS, so that a block's rows are written
+// together. Tiles past the last row or column, up to the padding of the other form, write zeros.
+// Bound: HBM, 2 or 4 bytes read and half a byte written for each form an element.
+enum Rounding : int { kRows = 0, kTiles = 1, kStochastic = 2 };
+
+struct Shared {
+  // Words of the transpose: 17 a column, so that a wave's writes spread over the banks.
+  static constexpr int pitch = 17;
+  uint32_t turned[128 * pitch];
+  float col_sum[4][128];
+  __attribute__((aligned(16))) uint8_t row_bytes[4][128], col_bytes[4][128];
+};
+
+template <typename T>
+struct Codes {
+  using S = Square<T>;
+  template <int B>
+  __device__ __forceinline__ static uint32_t row_pair(uint32_t old, const S& v, int i, float scale) {
+    if constexpr (sizeof(T) == 4) return codes2<B>(old, v.value(i, 2 * B), v.value(i, 2 * B + 1), scale);
+    else return codes2<B>(old, v.w[i][B], scale, T{});
+  }
+  template <int B>
+  __device__ __forceinline__ static uint32_t col_pair(uint32_t old, const S& v, int k, float scale) {
+    if constexpr (sizeof(T) == 4)
+      return codes2<B>(old, v.value(2 * B, k), v.value(2 * B + 1, k), scale);
+    else
+      return codes2<B>(old, __builtin_amdgcn_perm(v.w[2 * B + 1][k >> 1], v.w[2 * B][k >> 1],
+                                                  k & 1 ? 0x07060302u : 0x05040100u), scale, T{});
+  }
+  __device__ __forceinline__ static uint32_t row(const S& v, int i, float scale) {
+    return row_pair<3>(row_pair<2>(row_pair<1>(row_pair<0>(0, v, i, scale), v, i, scale), v, i, scale), v, i, scale);
+  }
+  __device__ __forceinline__ static uint32_t col(const S& v, int k, float scale) {
+    return col_pair<3>(col_pair<2>(col_pair<1>(col_pair<0>(0, v, k, scale), v, k, scale), v, k, scale), v, k, scale);
+  }
+};
+
+// Codes of 8 values that are the format's already.
+__device__ __forceinline__ uint32_t exact_codes(const float (&v)[8]) {
+  uint32_t c = codes2<0>(0, v[0], v[1], 1.f);
+  c = codes2<1>(c, v[2], v[3], 1.f);
+  c = codes2<2>(c, v[4], v[5], 1.f);
+  return codes2<3>(c, v[6], v[7], 1.f);
+}
+
+template <typename T, int ROUNDING>
+__device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t tile, Shared& shared) {
+  using S = Square<T>;
+  constexpr int RM = S::kRowMost, CM = S::kColMost, kPitch = Shared::pitch;
+  constexpr bool TILES = ROUNDING == kTiles, NOISY = ROUNDING == kStochastic;
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int64_t r0 = (int64_t)(tile / q.tiles_c) * 128;
+  const int64_t c0 = (int64_t)(tile % q.tiles_c) * 128;
+  const int tr = tid / 16 * 8, tc = tid % 16 * 8;  // the thread's first row and column
+  S v;
+  const T* at = reinterpret_cast<const T*>(q.x) + (r0 + tr) * q.ld + c0 + tc;
+  if (r0 + tr + 8 <= q.rows && c0 + tc + 8 <= q.cols) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.load(i, at + i * q.ld);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v.load(i, at + i * q.ld, r0 + tr + i < q.rows ? q.cols - c0 - tc : 0);
+  }
+  uint32_t row[RM], col[CM], tile_byte = 0;
+  v.maxima(row, col);
+  if (TILES) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = max(most, S::bits(col, k));
+    most = largest_of_four(most);
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+    tile_byte = scale_byte4<false>(most);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      row[i] = S::larger(row[i], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)row[i], 0xB1, 0xF, 0xF, false));
+      row[i] = S::larger(row[i], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)row[i], 0x4E, 0xF, 0xF, false));
+    }
+    if (q.by_col.data) {
+#pragma unroll
+      for (int k = 0; k < CM; ++k) {
+        col[k] = S::larger(col[k], (uint32_t)__shfl_xor((int)col[k], 16, kWave));
+        col[k] = S::larger(col[k], (uint32_t)__shfl_xor((int)col[k], 32, kWave));
+      }
+    }
+  }
+  if (q.sums) {
+    float s[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[k] += v.value(i, k);
+    }
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] += __shfl_xor(s[k], off, kWave);
+    if ((tid & 63) < 16)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) shared.col_sum[wave][tc + k] = s[k];
+  }
+  uint32_t h[8][4];
+  if constexpr (NOISY) {
+    const uint32_t key = noise_key(q.noise), near = mix32(key);
+    const int64_t pairs = (q.cols + 1) / 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t p = (r0 + tr + i) * pairs + (c0 + tc) / 2;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        h[i][k] = mix32((uint32_t)(p + k) ^ (q.far ? mix32(key + (uint32_t)((p + k) >> 32)) : near));
+    }
+  }
+  auto noise = [&](int i, int k) { return k & 1 ? odd_noise(h[i][k >> 1]) : even_noise(h[i][k >> 1]); };
+  if (q.by_row.data) {
+    uint8_t* out = q.by_row.data + (r0 + tr) * q.by_row.ld + (c0 + tc) / 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, out += q.by_row.ld) {
+      const uint32_t byte = TILES ? tile_byte : scale_byte4<NOISY>(S::bits(row, i));
+      uint32_t w;
+      if constexpr (NOISY) {
+        const float scale = power(byte), inverse = inverse4(byte);
+        float e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = stochastic4(v.value(i, k), scale, inverse, noise(i, k));
+        w = exact_codes(e);
+      } else {
+        w = Codes<T>::row(v, i, power(byte));
+      }
+      if (r0 + tr + i < q.rows) *reinterpret_cast<uint32_t*>(out) = w;
+      if (tid % 4 == 0) shared.row_bytes[tid % 16 / 4][tr + i] = (uint8_t)byte;
+    }
+  }
+  if (q.by_col.data) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t byte = TILES ? tile_byte : scale_byte4<NOISY>(S::bits(col, k));
+      uint32_t w;
+      if constexpr (NOISY) {
+        const float scale = power(byte), inverse = inverse4(byte);
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = stochastic4(v.value(i, k), scale, inverse, noise(i, k));
+        w = exact_codes(e);
+      } else {
+        w = Codes<T>::col(v, k, power(byte));
+      }
+      shared.turned[(tc + k) * kPitch + tr / 8] = w;
+      if ((tid & 63) < 16) shared.col_bytes[wave][tc + k] = (uint8_t)byte;
+    }
+  }
+  __syncthreads();
+  if (q.sums && tid < 128 && c0 + tid < q.cols)
+    q.sums[r0 / 128 * q.cols + c0 + tid] = (shared.col_sum[0][tid] + shared.col_sum[1][tid]) +
+                                           (shared.col_sum[2][tid] + shared.col_sum[3][tid]);
+  // A block's bytes run to a multiple of 16: 4 of them a thread, the first 128 threads the rows'.
+  const int b = tid / 32 % 4, place = tid % 32 * 4;
+  const Output& o = tid < 128 ? q.by_row : q.by_col;
+  const int64_t first = tid < 128 ? r0 : c0, other = tid < 128 ? c0 : r0;
+  if (o.data && first + place < o.scale_ld)
+    *reinterpret_cast<uint32_t*>(o.scale + (other / kBlock4 + b) * o.scale_ld + first + place) =
+        *reinterpret_cast<const uint32_t*>((tid < 128 ? shared.row_bytes[b] : shared.col_bytes[b]) + place);
+  if (!q.by_col.data) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int c = j * 64 + tid / 4, word = tid % 4 * 4;
+    if (c0 + c >= q.cols) continue;
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = shared.turned[c * kPitch + word + k];
+    *reinterpret_cast<u32x4*>(q.by_col.data + (c0 + c) * q.by_col.ld + r0 / 2 + 4 * word) = w;
+  }
+}
+
+template <typename T, int ROUNDING>
+__global__ __launch_bounds__(256) void float4_quantize_kernel(QuantizeArgs q) {
+  __shared__ Shared shared;
+  quantize_tile<T, ROUNDING>(q, blockIdx.x, shared);
+}
+
+// What a linear layer's forward pass quantizes, in one launch: a small layer's parts hide each
+// other's latency.
+template <typename TX, typename TW>
+__global__ __launch_bounds__(256) void float4_quantize_pair_kernel(QuantizeArgs x, QuantizeArgs w,
+                                                                   uint32_t x_tiles) {
+  __shared__ Shared shared;
+  if (blockIdx.x < x_tiles)
+    quantize_tile<TX, kRows>(x, blockIdx.x, shared);
+  else
+    quantize_tile<TW, kTiles>(w, blockIdx.x - x_tiles, shared);
+}
+
+// ---- by rows alone ---------------------------------------------------------------------
+//
+// A workgroup takes 8 R rows of 256 columns, 32 lanes a row, 8 columns a lane: nothing goes through
+// LDS but the scales. Few rows take R = 1, so that they still fill the GPU.
+template <typename T, int R>
+__global__ __launch_bounds__(256) void float4_quantize_rows_kernel(QuantizeArgs q) {
+  __shared__ __attribute__((aligned(16))) uint8_t bytes[8][8 * R];
+  const int tid = threadIdx.x, lane = tid & 31, y = tid >> 5;
+  const int64_t r0 = (int64_t)(blockIdx.x / q.tiles_c) * (8 * R);
+  const int64_t stage = blockIdx.x % q.tiles_c, c = stage * kDepth4 + 8 * lane;
+  Square<T> v;  // R of its rows
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int64_t row = r0 + 8 * i + y;
+    const T* at = reinterpret_cast<const T*>(q.x) + row * q.ld + c;
+    if (row < q.rows && c + 8 <= q.cols) v.load(i, at);
+    else v.load(i, at, row < q.rows ? q.cols - c : 0);
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(v.value(i, k)) & 0x7FFFFFFFu);
+    const uint32_t byte = scale_byte4<false>(largest_of_four(most));
+    const uint32_t w = Codes<T>::row(v, i, power(byte));
+    const int64_t row = r0 + 8 * i + y;
+    if (row < q.rows) *reinterpret_cast<uint32_t*>(q.by_row.data + row * q.by_row.ld + c / 2) = w;
+    if (lane % 4 == 0) bytes[lane / 4][8 * i + y] = (uint8_t)byte;
+  }
+  __syncthreads();
+  if (tid < 16 * R) {  // 4 rows' bytes of a block a thread
+    const int b = tid / (2 * R), place = tid % (2 * R) * 4;
+    if (r0 + place < q.by_row.scale_ld)
+      *reinterpret_cast<uint32_t*>(q.by_row.scale + (stage * 8 + b) * q.by_row.scale_ld + r0 + place) =
+          *reinterpret_cast<const uint32_t*>(bytes[b] + place);
+  }
+}
+
+// ---- reading back ------------------------------------------------------------------------
+//
+// The float32 values: a workgroup takes 32 rows of 256 columns, 8 columns of 4 rows a lane; the
+// scales come through LDS, as a lane's rows lie together there.
+// Bound: HBM, half a byte read and 4 written an element.
+struct ValuesArgs {
+  const uint8_t* data;
+  const uint8_t* scale;
+  int64_t scale_ld, rows, cols, depth;
+  float* out;
+  int32_t stages;
+};
+__global__ __launch_bounds__(256) void float4_values_kernel(ValuesArgs g) {
+  __shared__ uint8_t bytes[8][32];
+  const int tid = threadIdx.x, lane = tid & 31, y = tid >> 5;
+  const int64_t r0 = (int64_t)(blockIdx.x / g.stages) * 32, stage = blockIdx.x % g.stages;
+  const int64_t c = stage * kDepth4 + 8 * lane;
+  bytes[y][lane] = r0 + lane < g.rows ? g.scale[(stage * 8 + y) * g.scale_ld + r0 + lane] : 0;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = min(r0 + 8 * i + y, g.rows - 1);
+    w[i] = *reinterpret_cast<const uint32_t*>(g.data + row * (g.depth / 2) + c / 2);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = r0 + 8 * i + y;
+    if (row >= g.rows || c >= g.cols) continue;
+    const uint32_t byte = bytes[lane / 4][8 * i + y];
+    const float scale = byte == 255 ? __uint_as_float(0x7FC00000u) : power(byte);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 1);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 2);
+    const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 3);
+    const float v[8] = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale,
+                        d[0] * scale, d[1] * scale, e[0] * scale, e[1] * scale};
+    float* to = g.out + row * g.cols + c;
+    if (c + 8 <= g.cols) {
+      typedef float f4any __attribute__((ext_vector_type(4), aligned(4)));
+      *reinterpret_cast<f4any*>(to) = f4any{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f4any*>(to + 4) = f4any{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k < g.cols) to[k] = v[k];
+    }
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------
+
+template <typename T>
+int launch_rows(QuantizeArgs q, hipStream_t stream) {
+  q.tiles_c = (int32_t)(q.by_row.ld * 2 / kDepth4);
+  const int64_t most = ceil_div(q.rows, 8) * q.tiles_c;
+  const bool few = most < 2048;
+  const int64_t grid = ceil_div(q.rows, few ? 8 : 32) * q.tiles_c;
+  DIONW_REQUIRE(grid <= kMostGroups, "float4_quantize: too many tiles");
+  if (few)
+    hipLaunchKernelGGL((float4_quantize_rows_kernel<T, 1>), dim3((unsigned)grid), dim3(256), 0, stream, q);
+  else
+    hipLaunchKernelGGL((float4_quantize_rows_kernel<T, 4>), dim3((unsigned)grid), dim3(256), 0, stream, q);
+  return check_launch("float4_quantize_rows");
+}
+
+template <typename T>
+int launch_quantize(const QuantizeArgs& q, int rounding, int64_t tiles, hipStream_t stream) {
+  if (rounding == kRows && !q.by_col.data && !q.sums) return launch_rows<T>(q, stream);
+  const dim3 grid((unsigned)tiles);
+  if (rounding == kRows)
+    hipLaunchKernelGGL((float4_quantize_kernel<T, kRows>), grid, dim3(256), 0, stream, q);
+  else if (rounding == kTiles)
+    hipLaunchKernelGGL((float4_quantize_kernel<T, kTiles>), grid, dim3(256), 0, stream, q);
+  else
+    hipLaunchKernelGGL((float4_quantize_kernel<T, kStochastic>), grid, dim3(256), 0, stream, q);
+  return check_launch("float4_quantize");
+}
+
+bool good_elem(int32_t e) { return e == kF16 || e == kBF16 || e == kF32; }
+
+// Checks a quantization; `tiles`: its workgroups, 0 where there is nothing to do.
+int prepare(const Quantization4& j, QuantizeArgs& q, int64_t& tiles) {
+  tiles = 0;
+  DIONW_REQUIRE(good_elem(j.elem), "float4_quantize: bad element type %d", j.elem);
+  DIONW_REQUIRE(j.rows >= 0 && j.cols >= 0, "float4_quantize: negative extent");
+  if (j.rows == 0 || j.cols == 0) return kOk;
+  DIONW_REQUIRE(j.by_row.data || j.by_col.data || j.sums, "float4_quantize: no output");
+  DIONW_REQUIRE(j.x && j.ld >= j.cols, "float4_quantize: bad input");
+  auto fits = [](const Matrix4& o, int64_t r, int64_t c) {
+    return !o.data || (o.depth == round_up(c, kDepth4) && aligned16(o.data) && o.scale && o.scale_ld >= r &&
+                       o.scale_ld % 16 == 0 && aligned16(o.scale));
+  };
+  DIONW_REQUIRE(fits(j.by_row, j.rows, j.cols) && fits(j.by_col, j.cols, j.rows),
+                "float4_quantize: an output is too small or not aligned");
+  const int64_t tr = (j.by_col.data ? j.by_col.depth : round_up(j.rows, 128)) / 128;
+  const int64_t tc = (j.by_row.data ? j.by_row.depth : round_up(j.cols, 128)) / 128;
+  DIONW_REQUIRE(tr <= kMostGroups / tc, "float4_quantize: too many tiles");
+  auto output = [](const Matrix4& o) {
+    return Output{static_cast<uint8_t*>(o.data), o.depth / 2, static_cast<uint8_t*>(o.scale), o.scale_ld};
+  };
+  q = {};
+  q.x = j.x;
+  q.rows = j.rows;
+  q.cols = j.cols;
+  q.ld = j.ld;
+  q.by_row = output(j.by_row);
+  q.by_col = output(j.by_col);
+  q.sums = j.sums;
+  q.tiles_c = (int32_t)tc;
+  q.far = tr * 128 > (int64_t{1} << 32) / (tc * 64);
+  tiles = tr * tc;
+  return kOk;
+}
+
+template <typename TX>
+int launch_pair(const QuantizeArgs& x, int64_t x_tiles, int32_t w_elem, const QuantizeArgs& w,
+                int64_t w_tiles, hipStream_t stream) {
+  const dim3 grid((unsigned)(x_tiles + w_tiles));
+  auto launch = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, x, w, (uint32_t)x_tiles);
+  };
+  if (w_elem == kF16) launch(float4_quantize_pair_kernel<TX, _Float16>);
+  else if (w_elem == kBF16) launch(float4_quantize_pair_kernel<TX, __bf16>);
+  else launch(float4_quantize_pair_kernel<TX, float>);
+  return check_launch("float4_quantize_pair");
+}
+
+}  // namespace
+
+int quantize4(const Quantization4& x, bool tiles, const Noise* noise, hipStream_t stream) {
+  QuantizeArgs q{};
+  int64_t count;
+  DIONW_REQUIRE(!(tiles && noise), "float4_quantize: tiles are rounded to nearest");
+  DIONW_TRY(prepare(x, q, count));
+  if (count == 0) return kOk;
+  if (noise) q.noise = *noise;
+  const int rounding = noise ? kStochastic : tiles ? kTiles : kRows;
+  if (x.elem == kF16) return launch_quantize<_Float16>(q, rounding, count, stream);
+  if (x.elem == kBF16) return launch_quantize<__bf16>(q, rounding, count, stream);
+  return launch_quantize<float>(q, rounding, count, stream);
+}
+
+int quantize4_pair(const Quantization4& x, const Quantization4& w, hipStream_t stream) {
+  QuantizeArgs qx{}, qw{};
+  int64_t x_tiles, w_tiles;
+  DIONW_TRY(prepare(x, qx, x_tiles));
+  DIONW_TRY(prepare(w, qw, w_tiles));
+  if (x_tiles + w_tiles == 0) return kOk;
+  DIONW_REQUIRE(x_tiles + w_tiles <= kMostGroups, "float4_quantize: too many tiles");
+  if (x.elem == kF16) return launch_pair<_Float16>(qx, x_tiles, w.elem, qw, w_tiles, stream);
+  if (x.elem == kBF16) return launch_pair<__bf16>(qx, x_tiles, w.elem, qw, w_tiles, stream);
+  return launch_pair<float>(qx, x_tiles, w.elem, qw, w_tiles, stream);
+}
+
+}  // namespace dionw
+
+using namespace dionw;
+
+extern "C" {
+
+int dionw_float4_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
+                          int32_t rounding, int64_t seed, const int64_t* seed_at, void* data,
+                          void* scale, int64_t scale_ld, void* data_t, void* scale_t,
+                          int64_t scale_t_ld, hipStream_t stream) {
+  DIONW_REQUIRE(rounding >= kRows && rounding <= kStochastic, "float4_quantize: bad rounding %d", rounding);
+  const Noise noise{seed, seed_at};
+  return quantize4({elem, x, rows, cols, ld,
+                    {data, scale, rows, round_up(cols, kDepth4), scale_ld},
+                    {data_t, scale_t, cols, round_up(rows, kDepth4), scale_t_ld}, nullptr},
+                   rounding == kTiles, rounding == kStochastic ? &noise : nullptr, stream);
+}
+
+int dionw_float4_values(const void* data, const void* scale, int64_t scale_ld, int64_t rows,
+                        int64_t cols, float* out, hipStream_t stream) {
+  DIONW_REQUIRE(rows >= 0 && cols >= 0, "float4_values: negative extent");
+  if (rows == 0 || cols == 0) return kOk;
+  DIONW_REQUIRE(data && scale && out && aligned16(data) && scale_ld >= rows,
+                "float4_values: a matrix is too small or not aligned");
+  const int64_t depth = round_up(cols, kDepth4), stages = depth / kDepth4;
+  DIONW_REQUIRE(ceil_div(rows, 32) <= kMostGroups / stages, "float4_values: too many elements");
+  const ValuesArgs g{static_cast<const uint8_t*>(data), static_cast<const uint8_t*>(scale), scale_ld, rows,
+                     cols, depth, out, (int32_t)stages};
+  hipLaunchKernelGGL(float4_values_kernel, dim3((unsigned)(ceil_div(rows, 32) * stages)), dim3(256), 0, stream, g);
+  return check_launch("float4_values");
+}
+
+}  // extern "C"

@@ -1,0 +1,368 @@
+// The linear layer on 4-bit operands: its passes in order, with their scratch laid out here, and
+// the product of a few rows with a kept weight.
+#include "float4.h"
+
+namespace dionw {
+namespace {
+
+// ---- a few rows ----------------------------------------------------------------------
+//
+// y = x W^T + b for 16 rows of x at a time (the tokens being decoded): every byte of W passes
+// once, from memory to registers, and x is quantized on the way, so that the call is one launch.
+// A workgroup takes 16 R rows of W; its waves take the stages of 256 columns in turn and add their
+// sums through LDS, in a fixed order. Of a stage, a lane holds one token's (or weight row's) two
+// blocks of 32, number G = lane / 16 and 4 + G: a block's scale and codes are its lane's own, without
+// an exchange. A wave reads the next stage while it multiplies one.
+// Bound: HBM, n k / 2 bytes of W; the smallest calls: launch and the latency of two dependent reads.
+constexpr int kFew = 16;
+bool few_rows(int64_t m, int64_t k) { return k > 0 && m <= kFew; }
+
+struct FewArgs {
+  const void* x;
+  int64_t x_ld;
+  const uint8_t* w;
+  const uint8_t* w_scale;
+  int64_t w_scale_ld;
+  const float* bias;
+  void* y;
+  int64_t k;
+  int32_t m, n, stages;
+};
+
+// A token's block of 32 as it lies in memory, and its codes.
+template <typename T>
+struct Values {
+  static constexpr int kWords = 8 * sizeof(T);
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* at) {
+#pragma unroll
+    for (int v = 0; v < kWords / 4; ++v) {
+      const u32x4 r = *reinterpret_cast<const u32x4_any*>(at + 16 / sizeof(T) * v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * v + e] = r[e];
+    }
+  }
+  // Zeros from the `left`th value on.
+  __device__ __forceinline__ void load(const T* at, int64_t left) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) w[e] = e < left ? __float_as_uint(at[e]) : 0u;
+    } else {
+      const uint16_t* u = reinterpret_cast<const uint16_t*>(at);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t lo = 2 * e < left ? u[2 * e] : 0, hi = 2 * e + 1 < left ? u[2 * e + 1] : 0;
+        w[e] = lo | hi << 16;
+      }
+    }
+  }
+  // The float32 bits of the largest magnitude.
+  __device__ __forceinline__ uint32_t most() const {
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+      return m;
+    } else {
+      using P = Pair<T>;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) m = P::larger(m, w[i] & 0x7FFF7FFFu);
+      return P::bits(max(m & 0xFFFFu, m >> 16));
+    }
+  }
+  template <int B>
+  __device__ __forceinline__ uint32_t pair(uint32_t old, int i, float scale) const {
+    if constexpr (sizeof(T) == 4)
+      return codes2<B>(old, __uint_as_float(w[8 * i + 2 * B]), __uint_as_float(w[8 * i + 2 * B + 1]), scale);
+    else
+      return codes2<B>(old, w[4 * i + B], scale, T{});
+  }
+  __device__ __forceinline__ i32x4 codes(float scale) const {
+    i32x4 c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c[i] = (int)pair<3>(pair<2>(pair<1>(pair<0>(0, i, scale), i, scale), i, scale), i, scale);
+    return c;
+  }
+};
+
+__device__ __forceinline__ f32x4 multiply4(i32x4 b, i32x4 a, f32x4 c, uint32_t b_scale, uint32_t a_scale) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1),
+      __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4, 0, (int)b_scale, 0, (int)a_scale);
+}
+
+template <typename T, int R, int W, bool WHOLE>
+__global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
+  __shared__ f32x4 sums[W][R][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int G = lane >> 4, i16 = lane & 15;
+  const int n0 = blockIdx.x * 16 * R, token = blockIdx.y * 16 + i16;
+  const T* x = reinterpret_cast<const T*>(g.x) + min(token, g.m - 1) * g.x_ld + kBlock4 * G;
+  const uint8_t* w[R];
+  int row[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    row[r] = min(n0 + 16 * r + i16, g.n - 1);
+    w[r] = g.w + (int64_t)row[r] * g.stages * 128 + 16 * G;
+  }
+  struct Stage {
+    Values<T> x[2];
+    i32x4 w[R][2];
+    uint32_t byte[R][2];
+  };
+  auto read = [&](Stage& s, int kt) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s.w[r][h] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w[r] + (int64_t)kt * 128 + 64 * h));
+        s.byte[r][h] = g.w_scale[((int64_t)kt * 8 + 4 * h + G) * g.w_scale_ld + row[r]];
+      }
+    const int64_t at = (int64_t)kt * kDepth4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t left = g.k - at - 128 * h - kBlock4 * G;  // columns from the block's first one on
+      if (WHOLE || left >= kBlock4) s.x[h].load(x + at + 128 * h);
+      else s.x[h].load(x + at + 128 * h, left);
+    }
+  };
+  f32x4 acc[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
+  auto multiply = [&](Stage& s) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t byte = scale_byte4<false>(s.x[h].most());
+      const i32x4 c = s.x[h].codes(power(byte));
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[r] = multiply4(s.w[r][h], c, acc[r], s.byte[r][h], byte);
+    }
+  };
+  Stage a, b;
+  int kt = wave;
+  if (kt < g.stages) read(a, kt);
+  for (; kt < g.stages; kt += 2 * W) {
+    if (kt + W < g.stages) read(b, kt + W);
+    multiply(a);
+    if (kt + W >= g.stages) break;
+    if (kt + 2 * W < g.stages) read(a, kt + 2 * W);
+    multiply(b);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) sums[wave][r][lane] = acc[r];
+  __syncthreads();
+  for (int t = wave; t < R; t += W) {  // a fragment a wave: lane: token i16, rows 4 G .. + 3 of W
+    f32x4 s = sums[0][t][lane];
+#pragma unroll
+    for (int v = 1; v < W; ++v) s += sums[v][t][lane];
+    const int n = n0 + 16 * t + 4 * G;
+    if (token >= g.m || n >= g.n) continue;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef T t4any __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    t4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)(s[e] + (g.bias ? g.bias[min(n + e, g.n - 1)] : 0.f));
+    T* y = reinterpret_cast<T*>(g.y) + (int64_t)token * g.n + n;
+    if (n + 4 <= g.n) {
+      *reinterpret_cast<t4any*>(y) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < g.n) y[e] = o[e];
+    }
+  }
+}
+
+// R rows' fragments a wave and W waves a workgroup.
+template <typename T, bool WHOLE>
+int launch_few(const FewArgs& g, hipStream_t stream) {
+  const int fragments = (g.n + 15) / 16;
+  const unsigned groups = (unsigned)(g.m + 15) / 16;
+  const int64_t all = (int64_t)fragments * groups;
+  if (all < 320)
+    hipLaunchKernelGGL((float4_few_kernel<T, 1, 8, WHOLE>), dim3(fragments, groups), dim3(512), 0, stream, g);
+  else
+    hipLaunchKernelGGL((float4_few_kernel<T, 4, 4, WHOLE>), dim3((fragments + 3) / 4, groups), dim3(256), 0, stream, g);
+  return check_launch("float4_few");
+}
+
+// WHOLE: the depth is a multiple of 256, so that no block needs its columns counted.
+template <typename T>
+int launch_few(const FewArgs& g, hipStream_t stream) {
+  return g.k % kDepth4 ? launch_few<T, false>(g, stream) : launch_few<T, true>(g, stream);
+}
+
+// ---- scratch ---------------------------------------------------------------------------
+
+// Hands out parts of a buffer (of nothing, where only sizes are asked for).
+struct Parts {
+  uint8_t* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* at = base ? base + used : nullptr;
+    used += round_up((int64_t)bytes, 256);
+    return at;
+  }
+};
+
+Matrix4 codes_in(Parts& p, int64_t rows, int64_t cols) {
+  Matrix4 q{nullptr, nullptr, rows, round_up(cols, kDepth4), round_up(rows, 16)};
+  q.data = p.take((size_t)(rows * q.depth / 2));
+  q.scale = p.take((size_t)(q.depth / kBlock4 * q.scale_ld));
+  return q;
+}
+
+struct Saved {
+  Matrix4 wt{}, xt{};
+  Saved(Parts& p, int64_t m, int64_t n, int64_t k, bool need_x, bool need_w) {
+    if (need_x) wt = codes_in(p, k, n);
+    if (need_w) xt = codes_in(p, k, m);
+  }
+};
+
+struct Forward {
+  Matrix4 x, w;
+  size_t product_bytes;
+  void* product;
+  Forward(Parts& p, int64_t m, int64_t n, int64_t k) {
+    x = codes_in(p, m, k);
+    w = codes_in(p, n, k);
+    product_bytes = dionw_float4_gemm_workspace(m, n, x.depth);
+    product = p.take(product_bytes);
+  }
+};
+
+struct Backward {
+  Matrix4 rows{}, cols{};  // dy by rows and columns
+  float* sums = nullptr;
+  size_t product_bytes = 0;
+  void* product;
+  Backward(Parts& p, int64_t m, int64_t n, int64_t k, bool need_x, bool need_w, bool need_b) {
+    if (need_x) {
+      rows = codes_in(p, m, n);
+      product_bytes = dionw_float4_gemm_workspace(m, k, rows.depth);
+    }
+    if (need_w) {
+      cols = codes_in(p, n, m);
+      const size_t bytes = dionw_float4_gemm_workspace(n, k, cols.depth);
+      if (bytes > product_bytes) product_bytes = bytes;
+    }
+    if (need_b) sums = static_cast<float*>(p.take((size_t)(ceil_div(m, 128) * n) * 4));
+    product = p.take(product_bytes);
+  }
+};
+
+int product(const Matrix4& a, const Matrix4& b, const float* bias, int32_t elem, void* c, void* space,
+            size_t bytes, hipStream_t stream) {
+  return dionw_float4_gemm(a.rows, b.rows, a.depth, a.data, a.scale, a.scale_ld, b.data, b.scale, b.scale_ld,
+                           bias, elem, c, b.rows, space, bytes, stream);
+}
+
+// Whether rows of that many columns are ones that the products take.
+bool fits_row(int64_t cols) { return cols < 2 * kRowBytes - kDepth4; }
+
+bool good_elem(int32_t e) { return e == kF16 || e == kBF16 || e == kF32; }
+
+}  // namespace
+}  // namespace dionw
+
+using namespace dionw;
+
+extern "C" {
+
+void dionw_float4_linear_sizes(int64_t m, int64_t n, int64_t k, int32_t need_x, int32_t need_w,
+                               int32_t need_b, size_t* sizes) {
+  Parts saved{nullptr}, forward{nullptr}, backward{nullptr};
+  Saved s(saved, m, n, k, need_x, need_w);
+  Forward f(forward, m, n, k);
+  Backward b(backward, m, n, k, need_x, need_w, need_b);
+  sizes[0] = saved.used;
+  sizes[1] = forward.used;
+  sizes[2] = backward.used;
+}
+
+int dionw_float4_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int32_t w_elem,
+                                const void* w, int64_t w_ld, const float* bias, int64_t m,
+                                int64_t n, int64_t k, int32_t need_x, int32_t need_w, void* y,
+                                void* saved, void* scratch, size_t scratch_bytes,
+                                hipStream_t stream) {
+  DIONW_REQUIRE(good_elem(x_elem) && good_elem(w_elem), "float4_linear: bad element type");
+  DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0, "float4_linear: negative extent");
+  DIONW_REQUIRE(saved || !(need_x || need_w) || n == 0 || k == 0, "float4_linear: no room to save");
+  // The gradients sum over n and m: refused here rather than after the forward pass.
+  DIONW_REQUIRE(fits_row(k) && (!need_x || fits_row(n)) && (!need_w || fits_row(m)),
+                "float4_linear: the products take rows of less than 8 MB");
+  DIONW_REQUIRE(aligned16(saved) && aligned16(scratch), "float4_linear: buffers need 16-byte alignment");
+  Parts kept{static_cast<uint8_t*>(saved)}, room{static_cast<uint8_t*>(scratch)};
+  Saved s(kept, m, n, k, need_x, need_w);
+  Forward f(room, m, n, k);
+  DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float4_linear: scratch too small");
+  DIONW_TRY(quantize4_pair({x_elem, x, m, k, x_ld, f.x, s.xt, nullptr},
+                           {w_elem, w, n, k, w_ld, f.w, s.wt, nullptr}, stream));
+  return product(f.x, f.w, bias, x_elem, y, f.product, f.product_bytes, stream);
+}
+
+int dionw_float4_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, int32_t w_elem,
+                                 int64_t m, int64_t n, int64_t k, int32_t need_x, int32_t need_w,
+                                 int64_t seed, const int64_t* seed_at, const void* saved, void* dx,
+                                 void* dw, int32_t bias_elem, void* db, void* scratch,
+                                 size_t scratch_bytes, hipStream_t stream) {
+  DIONW_REQUIRE(good_elem(x_elem) && good_elem(w_elem), "float4_linear: bad element type");
+  DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0, "float4_linear: negative extent");
+  DIONW_REQUIRE(aligned16(saved) && aligned16(scratch), "float4_linear: buffers need 16-byte alignment");
+  Parts kept{static_cast<uint8_t*>(const_cast<void*>(saved))}, room{static_cast<uint8_t*>(scratch)};
+  Saved s(kept, m, n, k, need_x, need_w);
+  Backward b(room, m, n, k, need_x, need_w, db != nullptr);
+  DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float4_linear: scratch too small");
+  DIONW_REQUIRE(saved || kept.used == 0, "float4_linear: nothing was saved");
+  const Noise noise{seed, seed_at};
+  if (need_x || need_w || db)
+    DIONW_TRY(quantize4({x_elem, dy, m, n, dy_ld, b.rows, b.cols, b.sums}, false, &noise, stream));
+  if (need_x)
+    DIONW_TRY(product(b.rows, s.wt, nullptr, x_elem, dx, b.product, b.product_bytes, stream));
+  if (need_w)
+    DIONW_TRY(product(b.cols, s.xt, nullptr, w_elem, dw, b.product, b.product_bytes, stream));
+  return db ? dionw_sum_parts(b.sums, ceil_div(m, 128), n, bias_elem, db, stream) : kOk;
+}
+
+size_t dionw_float4_linear_kept_scratch(int64_t m, int64_t n, int64_t k) {
+  if (few_rows(m, k)) return 0;
+  Parts room{nullptr};
+  const Matrix4 x = codes_in(room, m, k);
+  room.take(dionw_float4_gemm_workspace(m, n, x.depth));
+  return room.used;
+}
+
+int dionw_float4_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const void* w,
+                             const void* w_scale, int64_t w_scale_ld, const float* bias, int64_t m,
+                             int64_t n, int64_t k, void* y, void* scratch, size_t scratch_bytes,
+                             hipStream_t stream) {
+  DIONW_REQUIRE(good_elem(x_elem), "float4_linear: bad element type %d", x_elem);
+  DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0 && n < INT32_MAX / 2, "float4_linear: bad extents");
+  if (m == 0 || n == 0) return kOk;
+  const int64_t depth = round_up(k, kDepth4);
+  DIONW_REQUIRE(y && (k == 0 || (x && w && w_scale)), "float4_linear: null pointer");
+  DIONW_REQUIRE(x_ld >= k && aligned16(w) && w_scale_ld >= n && aligned16(scratch),
+                "float4_linear: an operand is too small or not aligned");
+  if (few_rows(m, k)) {
+    DIONW_REQUIRE(depth / kDepth4 < INT32_MAX / 16, "float4_linear: depth too large");
+    const FewArgs g{x, x_ld, static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(w_scale),
+                    w_scale_ld, bias, y, k, (int32_t)m, (int32_t)n, (int32_t)(depth / kDepth4)};
+    if (x_elem == kF16) return launch_few<_Float16>(g, stream);
+    if (x_elem == kBF16) return launch_few<__bf16>(g, stream);
+    return launch_few<float>(g, stream);
+  }
+  Parts room{static_cast<uint8_t*>(scratch)};
+  const Matrix4 rows = codes_in(room, m, k);
+  const size_t bytes = dionw_float4_gemm_workspace(m, n, depth);
+  void* space = room.take(bytes);
+  DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float4_linear: scratch too small");
+  DIONW_TRY(quantize4({x_elem, x, m, k, x_ld, rows, {}, nullptr}, false, nullptr, stream));
+  const Matrix4 weight{const_cast<void*>(w), const_cast<void*>(w_scale), n, depth, w_scale_ld};
+  return product(rows, weight, bias, x_elem, y, space, bytes, stream);
+}
+
+}  // extern "C"

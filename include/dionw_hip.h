@@ -426,6 +426,96 @@ int dionw_float8_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const 
                              void* scratch, size_t scratch_bytes, dionw_stream_t stream);
 
 /*
+ * 4-bit matrices (not in the reference). A quantized matrix [rows, cols] is e2m1 codes, two a byte
+ * (the first column's in the low half), rows of depth / 2 bytes one behind the other, depth being
+ * cols rounded up to 256 (zeros from cols on), and the exponent bytes of float32 powers of two
+ * [depth / 32][scale_ld], scale_ld >= rows and a multiple of 16; 255 makes a block NaN. Codes and
+ * scales are 16-byte aligned.
+ *
+ * dionw_float4_quantize rounds x [rows, cols] (row pitch ld, element code elem) into data/scale by
+ * rows and into data_t/scale_t as the transpose [cols, rows]; either data may be NULL. rounding 0:
+ * to nearest, one scale for each row (of the transpose: column of x) and block of 32; 1: to
+ * nearest, one for each 32 x 32 tile; 2: as 0, stochastically, with bits from a hash of seed (of
+ * *seed_at in device memory, read by the kernel, where that is not NULL) and the element's place. A
+ * block with a value that is not finite is NaN. dionw_float4_values writes the float32 values,
+ * [rows][cols].
+ */
+int dionw_float4_quantize(int32_t elem, const void* x, int64_t rows, int64_t cols, int64_t ld,
+                          int32_t rounding, int64_t seed, const int64_t* seed_at, void* data,
+                          void* scale, int64_t scale_ld, void* data_t, void* scale_t,
+                          int64_t scale_t_ld, dionw_stream_t stream);
+int dionw_float4_values(const void* data, const void* scale, int64_t scale_ld, int64_t rows,
+                        int64_t cols, float* out, dionw_stream_t stream);
+
+/*
+ * C [m, n] = A B^T + bias for quantized A [m, depth] and B [n, depth] (depth: a multiple of 256, of
+ * less than 16 M), summed in float32 and rounded once to element code elem; bias: n floats or NULL.
+ * workspace: float32 scratch of dionw_float4_gemm_workspace bytes (0: none needed).
+ * dionw_float4_gemm_plan writes what a product of these extents runs on: the side of its tiles (256,
+ * 128 or 64) and in how many ranges its depth is summed (1: whole).
+ */
+int dionw_float4_gemm_plan(int64_t m, int64_t n, int64_t depth, int32_t* side, int32_t* ranges);
+size_t dionw_float4_gemm_workspace(int64_t m, int64_t n, int64_t depth);
+int dionw_float4_gemm(int64_t m, int64_t n, int64_t depth, const void* a, const void* a_scale,
+                      int64_t a_scale_ld, const void* b, const void* b_scale, int64_t b_scale_ld,
+                      const float* bias, int32_t elem, void* c, int64_t ldc, void* workspace,
+                      size_t workspace_bytes, dionw_stream_t stream);
+
+/*
+ * A linear layer on 4-bit operands: y [m, n] = x [m, k] W [n, k]^T + bias in x's element code
+ * (x_elem), from float x and W (pitches in elements). x is quantized by rows, W by tiles. saved
+ * (NULL where both needs are 0) keeps, for the backward, W's transpose (need_x) and x's (need_w) in
+ * codes. The backward gives dx (x_elem) = dy W when need_x, dw (w_elem) = dy^T x when need_w, dy
+ * rounded stochastically by rows and by columns, and db (bias_elem) = the column sums of dy when db
+ * is not NULL. dionw_float4_linear_sizes writes the bytes of saved and of the two calls' scratch.
+ */
+void dionw_float4_linear_sizes(int64_t m, int64_t n, int64_t k, int32_t need_x, int32_t need_w,
+                               int32_t need_b, size_t* sizes);
+int dionw_float4_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int32_t w_elem,
+                                const void* w, int64_t w_ld, const float* bias, int64_t m,
+                                int64_t n, int64_t k, int32_t need_x, int32_t need_w, void* y,
+                                void* saved, void* scratch, size_t scratch_bytes,
+                                dionw_stream_t stream);
+int dionw_float4_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, int32_t w_elem,
+                                 int64_t m, int64_t n, int64_t k, int32_t need_x, int32_t need_w,
+                                 int64_t seed, const int64_t* seed_at, const void* saved, void* dx,
+                                 void* dw, int32_t bias_elem, void* db, void* scratch,
+                                 size_t scratch_bytes, dionw_stream_t stream);
+
+/*
+ * The same y from a kept W: codes [n] rows with their scales [depth / 32][w_scale_ld]. Up to 16 rows
+ * of x are quantized by the product itself, in one launch and no scratch.
+ */
+size_t dionw_float4_linear_kept_scratch(int64_t m, int64_t n, int64_t k);
+int dionw_float4_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const void* w,
+                             const void* w_scale, int64_t w_scale_ld, const float* bias, int64_t m,
+                             int64_t n, int64_t k, void* y, void* scratch, size_t scratch_bytes,
+                             dionw_stream_t stream);
+
+/*
+ * Layer norm of the rows of x [rows, cols] (row pitch x_ld, element code elem): y [rows][cols] in x's
+ * code, (x - mean) / sqrt(variance + eps) * weight + bias, the parameters in codes of their own
+ * (NULL: ones, zeros). mean and rstd (both or neither): float32 [rows], for the backward.
+ * dionw_layer_norm_float4 writes the same y, not rounded to a type of its own first, quantized by rows
+ * to nearest (dionw_float4_quantize).
+ * The backward gives dx (x's code), dg (w_elem) and db (b_elem), each where it is not NULL; dg and db
+ * take scratch of dionw_layer_norm_backward_scratch bytes.
+ */
+int dionw_layer_norm_forward(int32_t elem, const void* x, int64_t x_ld, int64_t rows, int64_t cols,
+                             int32_t w_elem, const void* weight, int32_t b_elem, const void* bias,
+                             float eps, void* y, float* mean, float* rstd, dionw_stream_t stream);
+int dionw_layer_norm_float4(int32_t elem, const void* x, int64_t x_ld, int64_t rows, int64_t cols,
+                            int32_t w_elem, const void* weight, int32_t b_elem, const void* bias,
+                            float eps, void* data, void* scale, int64_t scale_ld,
+                            dionw_stream_t stream);
+size_t dionw_layer_norm_backward_scratch(int64_t rows, int64_t cols);
+int dionw_layer_norm_backward(int32_t elem, const void* x, int64_t x_ld, const void* dy, int64_t dy_ld,
+                              int64_t rows, int64_t cols, int32_t w_elem, const void* weight,
+                              const float* mean, const float* rstd, void* dx, void* dg,
+                              int32_t b_elem, void* db, void* scratch, size_t scratch_bytes,
+                              dionw_stream_t stream);
+
+/*
  * GPU EMA of float32 sources: shadow = lerp(shadow, source, weight), or a
  * copy when copy != 0. Replaces foreach_ema_update_ (ema/_update.py:32-70)
  * and the first-update _foreach_copy_ (ema/tracker.py:142-145).
