@@ -7,13 +7,16 @@ namespace dionw {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kBlock4 = 32;    // columns (and rows) that share a scale
-constexpr int kDepth4 = 256;   // a matrix's rows run to a multiple: 128 bytes, one stage of a product
+constexpr int kBlock4 = 32;   // columns (and rows) that share a scale
+constexpr int kDepth4 = 256;  // a matrix's rows run to a multiple: 128 bytes, one stage of a product
+
+constexpr int kTile4 = 128;   // side of a quantization's tiles; rows that share partial column sums
 
 // A 4-bit matrix: rows of depth / 2 bytes, one behind the other; data null: nothing.
 using Matrix4 = Matrix;
 
-// The random bits of a stochastic rounding: a seed, or where it lies in device memory.
+// The random bits of a stochastic rounding: a seed, or where it lies in device memory. Of a pair of
+// columns' 32 bits the even one's value takes the top 22, the odd one's the low 16.
 struct Noise {
   int64_t seed;
   const int64_t* at;
@@ -56,18 +59,40 @@ __device__ __forceinline__ uint32_t noise_key(const Noise& n) {
   const uint64_t seed = n.at ? (uint64_t)*n.at : (uint64_t)n.seed;
   return mix32((uint32_t)seed + 0x9E3779B1u * ((uint32_t)(seed >> 32) + 1u));
 }
-// 22 bits each for an even column's value and the next one's, from a pair's 32.
-__device__ __forceinline__ uint32_t even_noise(uint32_t h) { return h >> 10; }
-__device__ __forceinline__ uint32_t odd_noise(uint32_t h) { return (h & 0xFFFFu) << 6; }
-
-// x / scale rounded up by `noise` of 2^22, down otherwise, as a value of the format. From 1 on the
-// format keeps one fraction bit of a value, so the noise is added below it and what is below it
-// dropped; 1 is added to smaller values first, whose steps are those of the next binade
-// (which rounds them to a multiple of 2^-23).
-__device__ __forceinline__ float stochastic4(float x, float scale, float inverse, uint32_t noise) {
+// x / scale, below 1 rounded to a multiple of 2^-23: what lies below the last place kept is then a
+// multiple of 2^-22 of it, like the noise.
+__device__ __forceinline__ float scaled4(float x, float scale, float inverse) {
   const float one = __builtin_copysignf(fabsf(x) < scale ? 1.f : 0.f, x);
-  const uint32_t w = __float_as_uint(__builtin_fmaf(x, inverse, one)) + noise;
-  return __uint_as_float(w & 0xFFC00000u) - one;
+  return __builtin_fmaf(x, inverse, one) - one;
+}
+
+// Codes of eight values times 1 / scale, rounded up by chance: `noise` holds each value's bits at the
+// top of a word. The instruction takes two values and adds to the first one's part below the last
+// place kept its third operand / 2^32 of that place, to the second's the same word turned left by
+// one bit, and drops what is left of both; values below 1 lose what is below 2^-23 first (measured
+// bit by bit; its 16-bit forms lose what is below 2^-7 and 2^-10, so float32 serves every type). A pair's
+// bits are 22 and 16 of one word in places of their own, so that each of a pair's codes comes
+// from an instruction of its own: the words' low halves (bits 0..3 of each byte) from `even`, the others from
+// `odd`. In assembly, as the builtin leaves out that the destination's other bytes are kept; a
+// byte's write needs one more instruction before the next one that keeps it, which the two words'
+// turns are.
+__device__ __forceinline__ uint32_t noisy8(const f32x2 (&p)[4], const uint32_t (&noise)[8], float scale) {
+  uint32_t even = 0, odd = 0;
+#ifdef __HIP_DEVICE_COMPILE__
+  asm("v_cvt_scalef32_sr_pk_fp4_f32 %0, %2, %6, %14\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %1, %2, %7, %14\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %0, %3, %8, %14 op_sel:[0,0,1,0]\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %1, %3, %9, %14 op_sel:[0,0,1,0]\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %0, %4, %10, %14 op_sel:[0,0,0,1]\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %1, %4, %11, %14 op_sel:[0,0,0,1]\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %0, %5, %12, %14 op_sel:[0,0,1,1]\n\t"
+      "v_cvt_scalef32_sr_pk_fp4_f32 %1, %5, %13, %14 op_sel:[0,0,1,1]\n\t"
+      "s_nop 0"
+      : "=&v"(even), "=&v"(odd)
+      : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(noise[0]), "v"(noise[1] >> 1), "v"(noise[2]),
+        "v"(noise[3] >> 1), "v"(noise[4]), "v"(noise[5] >> 1), "v"(noise[6]), "v"(noise[7] >> 1), "v"(scale));
+#endif
+  return (even & 0x0F0F0F0Fu) | (odd & 0xF0F0F0F0u);
 }
 
 // Codes of two values times 1 / scale, rounded to nearest (ties to the even code) and cut at 6, in

@@ -42,15 +42,21 @@ struct QuantizeArgs {
 // column of lanes a column's. Codes by rows go from registers to memory, those of the transpose
 // through LDS, each in 64-byte runs; the scales through LDS, so that a block's rows are written
 // together. Tiles past the last row or column, up to the padding of the other form, write zeros.
-// Bound: HBM, 2 or 4 bytes read and half a byte written for each form an element.
+// Bound: HBM, 2 or 4 bytes read and half a byte written for each form an element; by chance, the hash and
+// the conversions too. us (and TB/s) of both forms, bfloat16: 8192 x 14336 77 (4.7), by chance 81; 8192 x
+// 4096 18.0 (5.7), 25; float32 8192 x 14336 133 (4.5), 14336 x 4096 by tiles 50 (5.9). Not kept: tiles
+// of 256 x 128 or 256 x 256, whose runs are twice as long (79 and 81 us for the first, 34 and 42 where
+// 128 x 128 takes 25 by chance), and two rows of tiles in turn on one XCD (79). By chance with the
+// arithmetic of the definition, an integer addition below the place kept, 116.
 enum Rounding : int { kRows = 0, kTiles = 1, kStochastic = 2 };
+
 
 struct Shared {
   // Words of the transpose: 17 a column, so that a wave's writes spread over the banks.
   static constexpr int pitch = 17;
-  uint32_t turned[128 * pitch];
-  float col_sum[4][128];
-  __attribute__((aligned(16))) uint8_t row_bytes[4][128], col_bytes[4][128];
+  uint32_t turned[kTile4 * pitch];
+  float col_sum[4][kTile4];
+  __attribute__((aligned(16))) uint8_t row_bytes[4][kTile4], col_bytes[4][kTile4];
 };
 
 template <typename T>
@@ -77,12 +83,20 @@ struct Codes {
   }
 };
 
-// Codes of 8 values that are the format's already.
-__device__ __forceinline__ uint32_t exact_codes(const float (&v)[8]) {
-  uint32_t c = codes2<0>(0, v[0], v[1], 1.f);
-  c = codes2<1>(c, v[2], v[3], 1.f);
-  c = codes2<2>(c, v[4], v[5], 1.f);
-  return codes2<3>(c, v[6], v[7], 1.f);
+// The same by chance, from each value's bits at the top of a word. 16-bit values need no rounding of
+// their own first: they are multiples of 2^-23 of the scale, but for those below 2^-12 of it, which the
+// noise's last 2^-10 alone could tell apart.
+template <typename T, typename V, typename N>
+__device__ __forceinline__ uint32_t noisy_codes(uint32_t byte, V value, N noise) {
+  const float scale = power(byte), inverse = inverse4(byte);
+  f32x2 p[4];
+  uint32_t bits[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    p[e >> 1][e & 1] = sizeof(T) == 4 ? scaled4(value(e), scale, inverse) : value(e);
+    bits[e] = noise(e);
+  }
+  return noisy8(p, bits, sizeof(T) == 4 ? 1.f : scale);
 }
 
 template <typename T, int ROUNDING>
@@ -90,10 +104,10 @@ __device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t ti
   using S = Square<T>;
   constexpr int RM = S::kRowMost, CM = S::kColMost, kPitch = Shared::pitch;
   constexpr bool TILES = ROUNDING == kTiles, NOISY = ROUNDING == kStochastic;
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int64_t r0 = (int64_t)(tile / q.tiles_c) * 128;
-  const int64_t c0 = (int64_t)(tile % q.tiles_c) * 128;
-  const int tr = tid / 16 * 8, tc = tid % 16 * 8;  // the thread's first row and column
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r0 = (int64_t)(tile / q.tiles_c) * kTile4;
+  const int64_t c0 = (int64_t)(tile % q.tiles_c) * kTile4;
+  const int tr = wave * 32 + lane / 16 * 8, tc = lane % 16 * 8;  // the thread's first row and column
   S v;
   const T* at = reinterpret_cast<const T*>(q.x) + (r0 + tr) * q.ld + c0 + tc;
   if (r0 + tr + 8 <= q.rows && c0 + tc + 8 <= q.cols) {
@@ -140,7 +154,7 @@ __device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t ti
     for (int off = 16; off <= 32; off <<= 1)
 #pragma unroll
       for (int k = 0; k < 8; ++k) s[k] += __shfl_xor(s[k], off, kWave);
-    if ((tid & 63) < 16)
+    if (lane < 16)
 #pragma unroll
       for (int k = 0; k < 8; ++k) shared.col_sum[wave][tc + k] = s[k];
   }
@@ -156,7 +170,8 @@ __device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t ti
         h[i][k] = mix32((uint32_t)(p + k) ^ (q.far ? mix32(key + (uint32_t)((p + k) >> 32)) : near));
     }
   }
-  auto noise = [&](int i, int k) { return k & 1 ? odd_noise(h[i][k >> 1]) : even_noise(h[i][k >> 1]); };
+  // Value (i, k)'s bits, at the top of a word.
+  auto noise = [&](int i, int k) { return k & 1 ? h[i][k >> 1] << 16 : h[i][k >> 1]; };
   if (q.by_row.data) {
     uint8_t* out = q.by_row.data + (r0 + tr) * q.by_row.ld + (c0 + tc) / 2;
 #pragma unroll
@@ -164,16 +179,12 @@ __device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t ti
       const uint32_t byte = TILES ? tile_byte : scale_byte4<NOISY>(S::bits(row, i));
       uint32_t w;
       if constexpr (NOISY) {
-        const float scale = power(byte), inverse = inverse4(byte);
-        float e[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = stochastic4(v.value(i, k), scale, inverse, noise(i, k));
-        w = exact_codes(e);
+        w = noisy_codes<T>(byte, [&](int k) { return v.value(i, k); }, [&](int k) { return noise(i, k); });
       } else {
         w = Codes<T>::row(v, i, power(byte));
       }
       if (r0 + tr + i < q.rows) *reinterpret_cast<uint32_t*>(out) = w;
-      if (tid % 4 == 0) shared.row_bytes[tid % 16 / 4][tr + i] = (uint8_t)byte;
+      if (lane % 4 == 0) shared.row_bytes[tc / 32][tr + i] = (uint8_t)byte;
     }
   }
   if (q.by_col.data) {
@@ -182,29 +193,25 @@ __device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t ti
       const uint32_t byte = TILES ? tile_byte : scale_byte4<NOISY>(S::bits(col, k));
       uint32_t w;
       if constexpr (NOISY) {
-        const float scale = power(byte), inverse = inverse4(byte);
-        float e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = stochastic4(v.value(i, k), scale, inverse, noise(i, k));
-        w = exact_codes(e);
+        w = noisy_codes<T>(byte, [&](int i) { return v.value(i, k); }, [&](int i) { return noise(i, k); });
       } else {
         w = Codes<T>::col(v, k, power(byte));
       }
       shared.turned[(tc + k) * kPitch + tr / 8] = w;
-      if ((tid & 63) < 16) shared.col_bytes[wave][tc + k] = (uint8_t)byte;
+      if (lane < 16) shared.col_bytes[wave][tc + k] = (uint8_t)byte;
     }
   }
   __syncthreads();
-  if (q.sums && tid < 128 && c0 + tid < q.cols)
-    q.sums[r0 / 128 * q.cols + c0 + tid] = (shared.col_sum[0][tid] + shared.col_sum[1][tid]) +
-                                           (shared.col_sum[2][tid] + shared.col_sum[3][tid]);
+  if (q.sums && tid < kTile4 && c0 + tid < q.cols)
+    q.sums[r0 / kTile4 * q.cols + c0 + tid] = (shared.col_sum[0][tid] + shared.col_sum[1][tid]) +
+                                              (shared.col_sum[2][tid] + shared.col_sum[3][tid]);
   // A block's bytes run to a multiple of 16: 4 of them a thread, the first 128 threads the rows'.
-  const int b = tid / 32 % 4, place = tid % 32 * 4;
+  const int block = tid / 32 % 4, place = tid % 32 * 4;
   const Output& o = tid < 128 ? q.by_row : q.by_col;
   const int64_t first = tid < 128 ? r0 : c0, other = tid < 128 ? c0 : r0;
   if (o.data && first + place < o.scale_ld)
-    *reinterpret_cast<uint32_t*>(o.scale + (other / kBlock4 + b) * o.scale_ld + first + place) =
-        *reinterpret_cast<const uint32_t*>((tid < 128 ? shared.row_bytes[b] : shared.col_bytes[b]) + place);
+    *reinterpret_cast<uint32_t*>(o.scale + (other / kBlock4 + block) * o.scale_ld + first + place) =
+        *reinterpret_cast<const uint32_t*>((tid < 128 ? shared.row_bytes[block] : shared.col_bytes[block]) + place);
   if (!q.by_col.data) return;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -239,6 +246,7 @@ __global__ __launch_bounds__(256) void float4_quantize_pair_kernel(QuantizeArgs 
 //
 // A workgroup takes 8 R rows of 256 columns, 32 lanes a row, 8 columns a lane: nothing goes through
 // LDS but the scales. Few rows take R = 1, so that they still fill the GPU.
+// Bound: HBM. bfloat16 8192 x 14336 44 us (6.7 TB/s), 8192 x 4096 13.8; float32 8192 x 14336 96 (5.5).
 template <typename T, int R>
 __global__ __launch_bounds__(256) void float4_quantize_rows_kernel(QuantizeArgs q) {
   __shared__ __attribute__((aligned(16))) uint8_t bytes[8][8 * R];
@@ -275,9 +283,11 @@ __global__ __launch_bounds__(256) void float4_quantize_rows_kernel(QuantizeArgs 
 
 // ---- reading back ------------------------------------------------------------------------
 //
-// The float32 values: a workgroup takes 32 rows of 256 columns, 8 columns of 4 rows a lane; the
-// scales come through LDS, as a lane's rows lie together there.
-// Bound: HBM, half a byte read and 4 written an element.
+// The float32 values: a workgroup takes 32 rows of 256 columns, a wave 8 rows, 4 columns a lane, so
+// that a wave's store is one run of 1 KB; the scales come through LDS, as a lane's rows lie together
+// there.
+// Bound: HBM, half a byte read and 4 written an element. 8192 x 14336 76 us (7.0 TB/s), with 8 columns a
+// lane in two stores of 16 bytes 115 to 135.
 struct ValuesArgs {
   const uint8_t* data;
   const uint8_t* scale;
@@ -287,37 +297,35 @@ struct ValuesArgs {
 };
 __global__ __launch_bounds__(256) void float4_values_kernel(ValuesArgs g) {
   __shared__ uint8_t bytes[8][32];
-  const int tid = threadIdx.x, lane = tid & 31, y = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r0 = (int64_t)(blockIdx.x / g.stages) * 32, stage = blockIdx.x % g.stages;
-  const int64_t c = stage * kDepth4 + 8 * lane;
-  bytes[y][lane] = r0 + lane < g.rows ? g.scale[(stage * 8 + y) * g.scale_ld + r0 + lane] : 0;
-  uint32_t w[4];
+  const int64_t c = stage * kDepth4 + 4 * lane;
+  uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = min(r0 + 8 * i + y, g.rows - 1);
-    w[i] = *reinterpret_cast<const uint32_t*>(g.data + row * (g.depth / 2) + c / 2);
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = min(r0 + 8 * wave + i, g.rows - 1);
+    w[i] = *reinterpret_cast<const uint16_t*>(g.data + row * (g.depth / 2) + c / 2);
   }
+  bytes[tid >> 5][tid & 31] =
+      r0 + (tid & 31) < g.rows ? g.scale[(stage * 8 + (tid >> 5)) * g.scale_ld + r0 + (tid & 31)] : 0;
   __syncthreads();
+  if (c >= g.cols) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = r0 + 8 * i + y;
-    if (row >= g.rows || c >= g.cols) continue;
-    const uint32_t byte = bytes[lane / 4][8 * i + y];
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = r0 + 8 * wave + i;
+    if (row >= g.rows) return;
+    const uint32_t byte = bytes[lane / 8][8 * wave + i];
     const float scale = byte == 255 ? __uint_as_float(0x7FC00000u) : power(byte);
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 0);
     const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 1);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 2);
-    const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 3);
-    const float v[8] = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale,
-                        d[0] * scale, d[1] * scale, e[0] * scale, e[1] * scale};
+    const f32x4 v = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
     float* to = g.out + row * g.cols + c;
-    if (c + 8 <= g.cols) {
+    if (c + 4 <= g.cols) {
       typedef float f4any __attribute__((ext_vector_type(4), aligned(4)));
-      *reinterpret_cast<f4any*>(to) = f4any{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f4any*>(to + 4) = f4any{v[4], v[5], v[6], v[7]};
+      __builtin_nontemporal_store(v, reinterpret_cast<f4any*>(to));
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 4; ++k)
         if (c + k < g.cols) to[k] = v[k];
     }
   }
@@ -368,8 +376,8 @@ int prepare(const Quantization4& j, QuantizeArgs& q, int64_t& tiles) {
   };
   DIONW_REQUIRE(fits(j.by_row, j.rows, j.cols) && fits(j.by_col, j.cols, j.rows),
                 "float4_quantize: an output is too small or not aligned");
-  const int64_t tr = (j.by_col.data ? j.by_col.depth : round_up(j.rows, 128)) / 128;
-  const int64_t tc = (j.by_row.data ? j.by_row.depth : round_up(j.cols, 128)) / 128;
+  const int64_t tr = ceil_div(j.by_col.data ? j.by_col.depth : j.rows, kTile4);
+  const int64_t tc = ceil_div(j.by_row.data ? j.by_row.depth : j.cols, kTile4);
   DIONW_REQUIRE(tr <= kMostGroups / tc, "float4_quantize: too many tiles");
   auto output = [](const Matrix4& o) {
     return Output{static_cast<uint8_t*>(o.data), o.depth / 2, static_cast<uint8_t*>(o.scale), o.scale_ld};
@@ -383,7 +391,7 @@ int prepare(const Quantization4& j, QuantizeArgs& q, int64_t& tiles) {
   q.by_col = output(j.by_col);
   q.sums = j.sums;
   q.tiles_c = (int32_t)tc;
-  q.far = tr * 128 > (int64_t{1} << 32) / (tc * 64);
+  q.far = tr * kTile4 > (int64_t{1} << 32) / (tc * kTile4 / 2);
   tiles = tr * tc;
   return kOk;
 }

@@ -14,7 +14,7 @@ extern "C" {
 int dionw_float4_gemm_plan(int64_t m, int64_t n, int64_t depth, int32_t* side, int32_t* ranges) {
   DIONW_REQUIRE(m > 0 && n > 0 && depth > 0 && depth % kDepth4 == 0 && side && ranges,
                 "float4_gemm_plan: bad arguments");
-  const Plan p = plan(m, n, depth / kDepth4);
+  const Plan p = plan(kCost4, m, n, depth / kDepth4);
   *side = kSide[p.tile];
   *ranges = p.splits;
   return kOk;
@@ -22,7 +22,7 @@ int dionw_float4_gemm_plan(int64_t m, int64_t n, int64_t depth, int32_t* side, i
 
 size_t dionw_float4_gemm_workspace(int64_t m, int64_t n, int64_t depth) {
   if (m <= 0 || n <= 0 || depth <= 0 || depth % kDepth4) return 0;
-  const Plan p = plan(m, n, depth / kDepth4);
+  const Plan p = plan(kCost4, m, n, depth / kDepth4);
   return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
 }
 
@@ -47,7 +47,7 @@ int dionw_float4_gemm(int64_t m, int64_t n, int64_t depth, const void* a, const 
                 "16, at multiples of 16 bytes");
   DIONW_REQUIRE(std::max(a_scale_ld, b_scale_ld) <= UINT32_MAX / std::max<int64_t>(depth / kBlock4, 1),
                 "float4_gemm: a matrix's scales need to lie within 4 GB");
-  const Plan p = depth ? plan(m, n, depth / kDepth4) : Plan{kSmall, 1, 1};
+  const Plan p = depth ? plan(kCost4, m, n, depth / kDepth4) : Plan{kSmall, 1, 1};
   DIONW_REQUIRE(p.splits == 1 || (workspace && workspace_bytes >= (size_t)p.splits * m * n * sizeof(float) &&
                                   (reinterpret_cast<uintptr_t>(workspace) & 3) == 0),
                 "float4_gemm: workspace too small");

@@ -250,7 +250,7 @@ struct Backward {
       const size_t bytes = dionw_float4_gemm_workspace(n, k, cols.depth);
       if (bytes > product_bytes) product_bytes = bytes;
     }
-    if (need_b) sums = static_cast<float*>(p.take((size_t)(ceil_div(m, 128) * n) * 4));
+    if (need_b) sums = static_cast<float*>(p.take((size_t)(ceil_div(m, kTile4) * n) * 4));
     product = p.take(product_bytes);
   }
 };
@@ -325,7 +325,7 @@ int dionw_float4_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
     DIONW_TRY(product(b.rows, s.wt, nullptr, x_elem, dx, b.product, b.product_bytes, stream));
   if (need_w)
     DIONW_TRY(product(b.cols, s.xt, nullptr, w_elem, dw, b.product, b.product_bytes, stream));
-  return db ? dionw_sum_parts(b.sums, ceil_div(m, 128), n, bias_elem, db, stream) : kOk;
+  return db ? dionw_sum_parts(b.sums, ceil_div(m, kTile4), n, bias_elem, db, stream) : kOk;
 }
 
 size_t dionw_float4_linear_kept_scratch(int64_t m, int64_t n, int64_t k) {

@@ -22,7 +22,7 @@ int dionw_float8_gemm_plan(int32_t expanded, int64_t m, int64_t n, int64_t depth
                            int32_t* ranges) {
   DIONW_REQUIRE(m > 0 && n > 0 && depth > 0 && depth % kTile == 0 && side && ranges,
                 "float8_gemm_plan: bad arguments");
-  const Plan p = plan(m, n, depth / kTile * (expanded ? 2 : 1));
+  const Plan p = plan(kCost8, m, n, depth / kTile * (expanded ? 2 : 1));
   *side = kSide[p.tile];
   *ranges = p.splits;
   return kOk;
@@ -30,7 +30,7 @@ int dionw_float8_gemm_plan(int32_t expanded, int64_t m, int64_t n, int64_t depth
 
 size_t dionw_float8_gemm_workspace(int32_t expanded, int64_t m, int64_t n, int64_t depth) {
   if (m <= 0 || n <= 0 || depth <= 0 || depth % kTile) return 0;
-  const Plan p = plan(m, n, depth / kTile * (expanded ? 2 : 1));
+  const Plan p = plan(kCost8, m, n, depth / kTile * (expanded ? 2 : 1));
   return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
 }
 
@@ -61,7 +61,7 @@ int dionw_float8_gemm(int32_t expanded, int64_t m, int64_t n, int64_t depth, con
                 "float8_gemm: codes need a scale for each row, at a pitch that is a multiple of 16");
   DIONW_REQUIRE(expanded || std::max(a_scale_ld, b_scale_ld) <= UINT32_MAX / std::max<int64_t>(row / 128, 1),
                 "float8_gemm: a matrix's scales need to lie within 4 GB");
-  const Plan p = depth ? plan(m, n, row / 128) : Plan{kSmall, 1, 1};
+  const Plan p = depth ? plan(kCost8, m, n, row / 128) : Plan{kSmall, 1, 1};
   DIONW_REQUIRE(p.splits == 1 ||
                     (workspace && workspace_bytes >= (size_t)p.splits * m * n * sizeof(float) &&
                      (reinterpret_cast<uintptr_t>(workspace) & 3) == 0),

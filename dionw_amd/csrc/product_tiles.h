@@ -94,26 +94,44 @@ __device__ __forceinline__ void tile_place(const ProductArgs& g, int t, int& tm,
   tn = (t % group) / gm;
 }
 
-// c += b a^T of a fragment pair; OA, OB: the scales' bytes.
-template <Form FORM, int OA, int OB>
-__device__ __forceinline__ void multiply(i32x8 b, i32x8 a, f32x4& c, const int (&b_scale)[kWords<FORM>],
-                                         const int (&a_scale)[kWords<FORM>]) {
+// One instruction's part of c += b a^T of a fragment pair (4 bits and bfloat16 take two); OA, OB: the
+// scales' bytes.
+template <Form FORM, int OA, int OB, int P>
+__device__ __forceinline__ void multiply_part(i32x8 b, i32x8 a, f32x4& c, const int (&b_scale)[kWords<FORM>],
+                                              const int (&a_scale)[kWords<FORM>]) {
+  constexpr int W = 4 * P;  // the part's first word of a lane's 8
   if constexpr (FORM == Form::kCodes8) {
     c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, OB, b_scale[0], OA, a_scale[0]);
   } else if constexpr (FORM == Form::kCodes4) {  // the instruction reads 16 bytes of a 4-bit operand
     c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-        __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1),
-        __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4, OB, b_scale[0], OA, a_scale[0]);
-    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-        __builtin_shufflevector(b, b, 4, 5, 6, 7, -1, -1, -1, -1),
-        __builtin_shufflevector(a, a, 4, 5, 6, 7, -1, -1, -1, -1), c, 4, 4, OB, b_scale[1], OA, a_scale[1]);
+        __builtin_shufflevector(b, b, W, W + 1, W + 2, W + 3, -1, -1, -1, -1),
+        __builtin_shufflevector(a, a, W, W + 1, W + 2, W + 3, -1, -1, -1, -1), c, 4, 4, OB, b_scale[P], OA,
+        a_scale[P]);
   } else {
     c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-        __builtin_bit_cast(bf16x8, __builtin_shufflevector(b, b, 0, 1, 2, 3)),
-        __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, a, 0, 1, 2, 3)), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-        __builtin_bit_cast(bf16x8, __builtin_shufflevector(b, b, 4, 5, 6, 7)),
-        __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, a, 4, 5, 6, 7)), c, 0, 0, 0);
+        __builtin_bit_cast(bf16x8, __builtin_shufflevector(b, b, W, W + 1, W + 2, W + 3)),
+        __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, a, W, W + 1, W + 2, W + 3)), c, 0, 0, 0);
+  }
+}
+
+// c0, c1 += b0 a^T, b1 a^T; the scales of b0 and b1 are bytes 0 and 1. 4 bits: the sums take turns, so
+// that no instruction waits for the one before it.
+template <Form FORM, int OA>
+__device__ __forceinline__ void multiply(i32x8 b0, i32x8 b1, i32x8 a, f32x4& c0, f32x4& c1,
+                                         const int (&b_scale)[kWords<FORM>], const int (&a_scale)[kWords<FORM>]) {
+  if constexpr (FORM == Form::kCodes8) {
+    multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
+    multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
+  } else if constexpr (FORM == Form::kCodes4) {
+    multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
+    multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
+    multiply_part<FORM, OA, 0, 1>(b0, a, c0, b_scale, a_scale);
+    multiply_part<FORM, OA, 1, 1>(b1, a, c1, b_scale, a_scale);
+  } else {
+    multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
+    multiply_part<FORM, OA, 0, 1>(b0, a, c0, b_scale, a_scale);
+    multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
+    multiply_part<FORM, OA, 1, 1>(b1, a, c1, b_scale, a_scale);
   }
 }
 
@@ -395,8 +413,7 @@ __device__ __forceinline__ void quad_tile(const ProductArgs& g, int w) {
   QUAD_FENCE
   auto row = [&](auto qi_, auto qj_, auto i_, i32x8 (&b)[FJ], const int (&s)[2][2][kWords<FORM>]) {
     constexpr int qi = decltype(qi_)::value, qj = decltype(qj_)::value, i = decltype(i_)::value;
-    multiply<FORM, i, 0>(b[0], a[i], acc[qi * FI + i][qj * FJ], s[1][qj], s[0][qi]);
-    multiply<FORM, i, 1>(b[1], a[i], acc[qi * FI + i][qj * FJ + 1], s[1][qj], s[0][qi]);
+    multiply<FORM, i>(b[0], b[1], a[i], acc[qi * FI + i][qj * FJ], acc[qi * FI + i][qj * FJ + 1], s[1][qj], s[0][qi]);
     QUAD_FENCE
   };
   using I0 = std::integral_constant<int, 0>;
@@ -682,10 +699,8 @@ __device__ __forceinline__ void small_tile(const ProductArgs& g, int w) {
       as[k] = scale_bytes<2>(now.as[k], i16);
       bs[k] = scale_bytes<2>(now.bs[k], i16);
     }
-    multiply<FORM, 0, 0>(now.b[0], now.a[0], acc[0][0], bs, as);
-    multiply<FORM, 0, 1>(now.b[1], now.a[0], acc[0][1], bs, as);
-    multiply<FORM, 1, 0>(now.b[0], now.a[1], acc[1][0], bs, as);
-    multiply<FORM, 1, 1>(now.b[1], now.a[1], acc[1][1], bs, as);
+    multiply<FORM, 0>(now.b[0], now.b[1], now.a[0], acc[0][0], acc[0][1], bs, as);
+    multiply<FORM, 1>(now.b[0], now.b[1], now.a[1], acc[1][0], acc[1][1], bs, as);
   };
 #pragma unroll 1
   for (int s = 0; s < min(R - 1, n_stages); ++s) issue(s);
@@ -796,17 +811,27 @@ struct Plan {
 
 // Estimated time, us: rounds of one workgroup per CU, each its stages plus a fixed part (first
 // loads, stores; a second round of 64 x 64 tiles waits for the LDS of the first), and, where the
-// depth is split, one more launch and the sums' way to memory and back. Measured, codes, us on 256 /
-// 128 / 64 tiles: 8192^3 395 / 448 / 1338, 8192 x 14336 x 4096 358 / 423 / 1285, 4096^3 56 / 63 / 186;
+// depth is split, one more launch and the sums' way to memory and back. Measured, us on 256 / 128 / 64
+// tiles, the time of an empty launch (3) included:
+// 8 bits: 8192^3 395 / 448 / 1338, 8192 x 14336 x 4096 358 / 423 / 1285, 4096^3 56 / 63 / 186;
 // 8192 x 2304 x 768 28 / 23 / 71, 3001 x 1408 x 2048 25 / 16 / 35, 2048^3 24 / 11 / 29; 64 x 14336 x
 // 4096 39 / 19 / 14, 1024^3 15 / 7.0 / 6.1, 512^3 11 / 5.7 / 4.7. Split in 1 / 2 / 4 / 8, 128 tiles:
-// 100 x 4096 x 14336 48 / 32 / 23 / 22, expanded 2304 x 768 x 8192 56 / 41 / 41 / 48. The rule takes the
-// fastest on all of them.
-inline double plan_time(int64_t m, int64_t n, int64_t stages, int tile, int64_t splits) {
-  constexpr double stage[3] = {1.4, 0.42, 0.28}, fixed[3] = {5.0, 1.0, 0.6};
+// 100 x 4096 x 14336 48 / 32 / 23 / 22, expanded 2304 x 768 x 8192 56 / 41 / 41 / 48.
+// 4 bits, whose stages are twice as deep: 8192 x 14336 x 4096 232 / 260, 8192 x 4096 x 14336 192 / 233 /
+// 642, 4096^3 35 / 40 / 116, 4096 x 14336 x 4096 128 / 133 / 401, 5000^3 74 / 77 / 214; 8192 x 2304 x 768
+// 24 / 17 / 30, 3001 x 1408 x 2048 19 / 13 / 25, 1024 x 4096 x 4096 26 / 13 / 31; 256 x 4096 x 4096 25 / 12 /
+// 8.7, 64 x 4096 x 4096 27 / 13 / 8.4. Split: 100 x 4096 x 14336 31 whole on 128 tiles, 17 in 8 there, 16 in
+// 2 on 64; 700 x 700 x 16384 24 whole on 64 tiles, 18 in 2. Either rule takes the fastest on nearly all of
+// them, and none that is 5% slower.
+struct Cost {
+  double stage[3], fixed[3];
+};
+constexpr Cost kCost8{{1.4, 0.42, 0.28}, {5.0, 1.0, 0.6}}, kCost4{{1.56, 0.5, 0.33}, {7.5, 1.4, 0.6}};
+
+inline double plan_time(const Cost& cost, int64_t m, int64_t n, int64_t stages, int tile, int64_t splits) {
   const int64_t per = ceil_div(stages, splits);
   const int64_t rounds = ceil_div(ceil_div(m, kSide[tile]) * ceil_div(n, kSide[tile]) * splits, 256);
-  double t = (double)rounds * (stage[tile] * (double)per + fixed[tile] +
+  double t = (double)rounds * (cost.stage[tile] * (double)per + cost.fixed[tile] +
                                (tile == kSmall && rounds > 1 ? 1.4 : 0.0));
   if (splits > 1) t += 3.0 + (double)(2 * splits * m * n * 4) / 4.0e6;
   return t;
@@ -814,15 +839,15 @@ inline double plan_time(int64_t m, int64_t n, int64_t stages, int tile, int64_t 
 
 constexpr int kMaxSplits = 16, kSplitStages = 8;  // ranges of a depth, least stages of one
 
-inline Plan plan(int64_t m, int64_t n, int64_t stages) {
+inline Plan plan(const Cost& cost, int64_t m, int64_t n, int64_t stages) {
   Plan best{kSmall, 1, (int)stages};
-  double least = plan_time(m, n, stages, kSmall, 1);
+  double least = plan_time(cost, m, n, stages, kSmall, 1);
   for (int tile = kBig; tile <= kSmall; ++tile)
     for (int64_t splits = 1; splits <= kMaxSplits; ++splits) {
       const int64_t per = ceil_div(stages, splits), used = ceil_div(stages, per);
       if (splits > 1 && per < kSplitStages) break;
       if (stages - (used - 1) * per < kMinStages[tile]) continue;  // the last range
-      const double t = plan_time(m, n, stages, tile, used);
+      const double t = plan_time(cost, m, n, stages, tile, used);
       if (t < least) {
         least = t;
         best = {tile, (int)used, (int)per};
