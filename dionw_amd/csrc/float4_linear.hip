@@ -2,6 +2,8 @@
 // the product of a few rows with a kept weight.
 #include "float4.h"
 
+#include <type_traits>
+
 namespace dionw {
 namespace {
 
@@ -13,7 +15,8 @@ namespace {
 // sums through LDS, in a fixed order. Of a stage, a lane holds one token's (or weight row's) two
 // blocks of 32, number G = lane / 16 and 4 + G: a block's scale and codes are its lane's own, without
 // an exchange. A wave reads the next stage while it multiplies one.
-// Bound: HBM, n k / 2 bytes of W; the smallest calls: launch and the latency of two dependent reads.
+// Bound: HBM, n k (1 / 2 + 1 / 32) bytes of W: 128256 x 4096 55 us, 5.0 TB/s; the smallest calls: launch
+// and the latency of two dependent reads.
 constexpr int kFew = 16;
 bool few_rows(int64_t m, int64_t k) { return k > 0 && m <= kFew; }
 
@@ -86,10 +89,12 @@ struct Values {
   }
 };
 
-__device__ __forceinline__ f32x4 multiply4(i32x4 b, i32x4 a, f32x4 c, uint32_t b_scale, uint32_t a_scale) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+// c += b a^T; b's scale is byte B of its word.
+template <int B>
+__device__ __forceinline__ void multiply4(i32x4 b, i32x4 a, f32x4& c, uint32_t b_scale, uint32_t a_scale) {
+  c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
       __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1),
-      __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4, 0, (int)b_scale, 0, (int)a_scale);
+      __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4, B, (int)b_scale, 0, (int)a_scale);
 }
 
 template <typename T, int R, int W, bool WHOLE>
@@ -100,25 +105,25 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
   const int n0 = blockIdx.x * 16 * R, token = blockIdx.y * 16 + i16;
   const T* x = reinterpret_cast<const T*>(g.x) + min(token, g.m - 1) * g.x_ld + kBlock4 * G;
   const uint8_t* w[R];
-  int row[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    row[r] = min(n0 + 16 * r + i16, g.n - 1);
-    w[r] = g.w + (int64_t)row[r] * g.stages * 128 + 16 * G;
-  }
+  for (int r = 0; r < R; ++r)
+    w[r] = g.w + (int64_t)min(n0 + R * i16 + r, g.n - 1) * g.stages * 128 + 16 * G;
+  // A block's bytes run to a multiple of 16; words past the last belong to rows past it too.
+  const uint8_t* scale = g.w_scale + G * g.w_scale_ld + min((int64_t)n0 + R * i16, g.w_scale_ld - R);
+  using Word = std::conditional_t<R == 4, uint32_t, std::conditional_t<R == 2, uint16_t, uint8_t>>;
   struct Stage {
     Values<T> x[2];
     i32x4 w[R][2];
-    uint32_t byte[R][2];
+    uint32_t bytes[2];
   };
   auto read = [&](Stage& s, int kt) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int r = 0; r < R; ++r)
         s.w[r][h] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w[r] + (int64_t)kt * 128 + 64 * h));
-        s.byte[r][h] = g.w_scale[((int64_t)kt * 8 + 4 * h + G) * g.w_scale_ld + row[r]];
-      }
+      s.bytes[h] = *reinterpret_cast<const Word*>(scale + ((int64_t)kt * 8 + 4 * h) * g.w_scale_ld);
+    }
     const int64_t at = (int64_t)kt * kDepth4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -137,8 +142,12 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
     for (int h = 0; h < 2; ++h) {
       const uint32_t byte = scale_byte4<false>(s.x[h].most());
       const i32x4 c = s.x[h].codes(power(byte));
-#pragma unroll
-      for (int r = 0; r < R; ++r) acc[r] = multiply4(s.w[r][h], c, acc[r], s.byte[r][h], byte);
+      multiply4<0>(s.w[0][h], c, acc[0], s.bytes[h], byte);
+      if constexpr (R > 1) multiply4<1>(s.w[1][h], c, acc[1], s.bytes[h], byte);
+      if constexpr (R > 2) {
+        multiply4<2>(s.w[2][h], c, acc[2], s.bytes[h], byte);
+        multiply4<3>(s.w[3][h], c, acc[3], s.bytes[h], byte);
+      }
     }
   };
   Stage a, b;
@@ -154,38 +163,52 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
 #pragma unroll
   for (int r = 0; r < R; ++r) sums[wave][r][lane] = acc[r];
   __syncthreads();
-  for (int t = wave; t < R; t += W) {  // a fragment a wave: lane: token i16, rows 4 G .. + 3 of W
-    f32x4 s = sums[0][t][lane];
+  // Value e of a lane's fragments: token i16, rows R (4 G + e) .. + R - 1 of W; a wave each.
+  for (int e = wave; e < 4; e += W) {
+    const int n = n0 + R * (4 * G + e);
+    float s[R];
 #pragma unroll
-    for (int v = 1; v < W; ++v) s += sums[v][t][lane];
-    const int n = n0 + 16 * t + 4 * G;
+    for (int r = 0; r < R; ++r) {
+      s[r] = sums[0][r][lane][e];
+#pragma unroll
+      for (int v = 1; v < W; ++v) s[r] += sums[v][r][lane][e];
+    }
     if (token >= g.m || n >= g.n) continue;
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    typedef T t4any __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    t4 o;
+    typedef T row __attribute__((ext_vector_type(R)));
+    typedef T anywhere __attribute__((ext_vector_type(R), aligned(sizeof(T))));
+    row o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (T)(s[e] + (g.bias ? g.bias[min(n + e, g.n - 1)] : 0.f));
+    for (int r = 0; r < R; ++r) o[r] = (T)(s[r] + (g.bias ? g.bias[min(n + r, g.n - 1)] : 0.f));
     T* y = reinterpret_cast<T*>(g.y) + (int64_t)token * g.n + n;
-    if (n + 4 <= g.n) {
-      *reinterpret_cast<t4any*>(y) = o;
+    if (n + R <= g.n) {
+      *reinterpret_cast<anywhere*>(y) = o;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < g.n) y[e] = o[e];
+      for (int r = 0; r < R; ++r)
+        if (n + r < g.n) y[r] = o[r];
     }
   }
 }
 
-// R rows' fragments a wave and W waves a workgroup.
+// R rows' fragments a wave and W waves a workgroup: many fragments take 64 rows each (x is read and
+// quantized once for them, and a lane's four scale bytes are one load), few the most workgroups. us in
+// calls from Python (7.6 at least), R W = 1 8 / 2 4 / 4 4 / 4 2, bfloat16, a row of x: 4096 x 4096 7.7 /
+// 7.9 / 9.8 / 11.0, 4096 x 14336 12.2 / 16.8 / 25.7 / 30.5, 6144 x 4096 8.0 / 7.6 / 10.1 / 11.1, 8192 x 4096
+// 8.4 / 7.7 / 10.2 / 11.4, 14336 x 4096 12.8 / 11.4 / 10.8 / 11.8 (16 rows 22 / 15.8 / 12.4 / 13.9), 128256 x
+// 4096 77 / 61 / 55.5 / 57.9 (16 rows 155 / 102 / 75 / 78). float32 values take twice the registers, so
+// that fewer workgroups of 4 waves fit: 128256 x 4096 163 / 82 / 85 / 66.5 (16 rows 342 / 189 / 128 / 105).
+// The number of rows is not asked, so that a row's sums do not depend on the rows beside it.
+template <typename T, int R, int W, bool WHOLE>
+void launch_few(const FewArgs& g, int fragments, hipStream_t stream) {
+  hipLaunchKernelGGL((float4_few_kernel<T, R, W, WHOLE>), dim3((unsigned)(fragments + R - 1) / R, (unsigned)(g.m + 15) / 16),
+                     dim3(W * 64), 0, stream, g);
+}
 template <typename T, bool WHOLE>
 int launch_few(const FewArgs& g, hipStream_t stream) {
   const int fragments = (g.n + 15) / 16;
-  const unsigned groups = (unsigned)(g.m + 15) / 16;
-  const int64_t all = (int64_t)fragments * groups;
-  if (all < 320)
-    hipLaunchKernelGGL((float4_few_kernel<T, 1, 8, WHOLE>), dim3(fragments, groups), dim3(512), 0, stream, g);
-  else
-    hipLaunchKernelGGL((float4_few_kernel<T, 4, 4, WHOLE>), dim3((fragments + 3) / 4, groups), dim3(256), 0, stream, g);
+  if (fragments < 320) launch_few<T, 1, 8, WHOLE>(g, fragments, stream);
+  else if (fragments <= 640) launch_few<T, 2, 4, WHOLE>(g, fragments, stream);
+  else launch_few<T, 4, sizeof(T) == 4 ? 2 : 4, WHOLE>(g, fragments, stream);
   return check_launch("float4_few");
 }
 
@@ -345,7 +368,8 @@ int dionw_float4_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const 
   if (m == 0 || n == 0) return kOk;
   const int64_t depth = round_up(k, kDepth4);
   DIONW_REQUIRE(y && (k == 0 || (x && w && w_scale)), "float4_linear: null pointer");
-  DIONW_REQUIRE(x_ld >= k && aligned16(w) && w_scale_ld >= n && aligned16(scratch),
+  DIONW_REQUIRE(x_ld >= k && aligned16(w) && w_scale_ld >= n && w_scale_ld % 16 == 0 && aligned16(w_scale) &&
+                    aligned16(scratch),
                 "float4_linear: an operand is too small or not aligned");
   if (few_rows(m, k)) {
     DIONW_REQUIRE(depth / kDepth4 < INT32_MAX / 16, "float4_linear: depth too large");
