@@ -3,6 +3,7 @@ they refuse, and how they call the library."""
 
 from __future__ import annotations
 
+from collections.abc import Callable
 from typing import Any, Final
 
 import torch
@@ -52,6 +53,28 @@ def readable(x: Tensor) -> Tensor:
 def pitch(x: Tensor) -> int:
     """Elements between the rows of a readable matrix."""
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def once_differentiable(backward: Callable[..., Any]) -> Callable[..., Any]:
+    """A backward pass whose gradients may not be differentiated again, whatever they depend on:
+    where a graph of it is asked for, they raise once one is. (torch's own decorator lets them pass as
+    constants where the incoming gradient is one, and costs a call on every pass.)"""
+
+    def run(ctx: Any, *gradients: Tensor) -> Any:
+        if not torch.is_grad_enabled():
+            return backward(ctx, *gradients)
+        with torch.no_grad():
+            found = backward(ctx, *gradients)
+        places = [i for i, g in enumerate(found) if g is not None]
+        refuse = torch._C._functions.DelayedError(
+            b"the gradients of dionw_amd's operators are not differentiable a second time", len(places))
+        refusing = refuse(*[found[i].detach().requires_grad_() for i in places])
+        found = list(found)
+        for i, g in zip(places, refusing if isinstance(refusing, tuple) else (refusing,)):
+            found[i] = g
+        return tuple(found)
+
+    return run
 
 
 def check_vector(name: str, v: Tensor | None, n: int, device: torch.device) -> None:

@@ -18,7 +18,6 @@ from typing import Any
 
 import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from dionw_amd import _lib
 from dionw_amd._operands import (
@@ -26,6 +25,7 @@ from dionw_amd._operands import (
     call,
     check_unrecorded,
     check_vector,
+    once_differentiable,
     pitch,
     readable,
     scratch,
@@ -48,7 +48,8 @@ def _rows(x: Tensor, weight: Tensor | None, bias: Tensor | None) -> Tensor:
 
 
 def _parameter(p: Tensor | None) -> tuple[int, Tensor | None]:
-    return (_lib.F32, None) if p is None else (CODES[p.dtype], p.detach().contiguous())
+    """A parameter as the kernels read it, held by the caller until the library call has returned."""
+    return (_lib.F32, None) if p is None else (CODES[p.dtype], p if p.is_contiguous() else p.contiguous())
 
 
 def _forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,

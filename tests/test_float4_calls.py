@@ -273,3 +273,12 @@ def test_a_seed_that_does_not_fit_is_refused_before_the_forward(calls) -> None:
         with pytest.raises(ValueError):
             float4_linear(x, w, seed=seed)
     assert not calls
+
+
+def test_a_second_derivative_is_refused(calls) -> None:
+    """Also where the incoming gradient is a constant: the gradient depends on the inputs all the same."""
+    x, w = torch.ones(3, 200, requires_grad=True), torch.ones(5, 200, requires_grad=True)
+    for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+        (dx,) = torch.autograd.grad(loss(float4_linear(x, w)), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second time"):
+            (dx.sum() + x.sum()).backward()

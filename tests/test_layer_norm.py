@@ -135,3 +135,12 @@ def test_the_library_checks_its_arguments() -> None:
                 {"scratch": 18}, {"size": 1}):
         with pytest.raises(ValueError):
             backward(**bad)
+
+
+def test_a_second_derivative_is_refused(calls) -> None:
+    """Also where the incoming gradient is a constant: the gradient depends on the inputs all the same."""
+    x = torch.ones(3, 8, requires_grad=True)
+    for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+        (dx,) = torch.autograd.grad(loss(layer_norm(x)), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second time"):
+            (dx.sum() + x.sum()).backward()
