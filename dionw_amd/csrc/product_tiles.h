@@ -114,25 +114,16 @@ __device__ __forceinline__ void multiply_part(i32x8 b, i32x8 a, f32x4& c, const 
   }
 }
 
-// c0, c1 += b0 a^T, b1 a^T; the scales of b0 and b1 are bytes 0 and 1. 4 bits: the sums take turns, so
-// that no instruction waits for the one before it.
+// c0, c1 += b0 a^T, b1 a^T; the scales of b0 and b1 are bytes 0 and 1. A sum's two parts follow each
+// other: with the sums taking turns the compiler moves 24 accumulation registers in every two stages of
+// the 256 x 256 tile (4 bits, 8192^3: 228 us, in turns 234).
 template <Form FORM, int OA>
 __device__ __forceinline__ void multiply(i32x8 b0, i32x8 b1, i32x8 a, f32x4& c0, f32x4& c1,
                                          const int (&b_scale)[kWords<FORM>], const int (&a_scale)[kWords<FORM>]) {
-  if constexpr (FORM == Form::kCodes8) {
-    multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
-    multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
-  } else if constexpr (FORM == Form::kCodes4) {
-    multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
-    multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
-    multiply_part<FORM, OA, 0, 1>(b0, a, c0, b_scale, a_scale);
-    multiply_part<FORM, OA, 1, 1>(b1, a, c1, b_scale, a_scale);
-  } else {
-    multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
-    multiply_part<FORM, OA, 0, 1>(b0, a, c0, b_scale, a_scale);
-    multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
-    multiply_part<FORM, OA, 1, 1>(b1, a, c1, b_scale, a_scale);
-  }
+  multiply_part<FORM, OA, 0, 0>(b0, a, c0, b_scale, a_scale);
+  if constexpr (FORM != Form::kCodes8) multiply_part<FORM, OA, 0, 1>(b0, a, c0, b_scale, a_scale);
+  multiply_part<FORM, OA, 1, 0>(b1, a, c1, b_scale, a_scale);
+  if constexpr (FORM != Form::kCodes8) multiply_part<FORM, OA, 1, 1>(b1, a, c1, b_scale, a_scale);
 }
 
 // A fragment's two chunks of a lane.
@@ -231,16 +222,21 @@ template <int F>
 __device__ __forceinline__ uint32_t scale_word(const unsigned char* rows, int i16) {
   return *reinterpret_cast<const uint32_t*>(rows + (F * i16 & ~3));
 }
-template <int F>
+template <Form FORM, int F>
 __device__ __forceinline__ int scale_bytes(uint32_t word, int i16) {
-  return F == 4 ? (int)word : (int)(word >> (16 * (i16 & 1)));
+  return F == 4 || FORM == Form::kCodes4 ? (int)word : (int)(word >> (16 * (i16 & 1)));
 }
-// The same word of 4-bit codes: its place among a stage's scales of one operand, for the rows from
-// `row` on and the first of a lane's two blocks, G (the other, 4 + G, lies 4 SIDE bytes behind it).
+// 4-bit codes: the F bytes alone, and their place among a stage's scales of one operand, for the rows
+// from `row` on and the first of a lane's two blocks, G (the other, 4 + G, lies 4 SIDE bytes behind it).
 template <int F, int SIDE>
 __device__ __forceinline__ int scale_place(int row, int G, int i16) {
-  const int r = row + (F * i16 & ~3);
+  const int r = row + F * i16;
   return G * SIDE + ((r / 16 + turn<SIDE>(G)) & (SIDE / 16 - 1)) * 16 + r % 16;
+}
+template <int F>
+__device__ __forceinline__ uint32_t scale_at(const unsigned char* at) {
+  if constexpr (F == 4) return *reinterpret_cast<const uint32_t*>(at);
+  else return *reinterpret_cast<const uint16_t*>(at);
 }
 
 // A lane's 8 columns' bias.
@@ -265,9 +261,13 @@ __device__ __forceinline__ void load_bias(const ProductArgs& g, int q, float (&b
 // load the last row (outputs that are never stored see them). A stage's scale bytes come the
 // same way, one load of a wave for 256 rows, and are read a stage ahead. Whole tiles store from
 // registers, 64 bytes of 16 rows an instruction.
-// Bound: the board's power (8192^3 395 us, 2785 TFLOP/s, 366 sustained at 1387 W of 1400 and 1.8 GHz,
-// the matrix pipe 77% busy; expanded 14336 x 4096 x 8192 720 us, 1336, at 1400 W and 2.05 GHz, 68%);
-// at few stages the first loads and the stores (plan_time; 8192 x 2304 x 768 24 us, 20%).
+// Bound: the board's power (8 bits: 8192^3 395 us, 2785 TFLOP/s, 366 sustained at 1387 W of 1400 and 1.8 GHz,
+// the matrix pipe 77% busy; 4 bits: 228 us, 4820 TFLOP/s, 60% busy at 1.7 GHz, on constant operands 174;
+// the instruction alone on random registers 7200; expanded 14336 x 4096 x 8192 720 us, 1336, at 1400 W and 2.05 GHz, 68%);
+// at few stages the first loads and the stores (plan_time; 8192 x 2304 x 768 24 us, 20%). Stores are
+// 14% of 4-bit 8192 x 14336 x 4096 (229 us, 197 without them): they wait for memory. Not kept there: stores
+// past the caches (241), through LDS in whole rows (232), and workgroups that take one tile after another
+// and load the next one's first stages before the stores (278: the sums leave their registers).
 template <int WM_, int WN_, int FI_, int FJ_>
 struct QuadCfg {
   static constexpr int WM = WM_, WN = WN_, FI = FI_, FJ = FJ_;
@@ -290,10 +290,11 @@ __device__ __forceinline__ void quad_tile(const ProductArgs& g, int w) {
   constexpr int HM = CFG::HM, HN = CFG::HN, FI = CFG::FI, FJ = CFG::FJ, BM = CFG::BM, BN = CFG::BN;
   constexpr int L = CFG::L, W = CFG::waves, S = kScales<FORM> ? 1 : 0;  // S: scale loads of a stage
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* lds_a = smem;                    // [buffer][half][HM][128]
-  unsigned char* lds_b = smem + 4 * CFG::half;
   constexpr int SB = kScaleBytes<FORM, BM>;
-  unsigned char* lds_s = smem + 8 * CFG::half;    // scales: [buffer][operand][SB]
+  // The scales come first, so that a read's offset from a lane's place fits its instruction.
+  unsigned char* lds_s = smem;                    // [buffer][operand][SB]
+  unsigned char* lds_a = smem + 4 * SB;           // [buffer][half][HM][128]
+  unsigned char* lds_b = lds_a + 4 * CFG::half;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -362,12 +363,12 @@ __device__ __forceinline__ void quad_tile(const ProductArgs& g, int w) {
   struct Scales {
     uint32_t a[2][kWords<FORM>], b[2][kWords<FORM>];  // by half: the words of scale_word
   };
-  int a_place[2], b_place[2];  // 4 bits: the words' places by half
+  const unsigned char *a_scale[2], *b_scale[2];  // 4 bits: the bytes by half
   if constexpr (FORM == Form::kCodes4) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      a_place[h] = scale_place<FI, BM>(h * HM + wm * FI * 16, G, i16);
-      b_place[h] = SB + scale_place<FJ, BM>(h * HN + wn * FJ * 16, G, i16);
+      a_scale[h] = lds_s + scale_place<FI, BM>(h * HM + wm * FI * 16, G, i16);
+      b_scale[h] = lds_s + SB + scale_place<FJ, BM>(h * HN + wn * FJ * 16, G, i16);
     }
   }
   auto read_s = [&](Scales& s, int buf) {
@@ -376,9 +377,9 @@ __device__ __forceinline__ void quad_tile(const ProductArgs& g, int w) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const unsigned char* at = lds_s + buf * 2 * SB + k * 4 * BM;
-          s.a[h][k] = *reinterpret_cast<const uint32_t*>(at + a_place[h]);
-          s.b[h][k] = *reinterpret_cast<const uint32_t*>(at + b_place[h]);
+          const int at = buf * 2 * SB + k * 4 * BM;
+          s.a[h][k] = scale_at<FI>(a_scale[h] + at);
+          s.b[h][k] = scale_at<FJ>(b_scale[h] + at);
         }
     } else if constexpr (S) {
 #pragma unroll
@@ -438,8 +439,8 @@ __device__ __forceinline__ void quad_tile(const ProductArgs& g, int w) {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int k = 0; k < kWords<FORM>; ++k) {
-        s[0][h][k] = scale_bytes<FI>(s0.a[h][k], i16);
-        s[1][h][k] = scale_bytes<FJ>(s0.b[h][k], i16);
+        s[0][h][k] = scale_bytes<FORM, FI>(s0.a[h][k], i16);
+        s[1][h][k] = scale_bytes<FORM, FJ>(s0.b[h][k], i16);
       }
     // rows half 0 x columns half 0; B1(kt) is read. Pending: A0(kt), B1(kt) and A1(kt) have
     // landed. Refilled next: A1(kt - 1), B0(kt), S(kt), all read before A0(kt).
@@ -662,8 +663,8 @@ __device__ __forceinline__ void small_tile(const ProductArgs& g, int w) {
     if constexpr (FORM == Form::kCodes4) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        f.as[k] = *reinterpret_cast<const uint32_t*>(s + k * 4 * BM + a_place);
-        f.bs[k] = *reinterpret_cast<const uint32_t*>(s + k * 4 * BM + b_place);
+        f.as[k] = scale_at<2>(s + k * 4 * BM + a_place);
+        f.bs[k] = scale_at<2>(s + k * 4 * BM + b_place);
       }
     } else if constexpr (FORM == Form::kCodes8) {
       f.as[0] = scale_word<2>(s + wm * 32, i16);
@@ -696,8 +697,8 @@ __device__ __forceinline__ void small_tile(const ProductArgs& g, int w) {
     int as[kWords<FORM>], bs[kWords<FORM>];
 #pragma unroll
     for (int k = 0; k < kWords<FORM>; ++k) {
-      as[k] = scale_bytes<2>(now.as[k], i16);
-      bs[k] = scale_bytes<2>(now.bs[k], i16);
+      as[k] = scale_bytes<FORM, 2>(now.as[k], i16);
+      bs[k] = scale_bytes<FORM, 2>(now.bs[k], i16);
     }
     multiply<FORM, 0>(now.b[0], now.b[1], now.a[0], acc[0][0], acc[0][1], bs, as);
     multiply<FORM, 1>(now.b[0], now.b[1], now.a[1], acc[1][0], acc[1][1], bs, as);
