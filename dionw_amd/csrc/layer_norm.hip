@@ -15,7 +15,8 @@ namespace dionw {
 namespace {
 
 constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;
-constexpr int kThreads = 256;
+// Threads of a workgroup whose rows take LANES threads each: one row, or 256 threads of rows of a wave.
+constexpr int threads_of(int lanes) { return lanes > kWave ? lanes : 256; }
 
 struct NormArgs {
   const void* x;
@@ -94,7 +95,8 @@ __device__ __forceinline__ float row_sum(float v, float* sums) {
 // ---- forward ------------------------------------------------------------------------------
 //
 // LANES threads a row, K chunks of 8 columns a thread, `LANES * 8 * K` columns at most.
-// Bound: HBM, x read and y (or half a byte an element) written.
+// Bound: HBM, x read and y (or half a byte an element) written: 8192 x 4096 bfloat16 23 us (5.8 TB/s),
+// float32 41 (6.5), to 4 bits 23.
 
 // Workgroup b's first row. 4-bit output: the rows whose scales share a line of memory run on one XCD
 // (the hardware deals workgroup b to XCD b % 8), whose L2 then writes the line once.
@@ -132,8 +134,8 @@ __device__ __forceinline__ void write8(const NormArgs& g, int64_t row, int64_t c
 }
 
 template <typename T, int LANES, int K, bool CODES>
-__global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void norm_kernel(NormArgs g) {
-  constexpr int kEach = LANES > kThreads ? 1 : kThreads / LANES;
+__global__ __launch_bounds__(threads_of(LANES)) void norm_kernel(NormArgs g) {
+  constexpr int kEach = threads_of(LANES) / LANES;
   __shared__ float sums[2][LANES / kWave + 1];
   const int lane = threadIdx.x % LANES;
   const int64_t row = first_row<CODES>(blockIdx.x, kEach, gridDim.x) + threadIdx.x / LANES;
@@ -228,7 +230,8 @@ __global__ __launch_bounds__(kWide) void norm_wide_kernel(NormArgs g) {
 // A group of rows per workgroup (per wave where a row is one wave's): its threads keep their columns,
 // whose sums for dg and db stay in registers over the group's rows, and the groups' sums are added by a
 // second launch. A row's x and dy are read one row ahead.
-// Bound: HBM, x and dy read and dx written, and 8 bytes a column for each group.
+// Bound: HBM, x and dy read and dx written, and 8 bytes a column for each group: 8192 x 4096 bfloat16
+// 39 us (5.1 TB/s without the groups' sums), the second launch's 4 among them, float32 80.
 struct GradArgs {
   const void *x, *dy;
   int64_t x_ld, dy_ld, rows, cols;
@@ -240,8 +243,8 @@ struct GradArgs {
 };
 
 template <typename T, int LANES, int K>
-__global__ __launch_bounds__(LANES > kThreads ? LANES : kThreads) void norm_grad_kernel(GradArgs g) {
-  constexpr int kEach = LANES > kThreads ? 1 : kThreads / LANES;  // rows at a time
+__global__ __launch_bounds__(threads_of(LANES)) void norm_grad_kernel(GradArgs g) {
+  constexpr int kEach = threads_of(LANES) / LANES;  // rows at a time
   constexpr int kWaves = LANES > kWave ? LANES / kWave : 1;
   __shared__ float sums[2][2][kWaves];
   __shared__ float join[kEach > 1 ? kEach * LANES * 8 : 1];
@@ -451,18 +454,21 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs g) {
 
 template <typename T, int LANES, int K, bool CODES>
 int launch_norm(const NormArgs& g, hipStream_t stream) {
-  constexpr int threads = LANES > kThreads ? LANES : kThreads;
+  constexpr int threads = threads_of(LANES);
   const int64_t grid = ceil_div(g.rows, threads / LANES);
   hipLaunchKernelGGL((norm_kernel<T, LANES, K, CODES>), dim3((unsigned)grid), dim3(threads), 0, stream, g);
   return check_launch("layer_norm");
 }
 
+// Fewer threads a row wait less for each other, more of them hold more rows' loads in flight. us of
+// 64 2 / 64 4 / 128 2 / 256 1 / 256 2 / 512 1, bfloat16: 8192 x 768 7.7 / 9.8 / 9.9 / 12.0 / 14.8 / 22.0, 16384 x
+// 2048 - / 25.0 / 22.9 / 27.3 / 27.8 / 42.4, 8192 x 4096 (64 8 28.6, 128 4 24.7) 256 2 23.3, 512 1 26.7.
 template <typename T, bool CODES>
 int launch_norm(const NormArgs& g, hipStream_t stream) {
   if (g.cols <= 128 && !CODES) return launch_norm<T, 16, 1, false>(g, stream);
   if (g.cols <= 512) return launch_norm<T, 64, 1, CODES>(g, stream);
   if (g.cols <= 1024) return launch_norm<T, 64, 2, CODES>(g, stream);
-  if (g.cols <= 2048) return launch_norm<T, 256, 1, CODES>(g, stream);
+  if (g.cols <= 2048) return launch_norm<T, 128, 2, CODES>(g, stream);
   if (g.cols <= 4096) return launch_norm<T, 256, 2, CODES>(g, stream);
   if (g.cols <= 8192) return launch_norm<T, 256, 4, CODES>(g, stream);
   if (g.cols <= 16384) return launch_norm<T, 512, 4, CODES>(g, stream);
@@ -477,18 +483,20 @@ int launch_norm(int32_t elem, const NormArgs& g, hipStream_t stream) {
   return launch_norm<float, CODES>(g, stream);
 }
 
-constexpr int64_t kWidest = 16384;  // columns of a row that a workgroup's registers hold
+constexpr int64_t kWidest = 8192;  // columns of a row whose gradients a workgroup's registers hold
 
-// Groups of rows whose column sums are kept apart: as many as the GPU runs at a time.
+// Groups of rows whose column sums are kept apart: as many as run at a time, of two rows a wave or
+// workgroup at least. us, bfloat16, 256 / 512 / 768 / 1024 groups: 8192 x 4096 42 / 39.3 / 46 / 46, 16384 x
+// 2048 - / 41 / 38 / 40, 8192 x 768 20 / 16.3 / 20.6 / 21, 32768 x 300 55 / 34 / 30 / 28, 2048 x 1024 9.5 / 10.6.
 int64_t row_groups(int64_t rows, int64_t cols) {
   if (cols > kWidest) return std::min<int64_t>(64, rows);
-  const int each = cols <= 1024 ? 4 : 1;
-  return std::min<int64_t>(ceil_div(rows, each), cols <= 4096 ? 512 : 256);
+  const int each = cols <= 1024 ? 8 : 2;
+  return std::min<int64_t>(ceil_div(rows, each), cols <= 512 ? 1024 : cols <= 4096 ? 512 : 256);
 }
 
 template <typename T, int LANES, int K>
 int launch_grad(const GradArgs& g, hipStream_t stream) {
-  constexpr int threads = LANES > kThreads ? LANES : kThreads;
+  constexpr int threads = threads_of(LANES);
   hipLaunchKernelGGL((norm_grad_kernel<T, LANES, K>), dim3((unsigned)row_groups(g.rows, g.cols)), dim3(threads), 0,
                      stream, g);
   return check_launch("layer_norm_backward");
@@ -500,8 +508,7 @@ int launch_grad(const GradArgs& g, hipStream_t stream) {
   if (g.cols <= 1024) return launch_grad<T, 64, 2>(g, stream);
   if (g.cols <= 2048) return launch_grad<T, 256, 1>(g, stream);
   if (g.cols <= 4096) return launch_grad<T, 256, 2>(g, stream);
-  if (g.cols <= 8192) return launch_grad<T, 512, 2>(g, stream);
-  if (g.cols <= kWidest) return launch_grad<T, 1024, 2>(g, stream);
+  if (g.cols <= kWidest) return launch_grad<T, 512, 2>(g, stream);
   if (g.dx) {
     hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)g.rows), dim3(kWide), 0, stream, g);
     DIONW_TRY(check_launch("layer_norm_backward_wide"));
