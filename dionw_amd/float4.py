@@ -240,14 +240,17 @@ def _sizes(m: int, n: int, k: int, need_x: bool, need_w: bool, need_b: bool) -> 
 def _forward(x: Tensor, weight: Tensor, bias: Tensor | None, need_x: bool, need_w: bool,
              need_b: bool) -> tuple[Tensor, Tensor | None, int]:
     """y, what the gradients asked for need of x and W, and the bytes of the backward's scratch."""
-    x, weight = _readable(x), _readable(weight)
+    if not x.is_contiguous():
+        x = readable(x)
+    if not weight.is_contiguous():
+        weight = readable(weight)
     m, k = x.shape
     n, device = weight.shape[0], x.device
     stream = _lib.stream_handle(device)
     keep, room, backward_room = _sizes(m, n, k, need_x, need_w, need_b)
     saved, scratch = _scratch(keep, device), _scratch(room, device)
     y = torch.empty(m, n, dtype=x.dtype, device=device)
-    added = float_bias(bias, n, device)
+    added = None if bias is None else float_bias(bias, n, device)
     call(device, "dionw_float4_linear_forward", CODES[x.dtype], x.data_ptr(), pitch(x), CODES[weight.dtype],
          weight.data_ptr(), pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w, y.data_ptr(),
          _lib.ptr(saved), _lib.ptr(scratch), room, stream)
@@ -259,34 +262,50 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None, seed: int | Tensor | None) -> Tensor:
-        needs = ctx.needs_input_grad[:3]
-        y, saved, ctx.room = _forward(x, weight, bias, *needs)
-        if seed is None and (needs[0] or needs[1]):
-            seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
+        # What the backward needs is worked out here: it runs on a thread of torch's own, whose caches
+        # hold none of this.
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        y, saved, room = _forward(x, weight, bias, need_x, need_w, need_b)
+        if seed is None:
+            seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_()) if need_x or need_w else 0
         # A seed on the device is read when the backward runs, whatever it holds then.
-        ctx.seed = 0 if seed is None else seed.detach() if isinstance(seed, Tensor) else seed
-        ctx.codes = CODES[x.dtype], CODES[weight.dtype]
-        ctx.sizes, ctx.dtypes = (x.shape[0], *weight.shape), (x.dtype, weight.dtype)
-        ctx.bias_dtype = bias.dtype if needs[2] else None
-        ctx.save_for_backward(*([] if saved is None else [saved]))
+        ctx.seed = seed.detach() if isinstance(seed, Tensor) else seed
+        ctx.number, ctx.seed_at = _seed(ctx.seed, x.device)
+        ctx.sizes, ctx.room = (x.shape[0], *weight.shape), room
+        ctx.dtypes = x.dtype, weight.dtype, bias.dtype if need_b else torch.float32
+        ctx.device = x.device
+        ctx.save_for_backward(saved)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, dy: Tensor) -> tuple[Tensor | None, ...]:
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         m, n, k = ctx.sizes
-        dy, device = _readable(dy), dy.device
-        saved = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        number, address = _seed(ctx.seed, device)
-        scratch = _scratch(ctx.room, device)
-        dx = torch.empty(m, k, dtype=ctx.dtypes[0], device=device) if need_x else None
-        dw = torch.empty(n, k, dtype=ctx.dtypes[1], device=device) if need_w else None
-        db = torch.empty(n, dtype=ctx.bias_dtype, device=device) if need_b else None
-        call(device, "dionw_float4_linear_backward", ctx.codes[0], dy.data_ptr(), pitch(dy), ctx.codes[1],
-             m, n, k, need_x, need_w, number, address, _lib.ptr(saved), _lib.ptr(dx), _lib.ptr(dw),
-             CODES[ctx.bias_dtype] if need_b else 0, _lib.ptr(db), _lib.ptr(scratch), ctx.room,
-             _lib.stream_handle(device))
+        x_dtype, w_dtype, b_dtype = ctx.dtypes
+        device, room = ctx.device, ctx.room
+        (saved,) = ctx.saved_tensors
+        ld = n
+        if not dy.is_contiguous():
+            dy = readable(dy)
+            ld = pitch(dy)
+        dx = dw = db = scratch = dx_at = dw_at = db_at = scratch_at = None
+        if need_x:
+            dx = torch.empty(m, k, dtype=x_dtype, device=device)
+            dx_at = dx.data_ptr()
+        if need_w:
+            dw = torch.empty(n, k, dtype=w_dtype, device=device)
+            dw_at = dw.data_ptr()
+        if need_b:
+            db = torch.empty(n, dtype=b_dtype, device=device)
+            db_at = db.data_ptr()
+        if room:
+            scratch = torch.empty(room, dtype=torch.uint8, device=device)
+            scratch_at = scratch.data_ptr()
+        # The engine runs this on x's device, and on the forward's stream.
+        _lib.call("dionw_float4_linear_backward", CODES[x_dtype], dy.data_ptr(), ld, CODES[w_dtype], m, n, k,
+                  need_x, need_w, ctx.number, ctx.seed_at, None if saved is None else saved.data_ptr(), dx_at,
+                  dw_at, CODES[b_dtype], db_at, scratch_at, room, _lib.stream_handle(device))
         return dx, dw, db, None
 
 
@@ -364,6 +383,9 @@ def float4_linear(x: Tensor, weight: Tensor | Float4Matrix, bias: Tensor | None 
     check_vector("bias", bias, weight.shape[0], x.device)
     if isinstance(seed, Tensor):
         _seed(seed, x.device)
+    for t in (x, weight):
+        if t.dtype not in CODES:
+            raise ValueError(f"float4_linear takes float16, bfloat16 or float32 tensors, got {t.dtype}")
     flat = x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), shape[-1])
     # Asked here: inside the function gradients are off, and what it is told of its inputs' needs
     # does not know whether they were on.

@@ -28,7 +28,6 @@ from dionw_amd._operands import (
     once_differentiable,
     pitch,
     readable,
-    scratch,
     watched,
 )
 from dionw_amd.float4 import Float4Matrix, empty
@@ -37,19 +36,29 @@ __all__ = ["LayerNorm", "float4_layer_norm", "layer_norm"]
 
 
 def _rows(x: Tensor, weight: Tensor | None, bias: Tensor | None) -> Tensor:
-    """x as a matrix, once the arguments fit each other."""
-    if x.dim() == 0 or x.shape[-1] == 0 or x.dtype not in CODES:
+    """x as a matrix that the kernels read, once the arguments fit each other."""
+    shape = x.shape
+    if not shape or shape[-1] == 0 or x.dtype not in CODES:
         raise ValueError("layer norm takes float16, bfloat16 or float32 rows of one value at least, got "
-                         f"{x.dtype} of shape {tuple(x.shape)}")
-    cols = x.shape[-1]
-    check_vector("norm's weight", weight, cols, x.device)
-    check_vector("norm's bias", bias, cols, x.device)
-    return x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), cols)
+                         f"{x.dtype} of shape {tuple(shape)}")
+    cols = shape[-1]
+    if weight is not None:
+        check_vector("norm's weight", weight, cols, x.device)
+    if bias is not None:
+        check_vector("norm's bias", bias, cols, x.device)
+    if len(shape) != 2:
+        x = x.reshape(math.prod(shape[:-1]), cols)
+    return x if x.is_contiguous() else readable(x)
 
 
-def _parameter(p: Tensor | None) -> tuple[int, Tensor | None]:
-    """A parameter as the kernels read it, held by the caller until the library call has returned."""
-    return (_lib.F32, None) if p is None else (CODES[p.dtype], p if p.is_contiguous() else p.contiguous())
+def _parameter(p: Tensor | None) -> tuple[int, Tensor | None, int | None]:
+    """A parameter's element code, and it as the kernels read it, held by the caller until the library
+    call has returned."""
+    if p is None:
+        return _lib.F32, None, None
+    if not p.is_contiguous():
+        p = p.contiguous()
+    return CODES[p.dtype], p, p.data_ptr()
 
 
 def _forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
@@ -58,11 +67,14 @@ def _forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
     (m, n), device = x.shape, x.device
     stream = _lib.stream_handle(device)
     y = torch.empty(m, n, dtype=x.dtype, device=device)
-    stats = torch.empty(2, m, dtype=torch.float32, device=device) if keep else None
-    (w_code, weight), (b_code, bias) = _parameter(weight), _parameter(bias)
-    at = (None, None) if stats is None else (stats.data_ptr(), stats.data_ptr() + 4 * m)
-    call(device, "dionw_layer_norm_forward", CODES[x.dtype], x.data_ptr(), pitch(x), m, n, w_code,
-         _lib.ptr(weight), b_code, _lib.ptr(bias), eps, y.data_ptr(), *at, stream)
+    stats, at = None, 0
+    if keep:
+        stats = torch.empty(2, m, dtype=torch.float32, device=device)
+        at = stats.data_ptr()
+    w_code, weight, w_at = _parameter(weight)
+    b_code, bias, b_at = _parameter(bias)
+    call(device, "dionw_layer_norm_forward", CODES[x.dtype], x.data_ptr(), pitch(x), m, n, w_code, w_at, b_code,
+         b_at, eps, y.data_ptr(), at or None, at + 4 * m if at else None, stream)
     return y, stats
 
 
@@ -77,9 +89,13 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float) -> Tensor:
-        x = readable(x)
-        y, stats = _forward(x, weight, bias, eps, any(ctx.needs_input_grad))
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        # What the backward needs is worked out here: it runs on a thread of torch's own, whose caches
+        # hold none of this.
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        y, stats = _forward(x, weight, bias, eps, need_x or need_w or need_b)
+        m, n = x.shape
+        ctx.bias_dtype = bias.dtype if need_b else torch.float32
+        ctx.room = _backward_scratch(m, n) if need_w or need_b else 0
         ctx.save_for_backward(x, weight, stats)
         return y
 
@@ -88,19 +104,30 @@ class _Norm(torch.autograd.Function):
     def backward(ctx: Any, dy: Tensor) -> tuple[Tensor | None, ...]:
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         x, weight, stats = ctx.saved_tensors
-        (m, n), device = x.shape, x.device
-        dy = readable(dy)
-        w_code, gain = _parameter(weight)
-        stream = _lib.stream_handle(device)
-        dx = torch.empty(m, n, dtype=x.dtype, device=device) if need_x else None
-        dg = torch.empty(n, dtype=weight.dtype, device=device) if need_w else None
-        db = torch.empty(n, dtype=ctx.bias_dtype, device=device) if need_b else None
-        size = _backward_scratch(m, n) if need_w or need_b else 0
-        space = scratch(size, device)
-        call(device, "dionw_layer_norm_backward", CODES[x.dtype], x.data_ptr(), pitch(x), dy.data_ptr(),
-             pitch(dy), m, n, w_code, _lib.ptr(gain), stats.data_ptr(), stats.data_ptr() + 4 * m, _lib.ptr(dx),
-             _lib.ptr(dg), CODES[ctx.bias_dtype] if need_b else _lib.F32, _lib.ptr(db), _lib.ptr(space), size,
-             stream)
+        (m, n), device, room = x.shape, x.device, ctx.room
+        ld = n
+        if not dy.is_contiguous():
+            dy = readable(dy)
+            ld = pitch(dy)
+        dx = dg = db = space = dx_at = dg_at = db_at = space_at = None
+        if need_x:
+            dx = x.new_empty(m, n)
+            dx_at = dx.data_ptr()
+        if need_w:
+            dg = torch.empty_like(weight, memory_format=torch.contiguous_format)
+            dg_at = dg.data_ptr()
+        if need_b:
+            db = torch.empty(n, dtype=ctx.bias_dtype, device=device)
+            db_at = db.data_ptr()
+        if room:
+            space = torch.empty(room, dtype=torch.uint8, device=device)
+            space_at = space.data_ptr()
+        w_code, weight, w_at = _parameter(weight)
+        at = stats.data_ptr()
+        # The engine runs this on x's device, and on the forward's stream.
+        _lib.call("dionw_layer_norm_backward", CODES[x.dtype], x.data_ptr(), pitch(x), dy.data_ptr(), ld, m, n,
+                  w_code, w_at, at, at + 4 * m, dx_at, dg_at, CODES[ctx.bias_dtype], db_at, space_at, room,
+                  _lib.stream_handle(device))
         return dx, dg, db, None
 
 
@@ -124,7 +151,7 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     if torch.is_grad_enabled():
         y = _Norm.apply(flat, weight, bias, eps)
     else:
-        y = _forward(readable(flat), weight, bias, eps, False)[0]
+        y = _forward(flat, weight, bias, eps, False)[0]
     return y if x.dim() == 2 else y.view(x.shape)
 
 
@@ -141,14 +168,14 @@ def float4_layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | No
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         raise ValueError("float4_layer_norm is for inference: use layer_norm and float4_linear where "
                          "gradients are needed, or call under torch.no_grad()")
-    flat = readable(_rows(x, weight, bias))
+    flat = _rows(x, weight, bias)
     (m, n), device = flat.shape, flat.device
     stream = _lib.stream_handle(device)
     q = empty(m, n, device)
-    (w_code, weight), (b_code, bias) = _parameter(weight), _parameter(bias)
-    call(device, "dionw_layer_norm_float4", CODES[flat.dtype], flat.data_ptr(), pitch(flat), m, n, w_code,
-         _lib.ptr(weight), b_code, _lib.ptr(bias), eps, q.data.data_ptr(), q.scale.data_ptr(), q.scale.shape[1],
-         stream)
+    w_code, weight, w_at = _parameter(weight)
+    b_code, bias, b_at = _parameter(bias)
+    call(device, "dionw_layer_norm_float4", CODES[flat.dtype], flat.data_ptr(), pitch(flat), m, n, w_code, w_at,
+         b_code, b_at, eps, q.data.data_ptr(), q.scale.data_ptr(), q.scale.shape[1], stream)
     return q
 
 
