@@ -241,10 +241,9 @@ def call(name: str, *args: Any) -> None:
         ValueError: For a rejected argument (code 1).
         RuntimeError: For a failed launch (code 2).
     """
-    lib = library()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(_LIB or library(), name)(*args)
     if rc != 0:
-        message = lib.dionw_last_error().decode(errors="replace")
+        message = library().dionw_last_error().decode(errors="replace")
         if rc == 1:
             raise ValueError(f"{name}: {message}")
         raise RuntimeError(f"{name}: {message}")

@@ -19,6 +19,8 @@ CODES: Final = {dtype: _lib.elem_code(dtype) for dtype in DTYPES}
 # make_fx runs under (as harmless ones do).
 tracing = torch._C._is_tracing
 function_modes = torch._C._len_torch_function_stack
+# Of a process that has a GPU tensor, which is what asks.
+_current_device = torch._C._cuda_getDevice
 
 
 def check_unrecorded(*tensors: Tensor | None) -> None:
@@ -97,7 +99,7 @@ def scratch(size: int, device: torch.device) -> Tensor | None:
 def call(device: torch.device, name: str, *args: Any) -> None:
     """``_lib.call`` with ``device`` the current one: a default stream has no device of its own."""
     index = device.index
-    if index is None or index == torch.cuda.current_device():
+    if index is None or index == _current_device():
         _lib.call(name, *args)
     else:
         with torch.cuda.device(index):

@@ -108,18 +108,24 @@ class Float4Matrix:
         """
         if watched():
             check_unrecorded()
-        stream = _lib.stream_handle(self.device)
-        out = torch.empty(self.shape, dtype=torch.float32, device=self.device)
-        call(self.device, "dionw_float4_values", self.data.data_ptr(), self.scale.data_ptr(),
-             self.scale.shape[1], *self.shape, out.data_ptr(), stream)
+        data, scale, cols = self.data, self.scale, self.cols
+        rows, device = data.shape[0], data.device
+        stream = _lib.stream_handle(device)
+        out = torch.empty(rows, cols, dtype=torch.float32, device=device)
+        call(device, "dionw_float4_values", data.data_ptr(), scale.data_ptr(), scale.shape[1], rows, cols,
+             out.data_ptr(), stream)
         return out
 
 
 def empty(rows: int, cols: int, device: torch.device) -> Float4Matrix:
-    depth = depth_of(cols)
-    return Float4Matrix(
-        torch.empty(rows, depth // 2, dtype=torch.uint8, device=device),
-        torch.empty(depth // BLOCK, -(-rows // 16) * 16, dtype=torch.uint8, device=device), cols)
+    """An unwritten matrix: its parts fit each other, so that nothing is checked."""
+    depth = -(-cols // STAGE) * STAGE
+    q = object.__new__(Float4Matrix)
+    put = object.__setattr__
+    put(q, "data", torch.empty(rows, depth // 2, dtype=torch.uint8, device=device))
+    put(q, "scale", torch.empty(depth // BLOCK, -(-rows // 16) * 16, dtype=torch.uint8, device=device))
+    put(q, "cols", cols)
+    return q
 
 
 def _readable(x: Tensor) -> Tensor:
@@ -151,15 +157,15 @@ def _quantize(x: Tensor, tiles: bool, seed: int | Tensor | None,
     m, n = x.shape
     stream = _lib.stream_handle(device)
     number, address = (0, None) if seed is None else _seed(seed, device)
-    by_row = empty(m, n, device)
-    by_column = empty(n, m, device) if both else None
-
-    def place(q: Float4Matrix | None) -> tuple[Any, ...]:
-        return (None, None, 0) if q is None else (q.data.data_ptr(), q.scale.data_ptr(), q.scale.shape[1])
-
+    by_row, by_column = empty(m, n, device), None
+    data, scale = by_row.data, by_row.scale
+    transpose: tuple[Any, ...] = None, None, 0
+    if both:
+        by_column = empty(n, m, device)
+        transpose = by_column.data.data_ptr(), by_column.scale.data_ptr(), by_column.scale.shape[1]
     rounding = _TILES if tiles else _NEAREST if seed is None else _STOCHASTIC
     call(device, "dionw_float4_quantize", CODES[x.dtype], x.data_ptr(), m, n, pitch(x), rounding, number,
-         address, *place(by_row), *place(by_column), stream)
+         address, data.data_ptr(), scale.data_ptr(), scale.shape[1], *transpose, stream)
     return by_row, by_column
 
 
@@ -177,7 +183,7 @@ def float4_quantize(x: Tensor, *, tiles: bool = False, seed: int | Tensor | None
         ValueError: For another shape or type, a tensor off the GPU, both ``tiles`` and a seed, or a
             call that ``torch.jit.trace`` or ``make_fx`` records.
     """
-    return _quantize(x.detach(), tiles, seed, False)[0]
+    return _quantize(x, tiles, seed, False)[0]
 
 
 def float4_quantize_both(x: Tensor, *, tiles: bool = False,
@@ -189,7 +195,7 @@ def float4_quantize_both(x: Tensor, *, tiles: bool = False,
     Raises:
         ValueError: As ``float4_quantize``.
     """
-    by_row, by_column = _quantize(x.detach(), tiles, seed, True)
+    by_row, by_column = _quantize(x, tiles, seed, True)
     return by_row, by_column
 
 
@@ -205,21 +211,23 @@ def float4_matmul(a: Float4Matrix, b: Float4Matrix, bias: Tensor | None = None, 
     """
     if watched():
         check_unrecorded(bias)
-    m, n, device = a.shape[0], b.shape[0], a.device
-    if a.cols != b.cols or device != b.device:
+    a_data, a_scale, b_data, b_scale = a.data, a.scale, b.data, b.scale
+    m, n, device = a_data.shape[0], b_data.shape[0], a_data.device
+    if a.cols != b.cols or device != b_data.device:
         raise ValueError(f"float4_matmul takes matrices of one depth on one device, got {a.shape} on "
                          f"{device} and {b.shape} on {b.device}")
-    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
-        raise ValueError("float4_matmul gives its bias no gradient: pass it detached, or use "
-                         "float4_linear on the float weight")
-    bias = float_bias(bias, n, device)
-    code, depth = _lib.elem_code(dtype), depth_of(a.cols)
+    if bias is not None:
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError("float4_matmul gives its bias no gradient: pass it detached, or use "
+                             "float4_linear on the float weight")
+        bias = float_bias(bias, n, device)
+    code, depth = _lib.elem_code(dtype), 2 * a_data.shape[1]
     stream = _lib.stream_handle(device)
     out = torch.empty(m, n, dtype=dtype, device=device)
     size = _workspace(m, n, depth)
-    space = _scratch(size, device)
-    call(device, "dionw_float4_gemm", m, n, depth, a.data.data_ptr(), a.scale.data_ptr(), a.scale.shape[1],
-         b.data.data_ptr(), b.scale.data_ptr(), b.scale.shape[1], _lib.ptr(bias), code, out.data_ptr(), n,
+    space = _scratch(size, device) if size else None
+    call(device, "dionw_float4_gemm", m, n, depth, a_data.data_ptr(), a_scale.data_ptr(), a_scale.shape[1],
+         b_data.data_ptr(), b_scale.data_ptr(), b_scale.shape[1], _lib.ptr(bias), code, out.data_ptr(), n,
          _lib.ptr(space), size, stream)
     return out
 
