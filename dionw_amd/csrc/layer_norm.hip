@@ -14,7 +14,6 @@
 namespace dionw {
 namespace {
 
-constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;
 // Threads of a workgroup whose rows take LANES threads each: one row, or 256 threads of rows of a wave.
 constexpr int threads_of(int lanes) { return lanes > kWave ? lanes : 256; }
 
@@ -452,10 +451,14 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(JoinArgs g) {
 
 // ---- launches -----------------------------------------------------------------------------
 
+// A launch takes fewer than 2^32 threads.
+bool fits(int64_t groups, int threads) { return groups <= (int64_t)UINT32_MAX / threads; }
+
 template <typename T, int LANES, int K, bool CODES>
 int launch_norm(const NormArgs& g, hipStream_t stream) {
   constexpr int threads = threads_of(LANES);
   const int64_t grid = ceil_div(g.rows, threads / LANES);
+  DIONW_REQUIRE(fits(grid, threads), "layer_norm: too many rows");
   hipLaunchKernelGGL((norm_kernel<T, LANES, K, CODES>), dim3((unsigned)grid), dim3(threads), 0, stream, g);
   return check_launch("layer_norm");
 }
@@ -528,7 +531,8 @@ int check_norm(int32_t elem, const void* x, int64_t x_ld, int64_t rows, int64_t 
   DIONW_REQUIRE(rows >= 0 && cols > 0 && cols < INT32_MAX / 2, "layer_norm: bad extents %lld x %lld",
                 (long long)rows, (long long)cols);
   DIONW_REQUIRE(rows == 0 || (x && x_ld >= cols), "layer_norm: bad input");
-  DIONW_REQUIRE(rows <= kMostGroups, "layer_norm: too many rows");
+  // As many as their gradients' kernel takes too.
+  DIONW_REQUIRE(cols <= kWidest || fits(rows, kWide), "layer_norm: too many rows");
   return kOk;
 }
 

@@ -115,24 +115,30 @@ def test_the_library_checks_its_arguments() -> None:
                   mean, rstd, None)
 
     for bad in ({"elem": 3}, {"x": None}, {"x_ld": 199}, {"rows": -1}, {"cols": 0}, {"cols": 1 << 31},
-                {"w_elem": 3}, {"b_elem": -1}, {"y": None}, {"mean": None}, {"rstd": None}, {"rows": 1 << 24}):
+                {"w_elem": 3}, {"b_elem": -1}, {"y": None}, {"mean": None}, {"rstd": None}, {"rows": 1 << 26}):
         with pytest.raises(ValueError):
             forward(**bad)
+    # A launch takes fewer than 2^32 threads: 16 to 1024 of them take a row.
+    for rows, cols in ((1 << 28, 128), (1 << 26, 129), (1 << 26, 1024), (1 << 25, 2048), (1 << 24, 8192),
+                       (1 << 22, 8193), (1 << 22, 20000)):
+        with pytest.raises(ValueError, match="rows"):
+            forward(rows=rows, x_ld=cols, cols=cols)
 
     def quantized(elem=1, x_ld=200, rows=4, data=16, scale=16, scale_ld=16):
         _lib.call("dionw_layer_norm_float4", elem, 16, x_ld, rows, 200, 2, None, 2, None, 1e-5, data, scale,
                   scale_ld, None)
 
-    for bad in ({"elem": 3}, {"x_ld": 199}, {"data": None}, {"data": 8}, {"scale": None}, {"scale_ld": 3}):
+    for bad in ({"elem": 3}, {"x_ld": 199}, {"data": None}, {"data": 8}, {"scale": None}, {"scale_ld": 3},
+                {"rows": 1 << 26, "scale_ld": 1 << 26}):
         with pytest.raises(ValueError):
             quantized(**bad)
 
-    def backward(elem=1, dy=16, dy_ld=200, mean=16, rstd=16, dg=16, scratch=16, size=1 << 30):
-        _lib.call("dionw_layer_norm_backward", elem, 16, 200, dy, dy_ld, 4, 200, 2, None, mean, rstd, 16, dg, 2,
+    def backward(elem=1, dy=16, dy_ld=200, mean=16, rstd=16, dg=16, scratch=16, size=1 << 30, rows=4, cols=200):
+        _lib.call("dionw_layer_norm_backward", elem, 16, cols, dy, dy_ld, rows, cols, 2, None, mean, rstd, 16, dg, 2,
                   None, scratch, size, None)
 
     for bad in ({"elem": 3}, {"dy": None}, {"dy_ld": 199}, {"mean": None}, {"rstd": None}, {"scratch": None},
-                {"scratch": 18}, {"size": 1}):
+                {"scratch": 18}, {"size": 1}, {"rows": 1 << 22, "cols": 8193, "dy_ld": 8193}):
         with pytest.raises(ValueError):
             backward(**bad)
 

@@ -275,6 +275,103 @@ def test_another_stream_a_graph_and_repeats() -> None:
             assert all(torch.equal(p, q) for p, q in zip(out, train()))
 
 
+def test_more_rows_than_a_launch_has_workgroups_of_a_wave() -> None:
+    """2^24 rows and more, forward and backward and in 4 bits: the last ones are as they are alone."""
+    rows, last = (1 << 24) + 9, 25
+    x, g, b, dy = _inputs(last, 8, torch.float16)
+    big, up = torch.ones(rows, 8, dtype=torch.float16, device="cuda"), torch.zeros(rows, 8, dtype=torch.float16,
+                                                                                  device="cuda")
+    big[-last:], up[-last:] = x, dy
+    args, alone = [t.requires_grad_() for t in (big, g, b)], x.requires_grad_()
+    y, want = layer_norm(*args), layer_norm(alone, g, b)
+    assert torch.equal(y[-last:], want)
+    grads = torch.autograd.grad(y, args, up)
+    assert torch.equal(grads[0][-last:], torch.autograd.grad(want, alone, dy)[0])
+    _Exact(x, g, b).check_gradients(dy, None, grads[1], grads[2])  # the other rows add zeros
+    with torch.no_grad():
+        q, part = float4_layer_norm(big, g, b), float4_layer_norm(x, g, b)
+    assert torch.equal(q.data[-last:], part.data)
+    assert torch.equal(q.scale[:, rows - last:rows], part.scale[:, :last])
+
+
+def test_two_threads_at_once() -> None:
+    """Calls from two threads on streams of their own, forward and backward, give what they give in turn."""
+    from threading import Thread
+
+    def work(k):
+        x, g, b, dy = _inputs(130 + k, 700, torch.bfloat16, 30 + k)
+        w = _inputs(200, 700, torch.float32, 40 + k)[0]
+        args = [t.requires_grad_() for t in (x, g, b, w)]
+        kept = float4_quantize(w.detach(), tiles=True)
+        up = _inputs(130 + k, 200, torch.bfloat16, 50 + k)[0]
+        torch.cuda.current_stream().synchronize()
+        results = []
+        for _ in range(20):
+            y = float4_linear(layer_norm(*args[:3]), w, seed=7)
+            grads = torch.autograd.grad(y, args, up)
+            with torch.no_grad():
+                served = float4_matmul(float4_layer_norm(x, g, b), kept)
+                one = float4_linear(x[:3], kept)
+            results.append([y.detach(), *grads, served, one])
+        torch.cuda.current_stream().synchronize()
+        assert all(torch.equal(p, q) for r in results[1:] for p, q in zip(results[0], r))
+        found[k] = results[0]
+
+    def threaded(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            work(k)
+
+    found = {}
+    for k in range(2):
+        work(k)
+    want, found = found, {}
+    threads = [Thread(target=threaded, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert found.keys() == want.keys()
+    assert all(torch.equal(p, q) for k in want for p, q in zip(found[k], want[k]))
+
+
+def test_serving_in_a_graph() -> None:
+    """A prompt's norm in 4 bits, its product and single tokens' on kept weights, replayed on new rows."""
+    x, g, b, _ = _inputs(100, 700, torch.bfloat16)
+    kept = float4_quantize(_inputs(300, 700, torch.float32, 5)[0], tiles=True)
+
+    def serve():
+        with torch.no_grad():
+            q = float4_layer_norm(x, g, b)
+            return [float4_matmul(q, kept), q.values(), float4_linear(x, kept), float4_linear(x[:1], kept),
+                    float4_quantize(x, seed=4).values()]
+
+    serve()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = serve()
+    for k in range(4):
+        x.copy_(_inputs(100, 700, torch.bfloat16, 60 + k)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, serve()))
+
+
+@pytest.mark.parametrize("held", DTYPES)
+def test_parameters_at_odd_places(held) -> None:
+    """Parts of longer vectors, which begin between the places that wide loads prefer, and strided ones."""
+    for cols in (300, 1029, 8195):
+        x, g, b, dy = _inputs(9, cols, torch.bfloat16, held=held)
+        want = layer_norm(x, g, b)
+        for step in (1, 2):
+            places = slice(1, 1 + step * cols, step)
+            far = [torch.zeros(2 * cols + 2, dtype=held, device="cuda") for _ in range(2)]
+            far[0][places], far[1][places] = g, b
+            args = [t[places].detach().requires_grad_() for t in far]
+            y = layer_norm(x, *args)
+            assert torch.equal(y, want)
+            _Exact(x, g, b).check_gradients(dy, None, *torch.autograd.grad(y, args, dy))
+
+
 def test_rows_behind_the_last_are_left_alone() -> None:
     """Nothing is written past a matrix, whichever way its rows are spread over the GPU."""
     from dionw_amd import _lib
