@@ -15,8 +15,8 @@ namespace {
 // sums through LDS, in a fixed order. Of a stage, a lane holds one token's (or weight row's) two
 // blocks of 32, number G = lane / 16 and 4 + G: a block's scale and codes are its lane's own, without
 // an exchange. A wave reads the next stage while it multiplies one.
-// Bound: HBM, n k (1 / 2 + 1 / 32) bytes of W: 128256 x 4096 55 us, 5.0 TB/s; the smallest calls: launch
-// and the latency of two dependent reads.
+// Bound: HBM, n k (1 / 2 + 1 / 32) bytes of W: 128256 x 4096 51.4 us, 5.4 TB/s (reading the codes alone, in
+// this order, 45, from end to end 39); the smallest calls: launch and the latency of two dependent reads.
 constexpr int kFew = 16;
 bool few_rows(int64_t m, int64_t k) { return k > 0 && m <= kFew; }
 
@@ -97,81 +97,118 @@ __device__ __forceinline__ void multiply4(i32x4 b, i32x4 a, f32x4& c, uint32_t b
       __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4, B, (int)b_scale, 0, (int)a_scale);
 }
 
-template <typename T, int R, int W, bool WHOLE>
+// A workgroup takes P parts of 16 R rows of W, for which x is read and quantized once.
+template <typename T, int R, int P, int W, bool WHOLE>
 __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
-  __shared__ f32x4 sums[W][R][64];
+  __shared__ f32x4 sums[W][P][R][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int G = lane >> 4, i16 = lane & 15;
-  const int n0 = blockIdx.x * 16 * R, token = blockIdx.y * 16 + i16;
+  const int n0 = blockIdx.x * 16 * R * P, token = blockIdx.y * 16 + i16;
   const T* x = reinterpret_cast<const T*>(g.x) + min(token, g.m - 1) * g.x_ld + kBlock4 * G;
-  const uint8_t* w[R];
+  const uint8_t *w[P][R], *scale[P];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    w[r] = g.w + (int64_t)min(n0 + R * i16 + r, g.n - 1) * g.stages * 128 + 16 * G;
-  // A block's bytes run to a multiple of 16; words past the last belong to rows past it too.
-  const uint8_t* scale = g.w_scale + G * g.w_scale_ld + min((int64_t)n0 + R * i16, g.w_scale_ld - R);
+  for (int p = 0; p < P; ++p) {
+    const int n = n0 + 16 * R * p + R * i16;  // the lane's first row
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[p][r] = g.w + (int64_t)min(n + r, g.n - 1) * g.stages * 128 + 16 * G;
+    // A block's bytes run to a multiple of 16; words past the last belong to rows past it too.
+    scale[p] = g.w_scale + G * g.w_scale_ld + min((int64_t)n, g.w_scale_ld - R);
+  }
   using Word = std::conditional_t<R == 4, uint32_t, std::conditional_t<R == 2, uint16_t, uint8_t>>;
-  struct Stage {
-    Values<T> x[2];
+  struct Rows {  // a stage of a part's rows
     i32x4 w[R][2];
     uint32_t bytes[2];
   };
-  auto read = [&](Stage& s, int kt) {
+  auto read = [&](Rows& s, int kt, int p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        s.w[r][h] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w[r] + (int64_t)kt * 128 + 64 * h));
-      s.bytes[h] = *reinterpret_cast<const Word*>(scale + ((int64_t)kt * 8 + 4 * h) * g.w_scale_ld);
+        s.w[r][h] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w[p][r] + (int64_t)kt * 128 + 64 * h));
+      s.bytes[h] = *reinterpret_cast<const Word*>(scale[p] + ((int64_t)kt * 8 + 4 * h) * g.w_scale_ld);
     }
+  };
+  Values<T> v[2];  // x as it comes, and its codes and scales
+  i32x4 c[2];
+  uint32_t byte[2];
+  auto read_x = [&](int kt) {
     const int64_t at = (int64_t)kt * kDepth4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t left = g.k - at - 128 * h - kBlock4 * G;  // columns from the block's first one on
-      if (WHOLE || left >= kBlock4) s.x[h].load(x + at + 128 * h);
-      else s.x[h].load(x + at + 128 * h, left);
+      if (WHOLE || left >= kBlock4) v[h].load(x + at + 128 * h);
+      else v[h].load(x + at + 128 * h, left);
     }
   };
-  f32x4 acc[R];
+  f32x4 acc[P][R];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[r][e] = 0.f;
-  auto multiply = [&](Stage& s) {
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[p][r][e] = 0.f;
+  // Part p of stage kt, which `now` holds; what follows it is read into `next`. x goes out before the
+  // rows that are multiplied by it, so that it can be quantized while they are on their way.
+  auto part = [&](auto p_, int kt, const Rows& now, Rows& next) {
+    constexpr int p = decltype(p_)::value;
+    if constexpr (p + 1 < P) read(next, kt, p + 1);
+    if constexpr (p == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        byte[h] = scale_byte4<false>(v[h].most());
+        c[h] = v[h].codes(power(byte[h]));
+      }
+      if (kt + W < g.stages) read_x(kt + W);
+    }
+    if constexpr (p + 1 == P)
+      if (kt + W < g.stages) read(next, kt + W, 0);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t byte = scale_byte4<false>(s.x[h].most());
-      const i32x4 c = s.x[h].codes(power(byte));
-      multiply4<0>(s.w[0][h], c, acc[0], s.bytes[h], byte);
-      if constexpr (R > 1) multiply4<1>(s.w[1][h], c, acc[1], s.bytes[h], byte);
+      multiply4<0>(now.w[0][h], c[h], acc[p][0], now.bytes[h], byte[h]);
+      if constexpr (R > 1) multiply4<1>(now.w[1][h], c[h], acc[p][1], now.bytes[h], byte[h]);
       if constexpr (R > 2) {
-        multiply4<2>(s.w[2][h], c, acc[2], s.bytes[h], byte);
-        multiply4<3>(s.w[3][h], c, acc[3], s.bytes[h], byte);
+        multiply4<2>(now.w[2][h], c[h], acc[p][2], now.bytes[h], byte[h]);
+        multiply4<3>(now.w[3][h], c[h], acc[p][3], now.bytes[h], byte[h]);
       }
     }
   };
-  Stage a, b;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  static_assert(P == 1 || P == 2 || P == 4, "a stage's parts begin in the same registers");
+  Rows a, b;
   int kt = wave;
-  if (kt < g.stages) read(a, kt);
-  for (; kt < g.stages; kt += 2 * W) {
-    if (kt + W < g.stages) read(b, kt + W);
-    multiply(a);
-    if (kt + W >= g.stages) break;
-    if (kt + 2 * W < g.stages) read(a, kt + 2 * W);
-    multiply(b);
+  if (kt < g.stages) {
+    read_x(kt);
+    read(a, kt, 0);
+  }
+  for (; kt < g.stages; kt += W) {
+    part(I0{}, kt, a, b);
+    if constexpr (P == 1) {
+      kt += W;
+      if (kt < g.stages) part(I0{}, kt, b, a);
+    }
+    if constexpr (P > 1) part(I1{}, kt, b, a);
+    if constexpr (P > 2) {
+      part(I2{}, kt, a, b);
+      part(I3{}, kt, b, a);
+    }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r) sums[wave][r][lane] = acc[r];
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int r = 0; r < R; ++r) sums[wave][p][r][lane] = acc[p][r];
   __syncthreads();
-  // Value e of a lane's fragments: token i16, rows R (4 G + e) .. + R - 1 of W; a wave each.
-  for (int e = wave; e < 4; e += W) {
-    const int n = n0 + R * (4 * G + e);
+  // Value e of a lane's fragments: token i16, rows R (4 G + e) .. + R - 1 of a part; a wave each.
+  for (int i = wave; i < 4 * P; i += W) {
+    const int p = i / 4, e = i % 4, n = n0 + 16 * R * p + R * (4 * G + e);
     float s[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s[r] = sums[0][r][lane][e];
+      s[r] = sums[0][p][r][lane][e];
 #pragma unroll
-      for (int v = 1; v < W; ++v) s[r] += sums[v][r][lane][e];
+      for (int u = 1; u < W; ++u) s[r] += sums[u][p][r][lane][e];
     }
     if (token >= g.m || n >= g.n) continue;
     typedef T row __attribute__((ext_vector_type(R)));
@@ -190,25 +227,29 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
   }
 }
 
-// R rows' fragments a wave and W waves a workgroup: many fragments take 64 rows each (x is read and
-// quantized once for them, and a lane's four scale bytes are one load), few the most workgroups. us in
-// calls from Python (7.6 at least), R W = 1 8 / 2 4 / 4 4 / 4 2, bfloat16, a row of x: 4096 x 4096 7.7 /
-// 7.9 / 9.8 / 11.0, 4096 x 14336 12.2 / 16.8 / 25.7 / 30.5, 6144 x 4096 8.0 / 7.6 / 10.1 / 11.1, 8192 x 4096
-// 8.4 / 7.7 / 10.2 / 11.4, 14336 x 4096 12.8 / 11.4 / 10.8 / 11.8 (16 rows 22 / 15.8 / 12.4 / 13.9), 128256 x
-// 4096 77 / 61 / 55.5 / 57.9 (16 rows 155 / 102 / 75 / 78). float32 values take twice the registers, so
-// that fewer workgroups of 4 waves fit: 128256 x 4096 163 / 82 / 85 / 66.5 (16 rows 342 / 189 / 128 / 105).
-// The number of rows is not asked, so that a row's sums do not depend on the rows beside it.
-template <typename T, int R, int W, bool WHOLE>
+// Few fragments take the most workgroups, many the most rows each: x is read and quantized once for
+// them, with R = 4 a lane's four scale bytes are one load, and up to 1024 fragments 64 rows each, past
+// them 128 are at most one round of the GPU. us in calls from Python (7 at least), R P W = 1 1 8 /
+// 2 1 4 / 4 1 4 / 4 2 4 / 4 4 2, a row of bfloat16: 4096 x 4096 6.9 / 7.3 / 9.7 / 13.3 / 26, 4096 x 14336 11.3 / 16.7 /
+// 25.3, 8192 x 4096 8.0 / 7.7 / 10.0 / 13.6, 14336 x 4096 12.5 / 11.2 / 10.4 / 14.0, 20480 x 4096 15.6 / 14.9 / 16.0 /
+// 14.6 / 27 (16 rows 29 / 21.7 / 20.6 / 17.2 / 29), 128256 x 4096 77 / 62 / 54 / 51.4 / 53.7 (16 rows 164 / 101 /
+// 76 / 65 / 58). float32, whose values take twice the registers: 14336 x 4096 - / 13.3 / 11.0 / 15.8, 65536 x
+// 4096 - / 41 / 39 / 32 / 30 (16 rows 99 / 62 / 45 / 36), 128256 x 4096 163 / 76 / 75 / 62 / 55 (16 rows 356 / 188 / 119 /
+// 88 / 66). The number of x's rows is not asked, so that a row's sums do not depend on the rows beside it.
+template <typename T, int R, int P, int W, bool WHOLE>
 void launch_few(const FewArgs& g, int fragments, hipStream_t stream) {
-  hipLaunchKernelGGL((float4_few_kernel<T, R, W, WHOLE>), dim3((unsigned)(fragments + R - 1) / R, (unsigned)(g.m + 15) / 16),
-                     dim3(W * 64), 0, stream, g);
+  hipLaunchKernelGGL((float4_few_kernel<T, R, P, W, WHOLE>),
+                     dim3((unsigned)ceil_div(fragments, R * P), (unsigned)ceil_div(g.m, 16)), dim3(W * 64), 0, stream, g);
 }
 template <typename T, bool WHOLE>
 int launch_few(const FewArgs& g, hipStream_t stream) {
+  constexpr bool kLong = sizeof(T) == 4;  // float32 alone comes in the widest form
   const int fragments = (g.n + 15) / 16;
-  if (fragments < 320) launch_few<T, 1, 8, WHOLE>(g, fragments, stream);
-  else if (fragments <= 640) launch_few<T, 2, 4, WHOLE>(g, fragments, stream);
-  else launch_few<T, 4, sizeof(T) == 4 ? 2 : 4, WHOLE>(g, fragments, stream);
+  if (fragments < 320) launch_few<T, 1, 1, 8, WHOLE>(g, fragments, stream);
+  else if (fragments <= 640) launch_few<T, 2, 1, 4, WHOLE>(g, fragments, stream);
+  else if (fragments <= 1024) launch_few<T, 4, 1, 4, WHOLE>(g, fragments, stream);
+  else if (!kLong || fragments < 4096) launch_few<T, 4, 2, 4, WHOLE>(g, fragments, stream);
+  else if constexpr (kLong) launch_few<T, 4, 4, 2, WHOLE>(g, fragments, stream);
   return check_launch("float4_few");
 }
 

@@ -381,6 +381,20 @@ def test_a_kept_weight_serves(size, dtype) -> None:
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(2, 300, 5104), (3, 520, 5105), (1, 2400, 5121), (16, 257, 10240), (5, 1300, 10245),
+                                  (7, 700, 16384), (1, 256, 16385), (16, 1281, 16399), (9, 600, 33001),
+                                  (4, 1000, 65520), (16, 513, 65521), (2, 770, 70001), (1, 31, 131073)], ids=str)
+def test_a_few_rows_on_weights_of_many(size, dtype) -> None:
+    """Around the weight's rows at which the kernel's form changes, and past each form's workgroups;
+    whole and ragged depths, from one stage to more than every wave takes."""
+    m, k, n = size
+    x, w = _random(m, k, 10, dtype, 0.5), _random(n, k, 11, spread=0.3) * k ** -0.5
+    bias = torch.randn(n, device="cuda") if n % 2 else None
+    kept = float4_quantize(w, tiles=True)
+    _check(float4_linear(x, kept, bias), oracle.quantize(x)[0], kept.values().cpu().double(), bias)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_a_rows_output_does_not_depend_on_the_rows_beside_it(dtype) -> None:
     """Among the few rows that one launch serves."""
     x, w = _random(16, 3000, 10, dtype, 0.5), _random(700, 3000, 11, spread=0.3)
