@@ -202,7 +202,8 @@ __device__ __forceinline__ void quantize_tile(const QuantizeArgs& q, uint32_t ti
     }
   }
   __syncthreads();
-  if (q.sums && tid < kTile4 && c0 + tid < q.cols)
+  // Tiles past the last row, where the transpose is padded by more than one, have no sums.
+  if (q.sums && r0 < q.rows && tid < kTile4 && c0 + tid < q.cols)
     q.sums[r0 / kTile4 * q.cols + c0 + tid] = (shared.col_sum[0][tid] + shared.col_sum[1][tid]) +
                                               (shared.col_sum[2][tid] + shared.col_sum[3][tid]);
   // A block's bytes run to a multiple of 16: 4 of them a thread, the first 128 threads the rows'.

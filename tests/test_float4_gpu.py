@@ -8,6 +8,8 @@ more to the output's type.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -272,6 +274,37 @@ def test_the_layer_trains(size, dtype) -> None:
     _check(w.grad, oracle.quantize(dy.t(), 1, bits.t())[0], oracle.quantize(x.t())[0])
     exact = dy.double().sum(0)
     assert bool(((b.grad.double() - exact).abs() <= (m + 1) * 2.0 ** -24 * dy.double().abs().sum(0)).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 70, 128, 129, 257, 300, 520])
+def test_nothing_is_written_past_the_buffers(rows, dtype) -> None:
+    """Of both passes, whatever gradients are asked for: each buffer of exactly its size, and what lies
+    behind it stays."""
+    from itertools import product as every
+
+    from dionw_amd import _lib
+
+    n, k, code, guard = 200, 300, _lib.elem_code(dtype), 1 << 16
+    x, dy = _random(rows, k, 1, dtype), _random(rows, n, 2, dtype)
+    w, b = _random(n, k, 3), torch.randn(n, device="cuda")
+    stream = _lib.stream_handle(x.device)
+
+    def room(size):
+        return torch.full((size + guard,), 77, dtype=torch.uint8, device="cuda")
+
+    for need_x, need_w, need_b in every((0, 1), repeat=3):
+        sizes = (ctypes.c_size_t * 3)()
+        _lib.library().dionw_float4_linear_sizes(rows, n, k, need_x, need_w, need_b, sizes)
+        saved, forward, backward = map(room, sizes)
+        y, dx, dw, db = (room(size) for size in (x.itemsize * rows * n, x.itemsize * rows * k, 4 * n * k, 4 * n))
+        _lib.call("dionw_float4_linear_forward", code, x.data_ptr(), k, 2, w.data_ptr(), k, b.data_ptr(), rows, n, k,
+                  need_x, need_w, y.data_ptr(), saved.data_ptr(), forward.data_ptr(), sizes[1], stream)
+        _lib.call("dionw_float4_linear_backward", code, dy.data_ptr(), n, 2, rows, n, k, need_x, need_w, 5, None,
+                  saved.data_ptr(), dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, 2,
+                  db.data_ptr() if need_b else None, backward.data_ptr(), sizes[2], stream)
+        for buffer in (saved, forward, backward, y, dx, dw, db):
+            assert bool((buffer[-guard:] == 77).all())
 
 
 def test_gradients_are_right_on_average() -> None:

@@ -396,6 +396,24 @@ def test_rows_behind_the_last_are_left_alone() -> None:
         assert not (stats[:, :rows] == 77).any()
 
 
+def test_nothing_is_written_past_the_scratch_and_the_parameters_gradients() -> None:
+    from dionw_amd import _lib
+
+    for rows, cols in ((1, 1), (9, 100), (2500, 300), (5, 700), (70, 2048), (9, 6001), (70, 20001)):
+        x, g, b, dy = _inputs(rows, cols, torch.float32)
+        stats = torch.zeros(2, rows, device="cuda")
+        size = _lib.library().dionw_layer_norm_backward_scratch(rows, cols)
+        scratch, dx, dg, db = (torch.full((n // 4 + 9999,), 77.0, device="cuda")
+                               for n in (size, 4 * rows * cols, 4 * cols, 4 * cols))
+        for at in ((dg, db), (dg, None), (None, db)):
+            _lib.call("dionw_layer_norm_backward", 2, x.data_ptr(), cols, dy.data_ptr(), cols, rows, cols, 2, g.data_ptr(),
+                      stats[0].data_ptr(), stats[1].data_ptr(), dx.data_ptr(),
+                      None if at[0] is None else dg.data_ptr(), 2, None if at[1] is None else db.data_ptr(),
+                      scratch.data_ptr(), size, _lib.stream_handle(x.device))
+            for t in (scratch, dx, dg, db):
+                assert bool((t[-9999:] == 77).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [(1, 1), (3, 200), (100, 768), (70, 1500), (5, 2048), (600, 4096), (9, 6000),
                                   (2, 16000), (3, 20000), (1000, 256)], ids=str)
