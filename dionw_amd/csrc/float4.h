@@ -110,6 +110,31 @@ __device__ __forceinline__ uint32_t codes2(uint32_t old, float a, float b, float
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, a, b, scale, B);
 }
 
+// Codes of a row or a column of a Square times 1 / scale, to nearest.
+template <typename T>
+struct Codes {
+  using S = Square<T>;
+  template <int B>
+  __device__ __forceinline__ static uint32_t row_pair(uint32_t old, const S& v, int i, float scale) {
+    if constexpr (sizeof(T) == 4) return codes2<B>(old, v.value(i, 2 * B), v.value(i, 2 * B + 1), scale);
+    else return codes2<B>(old, v.w[i][B], scale, T{});
+  }
+  template <int B>
+  __device__ __forceinline__ static uint32_t col_pair(uint32_t old, const S& v, int k, float scale) {
+    if constexpr (sizeof(T) == 4)
+      return codes2<B>(old, v.value(2 * B, k), v.value(2 * B + 1, k), scale);
+    else
+      return codes2<B>(old, __builtin_amdgcn_perm(v.w[2 * B + 1][k >> 1], v.w[2 * B][k >> 1],
+                                                  k & 1 ? 0x07060302u : 0x05040100u), scale, T{});
+  }
+  __device__ __forceinline__ static uint32_t row(const S& v, int i, float scale) {
+    return row_pair<3>(row_pair<2>(row_pair<1>(row_pair<0>(0, v, i, scale), v, i, scale), v, i, scale), v, i, scale);
+  }
+  __device__ __forceinline__ static uint32_t col(const S& v, int k, float scale) {
+    return col_pair<3>(col_pair<2>(col_pair<1>(col_pair<0>(0, v, k, scale), v, k, scale), v, k, scale), v, k, scale);
+  }
+};
+
 // The largest over 4 adjacent lanes.
 __device__ __forceinline__ uint32_t largest_of_four(uint32_t v) {
   v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));

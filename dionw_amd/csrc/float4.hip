@@ -59,31 +59,7 @@ struct Shared {
   __attribute__((aligned(16))) uint8_t row_bytes[4][kTile4], col_bytes[4][kTile4];
 };
 
-template <typename T>
-struct Codes {
-  using S = Square<T>;
-  template <int B>
-  __device__ __forceinline__ static uint32_t row_pair(uint32_t old, const S& v, int i, float scale) {
-    if constexpr (sizeof(T) == 4) return codes2<B>(old, v.value(i, 2 * B), v.value(i, 2 * B + 1), scale);
-    else return codes2<B>(old, v.w[i][B], scale, T{});
-  }
-  template <int B>
-  __device__ __forceinline__ static uint32_t col_pair(uint32_t old, const S& v, int k, float scale) {
-    if constexpr (sizeof(T) == 4)
-      return codes2<B>(old, v.value(2 * B, k), v.value(2 * B + 1, k), scale);
-    else
-      return codes2<B>(old, __builtin_amdgcn_perm(v.w[2 * B + 1][k >> 1], v.w[2 * B][k >> 1],
-                                                  k & 1 ? 0x07060302u : 0x05040100u), scale, T{});
-  }
-  __device__ __forceinline__ static uint32_t row(const S& v, int i, float scale) {
-    return row_pair<3>(row_pair<2>(row_pair<1>(row_pair<0>(0, v, i, scale), v, i, scale), v, i, scale), v, i, scale);
-  }
-  __device__ __forceinline__ static uint32_t col(const S& v, int k, float scale) {
-    return col_pair<3>(col_pair<2>(col_pair<1>(col_pair<0>(0, v, k, scale), v, k, scale), v, k, scale), v, k, scale);
-  }
-};
-
-// The same by chance, from each value's bits at the top of a word. 16-bit values need no rounding of
+// Codes of a row or a column of a Square by chance, from each value's bits at the top of a word. 16-bit values need no rounding of
 // their own first: they are multiples of 2^-23 of the scale, but for those below 2^-12 of it, which the
 // noise's last 2^-10 alone could tell apart.
 template <typename T, typename V, typename N>

@@ -9,16 +9,25 @@ namespace {
 
 // ---- a few rows ----------------------------------------------------------------------
 //
-// y = x W^T + b for 16 rows of x at a time (the tokens being decoded): every byte of W passes
-// once, from memory to registers, and x is quantized on the way, so that the call is one launch.
-// A workgroup takes 16 R rows of W; its waves take the stages of 256 columns in turn and add their
-// sums through LDS, in a fixed order. Of a stage, a lane holds one token's (or weight row's) two
-// blocks of 32, number G = lane / 16 and 4 + G: a block's scale and codes are its lane's own, without
-// an exchange. A wave reads the next stage while it multiplies one.
-// Bound: HBM, n k (1 / 2 + 1 / 32) bytes of W: 128256 x 4096 51.4 us, 5.4 TB/s (reading the codes alone, in
+// y = x W^T + b for up to 16 rows of x (the tokens being decoded): every byte of W passes once, from
+// memory to registers, and x is quantized on the way, so that the call is one launch. A workgroup takes
+// 16 R P rows of W; its waves take the stages of 256 columns in turn and add their sums through LDS, in a
+// fixed order. Of a stage, a lane holds one token's (or weight row's) two blocks of 32, number G = lane / 16
+// and 4 + G: a block's scale and codes of W are its lane's own, as they lie in memory. x is read two rows a load and
+// its codes change lanes through LDS (read as they are needed, 128 bytes a lane apart, 8 rows took 25.6 us
+// where now 15.9: 4096 x 14336, float32). A wave reads the next rows while it multiplies the last ones.
+// Bound: HBM, n k (1 / 2 + 1 / 32) bytes of W: 128256 x 4096 50.1 us, 5.6 TB/s (reading the codes alone, in
 // this order, 45, from end to end 39); the smallest calls: launch and the latency of two dependent reads.
-constexpr int kFew = 16;
-bool few_rows(int64_t m, int64_t k) { return k > 0 && m <= kFew; }
+constexpr int kFewFragments = 320, kManyFragments = 1024;  // of 16 rows of W, where the kernel's form changes
+int fragments_of(int64_t n) { return (int)((n + 15) / 16); }
+// Past 8 rows x costs the kernel as much as W where it is deep, or W's rows are in the middle: quantizing
+// first and the product on tiles is faster there. 16 rows, us, here and there: 4096 x 4096 7.5 / 11.1, 8192 x 4096
+// 11.2 / 11.2, 14336 x 4096 14.2 / 11.9, 28672 x 4096 16.5 / 19, 4096 x 14336 16.6 / 14.2, 16384 x 14336 40 / 27; 8 rows 8.9 /
+// 11.2 on 8192 x 4096, 11.0 / 12.0 on 14336 x 4096, 12.8 / 14.7 on 4096 x 14336, 33 / 34 on 16384 x 14336.
+bool few_rows(int64_t m, int64_t n, int64_t k) {
+  const bool middle = fragments_of(n) >= kFewFragments && fragments_of(n) <= kManyFragments;
+  return k > 0 && (m <= 8 || (m <= 16 && k <= 4096 && !middle));
+}
 
 struct FewArgs {
   const void* x;
@@ -32,62 +41,20 @@ struct FewArgs {
   int32_t m, n, stages;
 };
 
-// A token's block of 32 as it lies in memory, and its codes.
+// The float32 bits of the largest magnitude of a Square's row.
 template <typename T>
-struct Values {
-  static constexpr int kWords = 8 * sizeof(T);
-  uint32_t w[kWords];
-  __device__ __forceinline__ void load(const T* at) {
+__device__ __forceinline__ uint32_t most_of(const Square<T>& v, int i) {
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int v = 0; v < kWords / 4; ++v) {
-      const u32x4 r = *reinterpret_cast<const u32x4_any*>(at + 16 / sizeof(T) * v);
+    for (int k = 0; k < 8; ++k) m = max(m, v.w[i][k] & 0x7FFFFFFFu);
+    return m;
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[4 * v + e] = r[e];
-    }
+    for (int k = 0; k < 4; ++k) m = Square<T>::larger(m, v.w[i][k] & 0x7FFF7FFFu);
+    return Pair<T>::bits(max(m & 0xFFFFu, m >> 16));
   }
-  // Zeros from the `left`th value on.
-  __device__ __forceinline__ void load(const T* at, int64_t left) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) w[e] = e < left ? __float_as_uint(at[e]) : 0u;
-    } else {
-      const uint16_t* u = reinterpret_cast<const uint16_t*>(at);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint32_t lo = 2 * e < left ? u[2 * e] : 0, hi = 2 * e + 1 < left ? u[2 * e + 1] : 0;
-        w[e] = lo | hi << 16;
-      }
-    }
-  }
-  // The float32 bits of the largest magnitude.
-  __device__ __forceinline__ uint32_t most() const {
-    uint32_t m = 0;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
-      return m;
-    } else {
-      using P = Pair<T>;
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) m = P::larger(m, w[i] & 0x7FFF7FFFu);
-      return P::bits(max(m & 0xFFFFu, m >> 16));
-    }
-  }
-  template <int B>
-  __device__ __forceinline__ uint32_t pair(uint32_t old, int i, float scale) const {
-    if constexpr (sizeof(T) == 4)
-      return codes2<B>(old, __uint_as_float(w[8 * i + 2 * B]), __uint_as_float(w[8 * i + 2 * B + 1]), scale);
-    else
-      return codes2<B>(old, w[4 * i + B], scale, T{});
-  }
-  __device__ __forceinline__ i32x4 codes(float scale) const {
-    i32x4 c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c[i] = (int)pair<3>(pair<2>(pair<1>(pair<0>(0, i, scale), i, scale), i, scale), i, scale);
-    return c;
-  }
-};
+}
 
 // c += b a^T; b's scale is byte B of its word.
 template <int B>
@@ -101,10 +68,13 @@ __device__ __forceinline__ void multiply4(i32x4 b, i32x4 a, f32x4& c, uint32_t b
 template <typename T, int R, int P, int W, bool WHOLE>
 __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
   __shared__ f32x4 sums[W][P][R][64];
+  // A wave's stage of x: codes, at a pitch that spreads 16 rows' reads over the banks, and scales.
+  constexpr int kPitch = 36;
+  __shared__ __attribute__((aligned(16))) uint32_t x_codes[W][16][kPitch];
+  __shared__ uint8_t x_bytes[W][16][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int G = lane >> 4, i16 = lane & 15;
-  const int n0 = blockIdx.x * 16 * R * P, token = blockIdx.y * 16 + i16;
-  const T* x = reinterpret_cast<const T*>(g.x) + min(token, g.m - 1) * g.x_ld + kBlock4 * G;
+  const int n0 = blockIdx.x * 16 * R * P, token0 = blockIdx.y * 16, rows = min(16, g.m - token0);
   const uint8_t *w[P][R], *scale[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -128,17 +98,41 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
       s.bytes[h] = *reinterpret_cast<const Word*>(scale[p] + ((int64_t)kt * 8 + 4 * h) * g.w_scale_ld);
     }
   };
-  Values<T> v[2];  // x as it comes, and its codes and scales
+  // x as it comes, two rows a load: a lane holds 8 columns of row 2 j + lane / 32.
+  const int upper = lane >> 5, eight = lane & 31;
+  const T* x = reinterpret_cast<const T*>(g.x) + token0 * g.x_ld + 8 * eight;
+  Square<T> v;
+  auto read_x = [&](int kt) {
+    const int64_t at = (int64_t)kt * kDepth4, left = g.k - at - 8 * eight;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (2 * j >= rows) break;
+      const T* from = x + at + (2 * j + (2 * j + 1 < rows ? upper : 0)) * g.x_ld;
+      if (WHOLE || left >= 8) v.load(j, from);
+      else v.load(j, from, left);
+    }
+  };
+  // Its codes and scales, a lane's own two blocks of row i16: through LDS, in the wave's own part, so that
+  // no one is waited for. Rows past the last are whatever lies there: their sums are not stored.
   i32x4 c[2];
   uint32_t byte[2];
-  auto read_x = [&](int kt) {
-    const int64_t at = (int64_t)kt * kDepth4;
+  auto quantize = [&] {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (2 * j >= rows) break;
+      const uint32_t b = scale_byte4<false>(largest_of_four(most_of(v, j)));
+      x_codes[wave][2 * j + upper][eight] = Codes<T>::row(v, j, power(b));
+      if (eight % 4 == 0) x_bytes[wave][2 * j + upper][eight / 4] = (uint8_t)b;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int64_t left = g.k - at - 128 * h - kBlock4 * G;  // columns from the block's first one on
-      if (WHOLE || left >= kBlock4) v[h].load(x + at + 128 * h);
-      else v[h].load(x + at + 128 * h, left);
+      c[h] = *reinterpret_cast<const i32x4*>(&x_codes[wave][i16][4 * (4 * h + G)]);
+      byte[h] = x_bytes[wave][i16][4 * h + G];
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   };
   f32x4 acc[P][R];
 #pragma unroll
@@ -153,11 +147,7 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
     constexpr int p = decltype(p_)::value;
     if constexpr (p + 1 < P) read(next, kt, p + 1);
     if constexpr (p == 0) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        byte[h] = scale_byte4<false>(v[h].most());
-        c[h] = v[h].codes(power(byte[h]));
-      }
+      quantize();
       if (kt + W < g.stages) read_x(kt + W);
     }
     if constexpr (p + 1 == P)
@@ -210,13 +200,13 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
 #pragma unroll
       for (int u = 1; u < W; ++u) s[r] += sums[u][p][r][lane][e];
     }
-    if (token >= g.m || n >= g.n) continue;
+    if (i16 >= rows || n >= g.n) continue;
     typedef T row __attribute__((ext_vector_type(R)));
     typedef T anywhere __attribute__((ext_vector_type(R), aligned(sizeof(T))));
     row o;
 #pragma unroll
     for (int r = 0; r < R; ++r) o[r] = (T)(s[r] + (g.bias ? g.bias[min(n + r, g.n - 1)] : 0.f));
-    T* y = reinterpret_cast<T*>(g.y) + (int64_t)token * g.n + n;
+    T* y = reinterpret_cast<T*>(g.y) + (int64_t)(token0 + i16) * g.n + n;
     if (n + R <= g.n) {
       *reinterpret_cast<anywhere*>(y) = o;
     } else {
@@ -228,14 +218,13 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
 }
 
 // Few fragments take the most workgroups, many the most rows each: x is read and quantized once for
-// them, with R = 4 a lane's four scale bytes are one load, and up to 1024 fragments 64 rows each, past
-// them 128 are at most one round of the GPU. us in calls from Python (7 at least), R P W = 1 1 8 /
-// 2 1 4 / 4 1 4 / 4 2 4 / 4 4 2, a row of bfloat16: 4096 x 4096 6.9 / 7.3 / 9.7 / 13.3 / 26, 4096 x 14336 11.3 / 16.7 /
-// 25.3, 8192 x 4096 8.0 / 7.7 / 10.0 / 13.6, 14336 x 4096 12.5 / 11.2 / 10.4 / 14.0, 20480 x 4096 15.6 / 14.9 / 16.0 /
-// 14.6 / 27 (16 rows 29 / 21.7 / 20.6 / 17.2 / 29), 128256 x 4096 77 / 62 / 54 / 51.4 / 53.7 (16 rows 164 / 101 /
-// 76 / 65 / 58). float32, whose values take twice the registers: 14336 x 4096 - / 13.3 / 11.0 / 15.8, 65536 x
-// 4096 - / 41 / 39 / 32 / 30 (16 rows 99 / 62 / 45 / 36), 128256 x 4096 163 / 76 / 75 / 62 / 55 (16 rows 356 / 188 / 119 /
-// 88 / 66). The number of x's rows is not asked, so that a row's sums do not depend on the rows beside it.
+// them, and with R = 4 a lane's four scale bytes are one load. us in calls from Python (7 at least), R P W = 1 1 8 /
+// 2 1 4 / 4 1 4 / 4 2 4 / 4 4 2, a row of bfloat16: 4096 x 4096 7.4 / 7.4 / 9.8 / 13.1 / 25.7, 4096 x 14336 9.9 / 16.0 /
+// 24 / 41, 8192 x 4096 7.5 / 7.5 / 10.1 / 13.4, 14336 x 4096 11.0 / 9.4 / 10.6 / 13.7, 20480 x 4096 13.4 / 13.2 /
+// 15.7 / 14.3 / 27 (8 rows 17.1 / 15.6 / 17.3 / 14.9 / 28.6), 128256 x 4096 64 / 54 / 52.6 / 50.2 / 51.7 (8 rows 87 / 70 / 62 /
+// 55.3 / 53.2); float32: 65536 x 4096 48 / 31.5 / 29.4 / 28.3 / 29.2 (8 rows 70 / 44 / 36.8 / 31.8 / 31.8), 128256 x 4096
+// 91 / 56 / 53.5 / 55.0 / 53.2 (8 rows 135 / 84 / 70 / 63.6 / 56.2). The number of x's rows is not asked, so that a
+// row's sums do not depend on the rows beside it.
 template <typename T, int R, int P, int W, bool WHOLE>
 void launch_few(const FewArgs& g, int fragments, hipStream_t stream) {
   hipLaunchKernelGGL((float4_few_kernel<T, R, P, W, WHOLE>),
@@ -244,10 +233,9 @@ void launch_few(const FewArgs& g, int fragments, hipStream_t stream) {
 template <typename T, bool WHOLE>
 int launch_few(const FewArgs& g, hipStream_t stream) {
   constexpr bool kLong = sizeof(T) == 4;  // float32 alone comes in the widest form
-  const int fragments = (g.n + 15) / 16;
-  if (fragments < 320) launch_few<T, 1, 1, 8, WHOLE>(g, fragments, stream);
-  else if (fragments <= 640) launch_few<T, 2, 1, 4, WHOLE>(g, fragments, stream);
-  else if (fragments <= 1024) launch_few<T, 4, 1, 4, WHOLE>(g, fragments, stream);
+  const int fragments = fragments_of(g.n);
+  if (fragments < kFewFragments) launch_few<T, 1, 1, 8, WHOLE>(g, fragments, stream);
+  else if (fragments <= kManyFragments) launch_few<T, 2, 1, 4, WHOLE>(g, fragments, stream);
   else if (!kLong || fragments < 4096) launch_few<T, 4, 2, 4, WHOLE>(g, fragments, stream);
   else if constexpr (kLong) launch_few<T, 4, 4, 2, WHOLE>(g, fragments, stream);
   return check_launch("float4_few");
@@ -393,7 +381,7 @@ int dionw_float4_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
 }
 
 size_t dionw_float4_linear_kept_scratch(int64_t m, int64_t n, int64_t k) {
-  if (few_rows(m, k)) return 0;
+  if (few_rows(m, n, k)) return 0;
   Parts room{nullptr};
   const Matrix4 x = codes_in(room, m, k);
   room.take(dionw_float4_gemm_workspace(m, n, x.depth));
@@ -412,7 +400,7 @@ int dionw_float4_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const 
   DIONW_REQUIRE(x_ld >= k && aligned16(w) && w_scale_ld >= n && w_scale_ld % 16 == 0 && aligned16(w_scale) &&
                     aligned16(scratch),
                 "float4_linear: an operand is too small or not aligned");
-  if (few_rows(m, k)) {
+  if (few_rows(m, n, k)) {
     DIONW_REQUIRE(depth / kDepth4 < INT32_MAX / 16, "float4_linear: depth too large");
     const FewArgs g{x, x_ld, static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(w_scale),
                     w_scale_ld, bias, y, k, (int32_t)m, (int32_t)n, (int32_t)(depth / kDepth4)};

@@ -483,8 +483,9 @@ int dionw_float4_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
                                  size_t scratch_bytes, dionw_stream_t stream);
 
 /*
- * The same y from a kept W: codes [n] rows with their scales [depth / 32][w_scale_ld]. Up to 16 rows
- * of x are quantized by the product itself, in one launch and no scratch.
+ * The same y from a kept W: codes [n] rows with their scales [depth / 32][w_scale_ld]. Up to 8 rows
+ * of x (16 of up to 4096 columns, but for 5105 to 16384 rows of W) are quantized by the product itself,
+ * in one launch and no scratch.
  */
 size_t dionw_float4_linear_kept_scratch(int64_t m, int64_t n, int64_t k);
 int dionw_float4_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const void* w,
