@@ -343,7 +343,7 @@ int dionw_float4_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int
                                 hipStream_t stream) {
   DIONW_REQUIRE(good_elem(x_elem) && good_elem(w_elem), "float4_linear: bad element type");
   DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0, "float4_linear: negative extent");
-  DIONW_REQUIRE(saved || !(need_x || need_w) || n == 0 || k == 0, "float4_linear: no room to save");
+  DIONW_REQUIRE(saved || !(need_x || need_w) || m == 0 || n == 0 || k == 0, "float4_linear: no room to save");
   // The gradients sum over n and m: refused here rather than after the forward pass.
   DIONW_REQUIRE(fits_row(k) && (!need_x || fits_row(n)) && (!need_w || fits_row(m)),
                 "float4_linear: the products take rows of less than 8 MB");
@@ -352,6 +352,7 @@ int dionw_float4_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int
   Saved s(kept, m, n, k, need_x, need_w);
   Forward f(room, m, n, k);
   DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float4_linear: scratch too small");
+  if (m == 0) return kOk;  // y and dx are empty, dW and db sums of nothing: nothing that is saved is read
   DIONW_TRY(quantize4_pair({x_elem, x, m, k, x_ld, f.x, s.xt, nullptr},
                            {w_elem, w, n, k, w_ld, f.w, s.wt, nullptr}, stream));
   return product(f.x, f.w, bias, x_elem, y, f.product, f.product_bytes, stream);

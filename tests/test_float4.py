@@ -199,3 +199,14 @@ def test_sizes_follow_the_formats() -> None:
     assert sizes[2] >= matrix(100, 300) + matrix(300, 100) + padded(300 * 4)
     _lib.library().dionw_float4_linear_sizes(100, 300, 500, 0, 0, 0, sizes)
     assert sizes[0] == 0
+
+
+@pytest.mark.parametrize("need_x", [0, 1])
+@pytest.mark.parametrize("need_w", [0, 1])
+def test_a_forward_of_no_rows_needs_no_room_to_save(need_x, need_w) -> None:
+    """An expert that gets no tokens: y is empty, no gradient reads what would be saved, and nothing is launched."""
+    sizes = (ctypes.c_size_t * 3)()
+    _lib.library().dionw_float4_linear_sizes(0, 50, 130, need_x, need_w, 1, sizes)
+    assert need_x or sizes[0] == 0
+    _lib.call("dionw_float4_linear_forward", 1, None, 130, 2, 16, 130, None, 0, 50, 130, need_x, need_w, None,
+              16 if sizes[0] else None, 16, sizes[1], None)
