@@ -354,7 +354,7 @@ int dionw_float8_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int
                                 hipStream_t stream) {
   DIONW_REQUIRE(good_elem(x_elem) && good_elem(w_elem), "float8_linear: bad element type");
   DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0, "float8_linear: negative extent");
-  DIONW_REQUIRE(saved || !(need_x || need_w) || n == 0 || k == 0, "float8_linear: no room to save");
+  DIONW_REQUIRE(saved || !(need_x || need_w) || m == 0 || n == 0 || k == 0, "float8_linear: no room to save");
   // The gradients sum over n and m: refused here rather than after the forward pass.
   DIONW_REQUIRE((!need_x || fits_row(n, x_elem)) && (!need_w || fits_row(m, w_elem)),
                 "float8_linear: a gradient's product takes rows of less than 8 MB");
@@ -364,6 +364,7 @@ int dionw_float8_linear_forward(int32_t x_elem, const void* x, int64_t x_ld, int
   Saved s(kept, m, n, k, need_x, need_w);
   Forward f(room, exact, m, n, k);
   DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float8_linear: scratch too small");
+  if (m == 0) return kOk;  // y and dx are empty, dW and db sums of nothing: nothing that is saved is read
   DIONW_TRY(quantize_pair({x_elem, x, m, k, x_ld, f.x, s.xt, nullptr},
                           {w_elem, w, n, k, w_ld, f.w, s.wt, nullptr}, stream));
   return product(exact, f.x, f.w, bias, x_elem, y, f.product, f.product_bytes, stream);
@@ -383,8 +384,10 @@ int dionw_float8_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
   Backward b(room, exact_x, exact_w, m, n, k, need_x, need_w, db != nullptr);
   DIONW_REQUIRE(room.used <= scratch_bytes && (scratch || room.used == 0), "float8_linear: scratch too small");
   DIONW_REQUIRE(saved || kept.used == 0, "float8_linear: nothing was saved");
-  DIONW_TRY(quantize_and_expand({x_elem, dy, m, n, dy_ld, b.rows, b.cols, b.sums}, {s.wt, s.xt},
-                                {b.wt, b.xt}, stream));
+  if (m > 0) {
+    DIONW_TRY(quantize_and_expand({x_elem, dy, m, n, dy_ld, b.rows, b.cols, b.sums}, {s.wt, s.xt},
+                                  {b.wt, b.xt}, stream));
+  }
   if (need_x) {
     DIONW_TRY(product(exact_x, b.rows, exact_x ? b.wt : s.wt, nullptr, x_elem, dx, b.product,
                       b.product_bytes, stream));

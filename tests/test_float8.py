@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -122,3 +124,15 @@ def test_a_forward_refuses_what_its_gradients_could_not_sum() -> None:
             forward(*bad)
     with pytest.raises(ValueError, match="scratch"):
         forward(1 << 22, 4, 1, 0, 1)
+
+
+@pytest.mark.parametrize("elem", [1, 2])
+@pytest.mark.parametrize("need_x", [0, 1])
+@pytest.mark.parametrize("need_w", [0, 1])
+def test_a_forward_of_no_rows_needs_no_room_to_save(need_x, need_w, elem) -> None:
+    """An expert that gets no tokens: y is empty, no gradient reads what would be saved, and nothing is launched."""
+    sizes = (ctypes.c_size_t * 3)()
+    _lib.library().dionw_float8_linear_sizes(elem, 2, 0, 50, 130, need_x, need_w, 1, sizes)
+    assert need_x or sizes[0] == 0
+    _lib.call("dionw_float8_linear_forward", elem, None, 130, 2, 16, 130, None, 0, 50, 130, need_x, need_w, None,
+              16 if sizes[0] else None, 16, sizes[1], None)

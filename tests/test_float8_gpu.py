@@ -270,6 +270,20 @@ def test_empty_extents() -> None:
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("held", [torch.bfloat16, torch.float32])
+def test_no_rows_of_an_input_without_a_gradient(dtype, held) -> None:
+    """Whichever of weight and bias are trained: their gradients are zeros, in their own types."""
+    x = torch.zeros(0, 130, dtype=dtype, device="cuda")
+    for mask in range(1, 4):
+        w, b = _random(50, 130, 2).to(held), torch.randn(50, device="cuda")
+        trained = [t.requires_grad_() for i, t in enumerate((w, b)) if mask >> i & 1]
+        y = float8_linear(x, w, b)
+        assert y.shape == (0, 50) and y.dtype is dtype
+        for t, g in zip(trained, torch.autograd.grad(y, trained, torch.zeros_like(y))):
+            assert g.shape == t.shape and g.dtype is t.dtype and not g.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("size", [(1, 64, 64), (1, 4096, 1024), (3, 1000, 99), (8, 4096, 336), (16, 14336, 128),
                                   (17, 640, 77), (40, 5000, 100), (100, 2048, 1031), (1, 200, 20000)], ids=str)
 def test_a_kept_weight_serves(size, dtype) -> None:
