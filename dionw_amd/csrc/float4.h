@@ -59,14 +59,18 @@ __device__ __forceinline__ uint32_t noise_key(const Noise& n) {
   const uint64_t seed = n.at ? (uint64_t)*n.at : (uint64_t)n.seed;
   return mix32((uint32_t)seed + 0x9E3779B1u * ((uint32_t)(seed >> 32) + 1u));
 }
-// x / scale, below 1 rounded to a multiple of 2^-23: what lies below the last place kept is then a
-// multiple of 2^-22 of it, like the noise.
+// x / scale (6 at most), below 1 rounded to a multiple of 2^-23: what lies below the last place kept is
+// then a multiple of 2^-22 of it, like the noise. float32: 1 is added and taken off. 16 bits: 1.5, whatever
+// the sign and size, which takes an instruction less: a magnitude below 0.5 gives a sum from 1 to 2, whose last
+// place is 2^-23 (1.5 is an even multiple of it, so that ties go where they belong); a larger one is a
+// multiple of 2^-11 and stays exact in a sum below 8.
+template <typename T>
 __device__ __forceinline__ float scaled4(float x, float scale, float inverse) {
-  const float one = __builtin_copysignf(fabsf(x) < scale ? 1.f : 0.f, x);
+  const float one = sizeof(T) < 4 ? 1.5f : __builtin_copysignf(fabsf(x) < scale ? 1.f : 0.f, x);
   return __builtin_fmaf(x, inverse, one) - one;
 }
 
-// Codes of eight values times 1 / scale, rounded up by chance: `noise` holds each value's bits at the
+// Codes of eight scaled values, rounded up by chance: `noise` holds each value's bits at the
 // top of a word. The instruction takes two values and adds to the first one's part below the last
 // place kept its third operand / 2^32 of that place, to the second's the same word turned left by
 // one bit, and drops what is left of both; values below 1 lose what is below 2^-23 first (measured
@@ -76,7 +80,7 @@ __device__ __forceinline__ float scaled4(float x, float scale, float inverse) {
 // `odd`. In assembly, as the builtin leaves out that the destination's other bytes are kept; a
 // byte's write needs one more instruction before the next one that keeps it, which the two words'
 // turns are.
-__device__ __forceinline__ uint32_t noisy8(const f32x2 (&p)[4], const uint32_t (&noise)[8], float scale) {
+__device__ __forceinline__ uint32_t noisy8(const f32x2 (&p)[4], const uint32_t (&noise)[8]) {
   uint32_t even = 0, odd = 0;
 #ifdef __HIP_DEVICE_COMPILE__
   asm("v_cvt_scalef32_sr_pk_fp4_f32 %0, %2, %6, %14\n\t"
@@ -90,7 +94,7 @@ __device__ __forceinline__ uint32_t noisy8(const f32x2 (&p)[4], const uint32_t (
       "s_nop 0"
       : "=&v"(even), "=&v"(odd)
       : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(noise[0]), "v"(noise[1] >> 1), "v"(noise[2]),
-        "v"(noise[3] >> 1), "v"(noise[4]), "v"(noise[5] >> 1), "v"(noise[6]), "v"(noise[7] >> 1), "v"(scale));
+        "v"(noise[3] >> 1), "v"(noise[4]), "v"(noise[5] >> 1), "v"(noise[6]), "v"(noise[7] >> 1), "v"(1.f));
 #endif
   return (even & 0x0F0F0F0Fu) | (odd & 0xF0F0F0F0u);
 }

@@ -43,11 +43,12 @@ struct QuantizeArgs {
 // through LDS, each in 64-byte runs; the scales through LDS, so that a block's rows are written
 // together. Tiles past the last row or column, up to the padding of the other form, write zeros.
 // Bound: HBM, 2 or 4 bytes read and half a byte written for each form an element; by chance, the hash and
-// the conversions too. us (and TB/s) of both forms, bfloat16: 8192 x 14336 77 (4.7), by chance 81; 8192 x
-// 4096 18.0 (5.7), 25; float32 8192 x 14336 133 (4.5), 14336 x 4096 by tiles 50 (5.9). Not kept: tiles
+// the conversions too. us (and TB/s) of both forms, bfloat16: 8192 x 14336 77 (4.7), by chance 88; 8192 x
+// 4096 18.0 (5.7), 28; float32 8192 x 14336 133 (4.5), 14336 x 4096 by tiles 50 (5.9). Not kept: tiles
 // of 256 x 128 or 256 x 256, whose runs are twice as long (79 and 81 us for the first, 34 and 42 where
-// 128 x 128 takes 25 by chance), and two rows of tiles in turn on one XCD (79). By chance with the
-// arithmetic of the definition, an integer addition below the place kept, 116.
+// 128 x 128 took 25 by chance), and two rows of tiles in turn on one XCD (79). By chance with small
+// 16-bit values cut at 2^-23 and not rounded there 80 and 25; with the definition's own arithmetic, an integer addition
+// below the place kept, 116.
 enum Rounding : int { kRows = 0, kTiles = 1, kStochastic = 2 };
 
 
@@ -59,9 +60,7 @@ struct Shared {
   __attribute__((aligned(16))) uint8_t row_bytes[4][kTile4], col_bytes[4][kTile4];
 };
 
-// Codes of a row or a column of a Square by chance, from each value's bits at the top of a word. 16-bit values need no rounding of
-// their own first: they are multiples of 2^-23 of the scale, but for those below 2^-12 of it, which the
-// noise's last 2^-10 alone could tell apart.
+// Codes of a row or a column of a Square by chance, from each value's bits at the top of a word.
 template <typename T, typename V, typename N>
 __device__ __forceinline__ uint32_t noisy_codes(uint32_t byte, V value, N noise) {
   const float scale = power(byte), inverse = inverse4(byte);
@@ -69,10 +68,10 @@ __device__ __forceinline__ uint32_t noisy_codes(uint32_t byte, V value, N noise)
   uint32_t bits[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    p[e >> 1][e & 1] = sizeof(T) == 4 ? scaled4(value(e), scale, inverse) : value(e);
+    p[e >> 1][e & 1] = scaled4<T>(value(e), scale, inverse);
     bits[e] = noise(e);
   }
-  return noisy8(p, bits, sizeof(T) == 4 ? 1.f : scale);
+  return noisy8(p, bits);
 }
 
 template <typename T, int ROUNDING>

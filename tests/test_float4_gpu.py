@@ -568,3 +568,55 @@ def test_a_matrix_past_32_bit_offsets_is_quantized_from_its_place() -> None:
     values, byte = oracle.quantize(x[tail], 1, bits)
     part = Float4Matrix(q.data[tail].clone(), torch.nn.functional.pad(q.scale[:, tail], (0, 4)).contiguous(), cols)
     assert torch.equal(part.values().cpu().double(), values)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_small_values_of_16_bits_are_rounded_before_the_noise(dtype) -> None:
+    """By chance a scaled magnitude below 1 is rounded to a multiple of 2^-23 first. Where that rounding decides:
+    values that go up to 0.5 rounded, and down to 0 if what is below 2^-23 were cut."""
+    rows, cols, seed = 2048, 2048, 3
+    bits = oracle.noise(seed, rows, cols)
+    least = 2 ** 22 - bits  # multiples of 2^-23 from which on the value goes up
+    x = torch.full((rows, cols), 6 * 2.0 ** 12)  # every block's scale is 2^12
+    near = least < 1024
+    x[near] = (least[near] - 0.25).float() * 2.0 ** (12 - 23)
+    x = x.to(dtype)
+    parts = x[near].double() * 2.0 ** (23 - 12)
+    decided = (parts.round() >= least[near]) & (parts.floor() < least[near])
+    assert int(decided.sum()) > 20
+    got = float4_quantize_both(x.cuda(), seed=seed)
+    _same(got[0], x, bits=bits)
+    _same(got[1], x.t(), bits=bits.t())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("seed", [None, 3])
+def test_quantization_of_16_bit_values_at_the_edges(dtype, seed) -> None:
+    """The largest and smallest values of a type, its subnormals alone and beside normal ones, ties, and
+    values that are not finite."""
+    most, least = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    step = least * torch.finfo(dtype).eps  # the smallest subnormal
+    x = torch.zeros(32, 256, dtype=torch.float64)
+    x[0, 0], x[0, 1], x[0, 2] = most, -most, most / 2
+    x[1] = torch.arange(256) % 128 * step
+    x[2, 0], x[2, 1:100] = -least, torch.arange(1, 100) * step
+    x[3, 0], x[3, 1] = step, -step
+    x[4, 0], x[4, 1:] = 6.0, torch.arange(1, 256) * step
+    x[5] = 2.0 ** -torch.arange(0, 256).clamp(max=140).double()
+    x[6, 0], x[6, 40], x[6, 41] = float("inf"), 2.0, -1.0
+    x[7, 5], x[7, 100] = float("nan"), -float("inf")
+    x[8, :32] = torch.arange(32) * 0.25
+    x[9] = least
+    x[10, 0], x[10, 1] = 7.0, 6.96875
+    x = x.to(dtype)
+    bits = None if seed is None else oracle.noise(seed, *x.shape)
+    got = float4_quantize_both(x.cuda(), seed=seed)
+    for q, source, noise in zip(got, (x, x.t()), (bits, None if bits is None else bits.t())):
+        values, byte = oracle.quantize(source, 1, noise)
+        assert torch.equal(q.scale[:byte.shape[0], :source.shape[0]].cpu().int(), byte.int())
+        now = q.values().cpu().double()
+        assert torch.equal(now.isnan(), values.isnan())
+        assert torch.equal(now.nan_to_num(), values.float().double().nan_to_num())
+    if seed is None:
+        alone = float4_quantize(x.cuda())
+        assert torch.equal(alone.data, got[0].data) and torch.equal(alone.scale[:, :32], got[0].scale[:, :32])
