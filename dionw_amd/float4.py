@@ -406,10 +406,19 @@ def float4_linear(x: Tensor, weight: Tensor | Float4Matrix, bias: Tensor | None 
 
 class Float4Linear(nn.Linear):
     """``nn.Linear`` whose products run in 4 bits (``float4_linear``); the parameters stay as
-    they are, so the layer trains with any optimizer of float weights."""
+    they are, so the layer trains with any optimizer of float weights.
+
+    Attributes:
+        seed: ``float4_linear``'s, None unless set. Recorded in a HIP graph, a layer without one (or
+            with a number) rounds its gradients by the recorded bits at every replay: set it to one
+            int64 on the GPU, which layers may share, and change that between replays. It is no
+            buffer: neither moved nor saved with the module.
+    """
+
+    seed: int | Tensor | None = None
 
     def forward(self, input: Tensor) -> Tensor:
-        return float4_linear(input, self.weight, self.bias)
+        return float4_linear(input, self.weight, self.bias, seed=self.seed)
 
     def quantized_weight(self) -> Float4Matrix:
         """The weight as the layer's products read it, to be kept for inference."""

@@ -282,3 +282,16 @@ def test_a_second_derivative_is_refused(calls) -> None:
         (dx,) = torch.autograd.grad(loss(float4_linear(x, w)), x, create_graph=True)
         with pytest.raises(RuntimeError, match="second time"):
             (dx.sum() + x.sum()).backward()
+
+
+def test_a_modules_seed_reaches_the_backward(calls) -> None:
+    x, layer, at = torch.ones(30, 200, requires_grad=True), Float4Linear(200, 50), torch.tensor([7])
+    assert layer.seed is None
+    for layer.seed in (5, at):
+        layer(x).sum().backward()
+    given = [(args[SEED], args[SEED_AT]) for name, args in calls if name.endswith("backward")]
+    assert given == [(5, None), (0, at.data_ptr())]
+    assert set(layer.state_dict()) == {"weight", "bias"} and not list(layer.buffers())
+    layer.seed = torch.tensor([7, 8])
+    with pytest.raises(ValueError, match="seed"):
+        layer(x)

@@ -509,6 +509,30 @@ def test_another_stream_and_a_graph() -> None:
     assert not torch.equal(seen[0], seen[1])
 
 
+def test_a_modules_seed_gives_a_replayed_graph_new_bits() -> None:
+    layer, x, dy = Float4Linear(300, 200).cuda(), _random(40, 300, 1).requires_grad_(), _random(40, 200, 2)
+    layer.seed = torch.tensor([3], device="cuda")
+
+    def train():
+        return torch.autograd.grad(layer(x), (x, layer.weight, layer.bias), dy)
+
+    first = train()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = train()
+    seen = [first]
+    for seed in (3, 4, 5, 4):
+        layer.seed.fill_(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, train()))
+        seen.append([t.clone() for t in out])
+    assert all(torch.equal(a, b) for a, b in zip(seen[0], seen[1]))
+    assert all(torch.equal(a, b) for a, b in zip(seen[2], seen[4]))
+    for i in (0, 1):  # db is a plain sum
+        assert not torch.equal(seen[1][i], seen[2][i]) and not torch.equal(seen[2][i], seen[3][i])
+
+
 def test_two_graphs_keep_their_scratch_apart() -> None:
     x, y = _random(100, 4096, 1, torch.bfloat16), _random(100, 4096, 2, torch.bfloat16)
     kept = float4_quantize(_random(512, 4096, 3), tiles=True)
