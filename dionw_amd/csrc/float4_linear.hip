@@ -74,7 +74,7 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
   __shared__ uint8_t x_bytes[W][16][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int G = lane >> 4, i16 = lane & 15;
-  const int n0 = blockIdx.x * 16 * R * P, token0 = blockIdx.y * 16, rows = min(16, g.m - token0);
+  const int n0 = blockIdx.x * 16 * R * P, rows = g.m;
   const uint8_t *w[P][R], *scale[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
   };
   // x as it comes, two rows a load: a lane holds 8 columns of row 2 j + lane / 32.
   const int upper = lane >> 5, eight = lane & 31;
-  const T* x = reinterpret_cast<const T*>(g.x) + token0 * g.x_ld + 8 * eight;
+  const T* x = reinterpret_cast<const T*>(g.x) + 8 * eight;
   Square<T> v;
   auto read_x = [&](int kt) {
     const int64_t at = (int64_t)kt * kDepth4, left = g.k - at - 8 * eight;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
     row o;
 #pragma unroll
     for (int r = 0; r < R; ++r) o[r] = (T)(s[r] + (g.bias ? g.bias[min(n + r, g.n - 1)] : 0.f));
-    T* y = reinterpret_cast<T*>(g.y) + (int64_t)(token0 + i16) * g.n + n;
+    T* y = reinterpret_cast<T*>(g.y) + (int64_t)i16 * g.n + n;
     if (n + R <= g.n) {
       *reinterpret_cast<anywhere*>(y) = o;
     } else {
@@ -223,12 +223,13 @@ __global__ __launch_bounds__(W * 64) void float4_few_kernel(FewArgs g) {
 // 24 / 41, 8192 x 4096 7.5 / 7.5 / 10.1 / 13.4, 14336 x 4096 11.0 / 9.4 / 10.6 / 13.7, 20480 x 4096 13.4 / 13.2 /
 // 15.7 / 14.3 / 27 (8 rows 17.1 / 15.6 / 17.3 / 14.9 / 28.6), 128256 x 4096 64 / 54 / 52.6 / 50.2 / 51.7 (8 rows 87 / 70 / 62 /
 // 55.3 / 53.2); float32: 65536 x 4096 48 / 31.5 / 29.4 / 28.3 / 29.2 (8 rows 70 / 44 / 36.8 / 31.8 / 31.8), 128256 x 4096
-// 91 / 56 / 53.5 / 55.0 / 53.2 (8 rows 135 / 84 / 70 / 63.6 / 56.2). The number of x's rows is not asked, so that a
-// row's sums do not depend on the rows beside it.
+// 91 / 56 / 53.5 / 55.0 / 53.2 (8 rows 135 / 84 / 70 / 63.6 / 56.2). The choice does not ask for the number of x's rows: of
+// those that come here, a row's sums do not depend on the rows beside it. (More of them take the tiles, which sum in an
+// order of their own.)
 template <typename T, int R, int P, int W, bool WHOLE>
 void launch_few(const FewArgs& g, int fragments, hipStream_t stream) {
   hipLaunchKernelGGL((float4_few_kernel<T, R, P, W, WHOLE>),
-                     dim3((unsigned)ceil_div(fragments, R * P), (unsigned)ceil_div(g.m, 16)), dim3(W * 64), 0, stream, g);
+                     dim3((unsigned)ceil_div(fragments, R * P)), dim3(W * 64), 0, stream, g);
 }
 template <typename T, bool WHOLE>
 int launch_few(const FewArgs& g, hipStream_t stream) {

@@ -449,6 +449,20 @@ def test_a_rows_output_does_not_depend_on_the_rows_beside_it(dtype) -> None:
     assert all(torch.equal(float4_linear(x[i:i + 1], kept), y[i:i + 1]) for i in range(16))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(16, 4096, 5104), (8, 4097, 5104), (8, 300, 5105), (8, 513, 16384), (16, 300, 16385),
+                                  (8, 4100, 16390), (16, 256, 66000), (8, 5000, 66000)], ids=str)
+def test_a_rows_output_does_not_depend_on_the_rows_beside_it_up_to_those_of_one_launch(size, dtype) -> None:
+    """The most rows that one launch serves, for each of the kernel's forms and on both sides of where they end."""
+    m, k, n = size
+    x, w = _random(m, k, 10, dtype, 0.5), _random(n, k, 11, spread=0.3)
+    kept = float4_quantize(w, tiles=True)
+    y = float4_linear(x, kept)
+    for rows in (1, 2, 5, m - 1):
+        assert torch.equal(float4_linear(x[:rows], kept), y[:rows])
+    assert torch.equal(float4_linear(x[m - 1:], kept), y[m - 1:])
+
+
 @pytest.mark.parametrize("rows", [3, 40])
 def test_a_tokens_nan_stays_its_own(rows) -> None:
     x, kept = _random(rows, 500, 1), float4_quantize(_random(99, 500, 2))
