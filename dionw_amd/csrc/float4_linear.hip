@@ -20,13 +20,20 @@ namespace {
 // this order, 45, from end to end 39); the smallest calls: launch and the latency of two dependent reads.
 constexpr int kFewFragments = 320, kManyFragments = 1024;  // of 16 rows of W, where the kernel's form changes
 int fragments_of(int64_t n) { return (int)((n + 15) / 16); }
-// Past 8 rows x costs the kernel as much as W where it is deep, or W's rows are in the middle: quantizing
-// first and the product on tiles is faster there. 16 rows, us, here and there: 4096 x 4096 7.5 / 11.1, 8192 x 4096
-// 11.2 / 11.2, 14336 x 4096 14.2 / 11.9, 28672 x 4096 16.5 / 19, 4096 x 14336 16.6 / 14.2, 16384 x 14336 40 / 27; 8 rows 8.9 /
-// 11.2 on 8192 x 4096, 11.0 / 12.0 on 14336 x 4096, 12.8 / 14.7 on 4096 x 14336, 33 / 34 on 16384 x 14336.
+// Past 8 rows a deep x costs the kernel as much as W: from some depth on, quantizing first and the product on
+// tiles is faster. That depth is 10000 where every workgroup has a CU to itself, less where some wait for a
+// second turn. Calls of 16 rows from Python on weights that no cache holds, us, here / there, bfloat16 (float32):
+//   4096 rows of W: 4096 columns 7.5 / 11.5, 6144 9.1 / 14.2, 8192 11.1 / 14.2 (13.2 / 14.2), 10240 12.9 / 14.3 (16.3 / 14.3)
+//   5104: 2048 7.5 / 11.5, 4096 10.3 / 11.5 (12.9 / 11.5), 6144 14.4 / 14.2
+//   8192: 2048 7.5 / 11.5, 4096 11.3 / 11.5 (12.1 / 11.5), 6144 15.5 / 14.3; 16384: 2048 8.3 / 11.5 (9.4 / 11.4), 4096 12.9 /
+//   12.0 (16.0 / 12.0)
+//   28672: 2048 9.8 / 13.6, 4096 16.4 / 18.8 (17.7 / 19.7), 5120 23.3 / 22.5; 128256: 2048 32 / 36, 4096 61 / 59 (61 / 63).
+// 8 rows: 8.9 / 11.2 on 8192 x 4096, 11.0 / 12.0 on 14336 x 4096, 12.8 / 14.7 on 4096 x 14336, 33 / 34 on 16384 x 14336.
 bool few_rows(int64_t m, int64_t n, int64_t k) {
-  const bool middle = fragments_of(n) >= kFewFragments && fragments_of(n) <= kManyFragments;
-  return k > 0 && (m <= 8 || (m <= 16 && k <= 4096 && !middle));
+  const int fragments = fragments_of(n);
+  const bool middle = fragments >= kFewFragments && fragments <= kManyFragments;
+  const int64_t deepest = fragments <= 256 ? 8192 : middle ? 2048 : 4096;
+  return k > 0 && (m <= 8 || (m <= 16 && k <= deepest));
 }
 
 struct FewArgs {

@@ -362,10 +362,10 @@ def float4_linear(x: Tensor, weight: Tensor | Float4Matrix, bias: Tensor | None 
     32 of the weight's gradient. Under ``torch.autocast`` x is cast to its type first, as for
     ``nn.Linear``; the weight and the bias stay as they are. ``weight`` is ``[out, in]``: a float
     tensor, quantized at every call (gradients flow to x, weight and bias, the weight's in its
-    own type), or a ``Float4Matrix`` for inference. From a ``Float4Matrix`` up to 8 rows (16 of at
-    most 4096 columns, but for 5105 to 16384 outputs) are served by one launch, in which a row's bits
-    do not depend on the rows beside it; more rows are summed in an order that their number chooses,
-    so that a row's last bits may change with it.
+    own type), or a ``Float4Matrix`` for inference. From a ``Float4Matrix`` up to 8 rows are served by
+    one launch (16 of up to 8192 columns for 4096 outputs or less, of up to 2048 for 5105 to 16384 outputs, of
+    up to 4096 for others), in which a row's bits do not depend on the rows beside it; more rows are
+    summed in an order that their number chooses, so that a row's last bits may change with it.
 
     ``seed`` chooses the random bits of the gradient's rounding (see ``float4_quantize``). Without
     one a number is drawn from torch's CPU generator at every call that records gradients, as

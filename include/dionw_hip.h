@@ -484,8 +484,8 @@ int dionw_float4_linear_backward(int32_t x_elem, const void* dy, int64_t dy_ld, 
 
 /*
  * The same y from a kept W: codes [n] rows with their scales [depth / 32][w_scale_ld]. Up to 8 rows
- * of x (16 of up to 4096 columns, but for 5105 to 16384 rows of W) are quantized by the product itself,
- * in one launch and no scratch.
+ * of x (16 of up to 8192 columns where W has 4096 rows or less, of up to 2048 where it has 5105 to 16384,
+ * of up to 4096 elsewhere) are quantized by the product itself, in one launch and no scratch.
  */
 size_t dionw_float4_linear_kept_scratch(int64_t m, int64_t n, int64_t k);
 int dionw_float4_linear_kept(int32_t x_elem, const void* x, int64_t x_ld, const void* w,

@@ -210,3 +210,14 @@ def test_a_forward_of_no_rows_needs_no_room_to_save(need_x, need_w) -> None:
     assert need_x or sizes[0] == 0
     _lib.call("dionw_float4_linear_forward", 1, None, 130, 2, 16, 130, None, 0, 50, 130, need_x, need_w, None,
               16 if sizes[0] else None, 16, sizes[1], None)
+
+
+def test_which_rows_one_launch_serves() -> None:
+    """Without scratch: up to 8 rows, and 16 up to the depth from which tiles are faster."""
+    scratch = _lib.library().dionw_float4_linear_kept_scratch
+    for n in (1, 4096, 4097, 5104, 5105, 16384, 16385, 128256):
+        assert scratch(1, n, 1 << 20) == scratch(8, n, 1 << 20) == 0
+        deepest = 8192 if n <= 4096 else 2048 if 5104 < n <= 16384 else 4096
+        for rows in (9, 16):
+            assert scratch(rows, n, deepest) == 0 and scratch(rows, n, deepest + 1) > 0
+        assert scratch(17, n, 32) > 0

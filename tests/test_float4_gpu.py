@@ -450,7 +450,7 @@ def test_a_rows_output_does_not_depend_on_the_rows_beside_it(dtype) -> None:
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("size", [(16, 4096, 5104), (8, 4097, 5104), (8, 300, 5105), (8, 513, 16384), (16, 300, 16385),
+@pytest.mark.parametrize("size", [(16, 8192, 4096), (16, 4096, 5104), (8, 4097, 5104), (16, 2048, 5105), (8, 2049, 16384), (16, 300, 16385),
                                   (8, 4100, 16390), (16, 256, 66000), (8, 5000, 66000)], ids=str)
 def test_a_rows_output_does_not_depend_on_the_rows_beside_it_up_to_those_of_one_launch(size, dtype) -> None:
     """The most rows that one launch serves, for each of the kernel's forms and on both sides of where they end."""
