@@ -33,6 +33,7 @@ from dionw_amd import _lib
 from dionw_amd._operands import (
     CODES,
     DTYPES,
+    call,
     check_unrecorded,
     check_vector,
     float_bias,
@@ -114,8 +115,8 @@ def _expand(q: Float8Matrix) -> Tensor:
     """The matrix as a product summed in float32 reads it: bfloat16 halves of the values."""
     rows, depth = q.data.shape
     out = torch.empty(rows, depth, dtype=torch.bfloat16, device=q.device)
-    _lib.call("dionw_float8_expand", q.data.data_ptr(), depth, q.scale.data_ptr(), q.scale.shape[1],
-              rows, depth, out.data_ptr(), depth, _lib.stream_handle(q.device))
+    call(q.device, "dionw_float8_expand", q.data.data_ptr(), depth, q.scale.data_ptr(), q.scale.shape[1],
+         rows, depth, out.data_ptr(), depth, _lib.stream_handle(q.device))
     return out
 
 
@@ -127,9 +128,8 @@ def _product(m: int, n: int, depth: int, a: tuple[int, int | None, int], b: tupl
     out = torch.empty(m, n, dtype=dtype, device=device)
     size = _lib.library().dionw_float8_gemm_workspace(expanded, m, n, depth)
     space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _lib.call("dionw_float8_gemm", expanded, m, n, depth, a[0], depth, a[1], a[2], b[0], depth, b[1],
-              b[2], _lib.ptr(bias), _lib.elem_code(dtype), out.data_ptr(), n, _lib.ptr(space), size,
-              stream)
+    call(device, "dionw_float8_gemm", expanded, m, n, depth, a[0], depth, a[1], a[2], b[0], depth, b[1],
+         b[2], _lib.ptr(bias), _lib.elem_code(dtype), out.data_ptr(), n, _lib.ptr(space), size, stream)
     return out
 
 
@@ -154,8 +154,8 @@ def _quantize(x: Tensor, tiles: bool, both: bool) -> tuple[Float8Matrix, Float8M
         return (None, 0, None, 0) if q is None else (
             q.data.data_ptr(), q.data.shape[1], q.scale.data_ptr(), q.scale.shape[1])
 
-    _lib.call("dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, pitch(x),
-              int(tiles), *place(by_row), *place(by_column), 0, None, stream)
+    call(x.device, "dionw_float8_quantize", _lib.elem_code(x.dtype), x.data_ptr(), m, n, pitch(x),
+         int(tiles), *place(by_row), *place(by_column), 0, None, stream)
     return by_row, by_column
 
 
@@ -237,9 +237,9 @@ def _forward(x: Tensor, weight: Tensor, bias: Tensor | None, need_x: bool, need_
     saved, scratch = _scratch(keep, device), _scratch(room, device)
     y = torch.empty(m, n, dtype=x.dtype, device=device)
     added = float_bias(bias, n, device)
-    _lib.call("dionw_float8_linear_forward", x_code, x.data_ptr(), pitch(x), w_code,
-              weight.data_ptr(), pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
-              y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
+    call(device, "dionw_float8_linear_forward", x_code, x.data_ptr(), pitch(x), w_code,
+         weight.data_ptr(), pitch(weight), _lib.ptr(added), m, n, k, need_x, need_w,
+         y.data_ptr(), _lib.ptr(saved), _lib.ptr(scratch), room, stream)
     return y, saved, backward_room
 
 
@@ -266,6 +266,7 @@ class _Linear(torch.autograd.Function):
         dx = torch.empty(m, k, dtype=ctx.dtypes[0], device=device) if need_x else None
         dw = torch.empty(n, k, dtype=ctx.dtypes[1], device=device) if need_w else None
         db = torch.empty(n, dtype=ctx.bias_dtype, device=device) if need_b else None
+        # The engine runs this on x's device, and on the forward's stream.
         _lib.call("dionw_float8_linear_backward", ctx.codes[0], dy.data_ptr(), pitch(dy), ctx.codes[1],
                   m, n, k, need_x, need_w, _lib.ptr(saved), _lib.ptr(dx), _lib.ptr(dw),
                   _lib.elem_code(ctx.bias_dtype) if need_b else 0, _lib.ptr(db), _lib.ptr(scratch),
@@ -304,9 +305,9 @@ def _kept_linear(x: Tensor, weight: Float8Matrix, bias: Tensor | None) -> Tensor
     room = _kept_scratch(code, m, n, k)
     scratch = _scratch(room, device) if room else None
     y = x.new_empty(out)
-    _lib.call("dionw_float8_linear_kept", code, x.data_ptr(), ld, data.data_ptr(), depth,
-              scale.data_ptr(), scale.shape[1], None if bias is None else bias.data_ptr(), m, n, k,
-              y.data_ptr(), _lib.ptr(scratch), room, stream)
+    call(device, "dionw_float8_linear_kept", code, x.data_ptr(), ld, data.data_ptr(), depth,
+         scale.data_ptr(), scale.shape[1], None if bias is None else bias.data_ptr(), m, n, k,
+         y.data_ptr(), _lib.ptr(scratch), room, stream)
     return y
 
 
