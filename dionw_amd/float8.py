@@ -27,7 +27,6 @@ from typing import Any, Final
 import torch
 from torch import Tensor, nn
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from dionw_amd import _lib
 from dionw_amd._operands import (
@@ -38,6 +37,7 @@ from dionw_amd._operands import (
     check_vector,
     float_bias,
     function_modes,
+    once_differentiable,
     pitch,
     readable,
     scratch as _scratch,

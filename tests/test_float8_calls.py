@@ -228,3 +228,12 @@ def test_autocast_leaves_other_types_refused(autocast, calls) -> None:
             with pytest.raises(ValueError):
                 float8_linear(torch.ones(3, 200, dtype=dtype), w)
     assert not calls
+
+
+def test_a_second_derivative_is_refused(calls) -> None:
+    """Also where the incoming gradient is a constant: the gradient depends on the inputs all the same."""
+    x, w = torch.ones(3, 200, requires_grad=True), torch.ones(5, 200, requires_grad=True)
+    for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+        (dx,) = torch.autograd.grad(loss(float8_linear(x, w)), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second time"):
+            (dx.sum() + x.sum()).backward()
