@@ -94,8 +94,10 @@ __device__ __forceinline__ float row_sum(float v, float* sums) {
 // ---- forward ------------------------------------------------------------------------------
 //
 // LANES threads a row, K chunks of 8 columns a thread, `LANES * 8 * K` columns at most.
-// Bound: HBM, x read and y (or half a byte an element) written: 8192 x 4096 bfloat16 23 us (5.8 TB/s),
-// float32 41 (6.5), to 4 bits 23.
+// Bound: HBM, x read and y written: 8192 x 4096 bfloat16 24 us (5.6 TB/s); float32 41 again and again, its x then
+// from the Infinity Cache, 59 (4.5) in a training pass. To 4 bits not HBM: 26 us for 85 MB (3.3 TB/s; quantizing such
+// rows alone takes 13.8). A workgroup takes one row, meets twice with no other row of its own on its way, and reads
+// 32 KB of parameters beside 8 KB of x. 8192 x 768 float32 10, 2048 x 16384 bfloat16 32.
 
 // Workgroup b's first row. 4-bit output: the rows whose scales share a line of memory run on one XCD
 // (the hardware deals workgroup b to XCD b % 8), whose L2 then writes the line once.
@@ -366,7 +368,10 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_grad_kernel(GradArgs g
   write(db, g.db);
 }
 
-// Rows past the registers: a workgroup a row for dx, which reads x and dy twice.
+// Rows past the registers: a workgroup a row for dx, which reads x and dy twice; the column sums read them
+// again. dx, column sums and their join, us: 2048 x 12288 bfloat16 33 + 16 + 4, 2048 x 16384 44 + 25 + 4 (float32 99 +
+// 55 + 5), 2048 x 20000 58 + 28 + 5: 2.7 TB/s of the 201 MB that 2048 x 16384 has to read and write, where rows of
+// 8192 columns, read once, take 24 + 4 for half of it.
 template <typename T>
 __global__ __launch_bounds__(kWide) void norm_grad_wide_kernel(GradArgs g) {
   __shared__ float sums[2][kWide / kWave];

@@ -262,8 +262,9 @@ __device__ __forceinline__ void load_bias(const ProductArgs& g, int q, float (&b
 // same way, one load of a wave for 256 rows, and are read a stage ahead. Whole tiles store from
 // registers, 64 bytes of 16 rows an instruction.
 // Bound: the board's power (8 bits: 8192^3 395 us, 2785 TFLOP/s, 366 sustained at 1387 W of 1400 and 1.8 GHz,
-// the matrix pipe 77% busy; 4 bits: 228 us, 4820 TFLOP/s, 60% busy at 1.7 GHz, on constant operands 174;
-// the instruction alone on random registers 7200; expanded 14336 x 4096 x 8192 720 us, 1336, at 1400 W and 2.05 GHz, 68%);
+// the matrix pipe 77% busy; 4 bits: 228 us, 4820 TFLOP/s, 237 sustained at 1396 W and 1.7 GHz, 61% busy; on constant
+// operands 169 at 1324 W and 2.36 GHz, on zeros 167 at 1164 W, where neither power nor the pipe (66%) is the bound;
+// the instruction alone on random registers 7200 TFLOP/s; expanded 14336 x 4096 x 8192 720 us, 1336, at 1400 W and 2.05 GHz, 68%);
 // at few stages the first loads and the stores (plan_time; 8192 x 2304 x 768 24 us, 20%). Stores are
 // 14% of 4-bit 8192 x 14336 x 4096 (229 us, 197 without them): they wait for memory. Not kept there: stores
 // past the caches (241), through LDS in whole rows (232), and workgroups that take one tile after another
@@ -821,9 +822,10 @@ struct Plan {
 // 4 bits, whose stages are twice as deep: 8192 x 14336 x 4096 232 / 260, 8192 x 4096 x 14336 192 / 233 /
 // 642, 4096^3 35 / 40 / 116, 4096 x 14336 x 4096 128 / 133 / 401, 5000^3 74 / 77 / 214; 8192 x 2304 x 768
 // 24 / 17 / 30, 3001 x 1408 x 2048 19 / 13 / 25, 1024 x 4096 x 4096 26 / 13 / 31; 256 x 4096 x 4096 25 / 12 /
-// 8.7, 64 x 4096 x 4096 27 / 13 / 8.4. Split: 100 x 4096 x 14336 31 whole on 128 tiles, 17 in 8 there, 16 in
-// 2 on 64; 700 x 700 x 16384 24 whole on 64 tiles, 18 in 2. Either rule takes the fastest on nearly all of
-// them, and none that is 5% slower.
+// 8.7, 64 x 4096 x 4096 27 / 13 / 8.4. Split: 100 x 4096 x 14336 29 whole on 128 tiles, 16.5 in 7
+// there (chosen) and in 2 on 64; 700 x 700 x 16384 24.5 whole on 64 tiles, 18.5 in 2, 19.1 in 6 on 128 (chosen);
+// 130 x 770 x 6144 11.2 whole on 64 tiles, 10.2 in 3 (chosen), 9.7 in 4 or 6. Either rule takes the fastest on
+// nearly all of them, and on these none that is more than 5% slower.
 struct Cost {
   double stage[3], fixed[3];
 };
