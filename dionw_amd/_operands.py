@@ -58,25 +58,38 @@ def pitch(x: Tensor) -> int:
 
 
 def once_differentiable(backward: Callable[..., Any]) -> Callable[..., Any]:
-    """A backward pass whose gradients may not be differentiated again, whatever they depend on:
-    where a graph of it is asked for, they raise once one is. (torch's own decorator lets them pass as
-    constants where the incoming gradient is one, and costs a call on every pass.)"""
+    """A backward pass whose gradients may not be differentiated again, whatever they depend on and
+    with respect to whatever: where a graph of it is asked for, they raise once one is. (torch's own
+    decorator lets them pass as constants where the incoming gradient is one, or where
+    ``torch.autograd.grad`` asks for some tensors alone, and costs a call on every pass.)
 
-    def run(ctx: Any, *gradients: Tensor) -> Any:
+    What refuses stands between the gradients and the incoming ones and the saved tensors, so that one
+    of the latter has to depend on each input: the inputs themselves, or an empty output of the
+    forward (``tie``)."""
+
+    def run(ctx: Any, *gradients: Tensor | None) -> Any:
         if not torch.is_grad_enabled():
             return backward(ctx, *gradients)
         with torch.no_grad():
             found = backward(ctx, *gradients)
         places = [i for i, g in enumerate(found) if g is not None]
+        tied = [t for t in (*gradients, *ctx.saved_tensors) if t is not None and t.requires_grad]
         refuse = torch._C._functions.DelayedError(
-            b"the gradients of dionw_amd's operators are not differentiable a second time", len(places))
-        refusing = refuse(*[found[i].detach().requires_grad_() for i in places])
+            b"the gradients of dionw_amd's operators are not differentiable a second time",
+            len(places) + len(tied))
+        refusing = refuse(*[found[i].detach().requires_grad_() for i in places], *tied)
         found = list(found)
         for i, g in zip(places, refusing if isinstance(refusing, tuple) else (refusing,)):
             found[i] = g
         return tuple(found)
 
     return run
+
+
+def tie(y: Tensor) -> Tensor:
+    """An output of no elements beside y, saved for the backward: it depends on the inputs and keeps
+    none of them."""
+    return y.new_empty(0)
 
 
 def check_vector(name: str, v: Tensor | None, n: int, device: torch.device) -> None:

@@ -39,6 +39,7 @@ from dionw_amd._operands import (
     pitch,
     readable,
     scratch as _scratch,
+    tie,
     watched,
 )
 
@@ -269,7 +270,8 @@ class _Linear(torch.autograd.Function):
     """y = x W^T + b; dx = dy W, dW = dy^T x, db = the sum of dy over the rows."""
 
     @staticmethod
-    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None, seed: int | Tensor | None) -> Tensor:
+    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None,
+                seed: int | Tensor | None) -> tuple[Tensor, Tensor]:
         # What the backward needs is worked out here: it runs on a thread of torch's own, whose caches
         # hold none of this.
         need_x, need_w, need_b, _ = ctx.needs_input_grad
@@ -282,17 +284,21 @@ class _Linear(torch.autograd.Function):
         ctx.sizes, ctx.room = (x.shape[0], *weight.shape), room
         ctx.dtypes = x.dtype, weight.dtype, bias.dtype if need_b else torch.float32
         ctx.device = x.device
-        ctx.save_for_backward(saved)
-        return y
+        tied = tie(y)
+        ctx.save_for_backward(saved, tied)
+        ctx.set_materialize_grads(False)
+        return y, tied
 
     @staticmethod
     @once_differentiable
-    def backward(ctx: Any, dy: Tensor) -> tuple[Tensor | None, ...]:
+    def backward(ctx: Any, dy: Tensor | None, _: None) -> tuple[Tensor | None, ...]:
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         m, n, k = ctx.sizes
         x_dtype, w_dtype, b_dtype = ctx.dtypes
         device, room = ctx.device, ctx.room
-        (saved,) = ctx.saved_tensors
+        saved, tied = ctx.saved_tensors
+        if dy is None:
+            dy = tied.new_zeros(m, n)
         ld = n
         if not dy.is_contiguous():
             dy = readable(dy)
@@ -401,7 +407,7 @@ def float4_linear(x: Tensor, weight: Tensor | Float4Matrix, bias: Tensor | None 
     # Asked here: inside the function gradients are off, and what it is told of its inputs' needs
     # does not know whether they were on.
     if torch.is_grad_enabled():
-        y = _Linear.apply(flat, weight, bias, seed)
+        y, _ = _Linear.apply(flat, weight, bias, seed)
     else:
         y = _forward(flat, weight, bias, False, False, False)[0]
     return y if len(shape) == 2 else y.view(*shape[:-1], weight.shape[0])

@@ -41,6 +41,7 @@ from dionw_amd._operands import (
     pitch,
     readable,
     scratch as _scratch,
+    tie,
     tracing,
 )
 
@@ -247,21 +248,23 @@ class _Linear(torch.autograd.Function):
     """y = x W^T + b; dx = dy W, dW = dy^T x, db = the sum of dy over the rows."""
 
     @staticmethod
-    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
+    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> tuple[Tensor, Tensor]:
         y, saved, ctx.room = _forward(x, weight, bias, *ctx.needs_input_grad)
         ctx.codes = CODES[x.dtype], CODES[weight.dtype]
         ctx.sizes, ctx.dtypes = (x.shape[0], *weight.shape), (x.dtype, weight.dtype)
         ctx.bias_dtype = bias.dtype if ctx.needs_input_grad[2] else None
-        ctx.save_for_backward(*([] if saved is None else [saved]))
-        return y
+        tied = tie(y)
+        ctx.save_for_backward(saved, tied)
+        ctx.set_materialize_grads(False)
+        return y, tied
 
     @staticmethod
     @once_differentiable
-    def backward(ctx: Any, dy: Tensor) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    def backward(ctx: Any, dy: Tensor | None, _: None) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
         need_x, need_w, need_b = ctx.needs_input_grad
         m, n, k = ctx.sizes
-        dy, device = _readable(dy), dy.device
-        saved = ctx.saved_tensors[0] if ctx.saved_tensors else None
+        saved, tied = ctx.saved_tensors
+        dy, device = tied.new_zeros(m, n) if dy is None else _readable(dy), tied.device
         scratch = _scratch(ctx.room, device)
         dx = torch.empty(m, k, dtype=ctx.dtypes[0], device=device) if need_x else None
         dw = torch.empty(n, k, dtype=ctx.dtypes[1], device=device) if need_w else None
@@ -345,7 +348,7 @@ def float8_linear(x: Tensor, weight: Tensor | Float8Matrix, bias: Tensor | None 
     # Asked here: inside the function gradients are off, and what it is told of its inputs' needs
     # does not know whether they were on.
     if torch.is_grad_enabled():
-        y = _Linear.apply(flat, weight, bias)
+        y, _ = _Linear.apply(flat, weight, bias)
     else:
         y = _forward(flat, weight, bias, False, False, False)[0]
     return y if len(shape) == 2 else y.view(*shape[:-1], weight.shape[0])

@@ -7,6 +7,7 @@ GPU ones would.
 from __future__ import annotations
 
 import gc
+import weakref
 from collections.abc import Callable, Iterator
 from typing import Any
 
@@ -295,3 +296,65 @@ def test_a_modules_seed_reaches_the_backward(calls) -> None:
     layer.seed = torch.tensor([7, 8])
     with pytest.raises(ValueError, match="seed"):
         layer(x)
+
+
+@pytest.mark.parametrize("trained", ["x", "weight", "both"])
+def test_a_second_derivative_is_refused_with_respect_to_any_tensor(trained, calls) -> None:
+    """Also where only some tensors' gradients are asked for, an intermediate one's among them."""
+    for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+        x, w = (torch.ones(s, 200, requires_grad=trained in (name, "both")) for s, name in ((3, "x"), (5, "weight")))
+        args = [t * 2 if t.requires_grad else t for t in (x, w)]
+        first = [t for t in args if t.requires_grad]
+        grads = torch.autograd.grad(loss(float4_linear(*args)), first, create_graph=True)
+        for asked in [*first, *(t for t in (x, w) if t.requires_grad)]:
+            with pytest.raises(RuntimeError, match="second time"):
+                torch.autograd.grad(sum(t.sum() for t in (*grads, *first)), asked, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.functional.hessian(lambda t: float4_linear(t, w.detach()).square().sum(), torch.ones(3, 200))
+
+
+def test_a_graph_of_gradients_that_nobody_differentiates_is_served(calls) -> None:
+    x, w = torch.ones(3, 200, requires_grad=True), torch.ones(5, 200, requires_grad=True)
+    y = float4_linear(x, w)
+    torch.autograd.grad(y.sum(), (x, w), create_graph=True)
+    assert len(calls) == 2
+    torch.autograd.grad(y.square().sum(), (x, w))
+    assert len(calls) == 3
+
+
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, dy):
+        return None
+
+
+def test_a_gradient_that_does_not_come_counts_as_zeros(calls) -> None:
+    x, w = torch.ones(3, 200, requires_grad=True), torch.ones(5, 200, requires_grad=True)
+    dx, dw = torch.autograd.grad(_NoGradient.apply(float4_linear(x, w)).sum(), (x, w))
+    assert dx.shape == x.shape and dw.shape == w.shape and len(calls) == 2
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_checkpoints_run_the_forward_again(reentrant, calls) -> None:
+    x, w = torch.ones(3, 200, requires_grad=True), torch.ones(5, 200, requires_grad=True)
+    y = torch.utils.checkpoint.checkpoint(lambda t: float4_linear(t, w), x, use_reentrant=reentrant)
+    y.sum().backward()
+    assert len(calls) == 3 and x.grad is not None and w.grad is not None
+
+
+def test_a_pass_is_freed_when_its_output_is(calls) -> None:
+    """What the backward keeps holds no cycle: nothing waits for the collector."""
+    x, w = torch.ones(3, 200, requires_grad=True), torch.ones(5, 200, requires_grad=True)
+    gc.collect()
+    gc.disable()
+    try:
+        y = float4_linear(x, w)
+        node = weakref.ref(y.grad_fn)
+        del y
+        assert node() is None
+    finally:
+        gc.enable()

@@ -150,3 +150,19 @@ def test_a_second_derivative_is_refused(calls) -> None:
         (dx,) = torch.autograd.grad(loss(layer_norm(x)), x, create_graph=True)
         with pytest.raises(RuntimeError, match="second time"):
             (dx.sum() + x.sum()).backward()
+
+
+@pytest.mark.parametrize("trained", ["x", "weight", "both"])
+def test_a_second_derivative_is_refused_with_respect_to_any_tensor(trained, calls) -> None:
+    """Also where only some tensors' gradients are asked for, an intermediate one's among them."""
+    for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+        x = torch.ones(3, 200, requires_grad=trained != "weight")
+        w, b = torch.ones(200, requires_grad=trained != "x"), torch.ones(200, requires_grad=True)
+        args = [t * 2 if t.requires_grad else t for t in (x, w, b)]
+        first = [t for t in args[:2] if t.requires_grad]
+        grads = torch.autograd.grad(loss(layer_norm(*args)), first, create_graph=True)
+        for asked in [*first, *(t for t in (x, w) if t.requires_grad)]:
+            with pytest.raises(RuntimeError, match="second time"):
+                torch.autograd.grad(sum(t.sum() for t in (*grads, *first)), asked, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.functional.hessian(lambda t: layer_norm(t).square().sum(), torch.ones(3, 200))
